@@ -22,11 +22,43 @@
 
 #include "kv_hip_common.h"
 #include "kv_host_calls.h"
+#include "kv_host_wait.h"
 #include "kv_launch.h"
 #include "musa_aiter_kv_hip.h"
 
 using kvhip::PagedTileParams;
 using kvhip::RowCopyParams;
+
+namespace kvhip {
+
+// Nothing but verdicts is ever written
+// to these words, so a word that carries the stamp is this call's.  The words
+// arrive as the checking kernel runs, so polling them returns sooner than a
+// stream synchronisation; a kernel that has not run after 0.2 s (the stream
+// busy with earlier work) is waited for by the synchronisation.
+hipError_t await_verdict(const int64_t* report, int64_t words, int64_t stamp, hipStream_t stream, bool* refused) {
+  const auto deadline = std::chrono::steady_clock::now() + std::chrono::milliseconds(200);
+  *refused = false;
+  bool synced = false;
+  for (int64_t w = 0; w < words;) {
+    const int64_t v = __atomic_load_n(&report[w], __ATOMIC_ACQUIRE);
+    if ((v >> 1) == stamp) {
+      *refused = *refused || (v & 1) != 0;
+      ++w;
+    } else if (synced) {
+      return hipErrorUnknown;  // the kernel has ended without its verdict
+    } else if (std::chrono::steady_clock::now() > deadline) {
+      const hipError_t err = hipStreamSynchronize(stream);
+      if (err != hipSuccess) return err;
+      synced = true;
+    } else {
+      __builtin_ia32_pause();
+    }
+  }
+  return hipSuccess;
+}
+
+}  // namespace kvhip
 
 // Claim tags of musa_aiter_hip_paged_tiles_noalloc: one uint64 per destination
 // slot of the caches (16 MiB on every device the library runs on, held until
@@ -370,34 +402,6 @@ int paged_tiles(int scatter, int codec, int cache_elt, int lin_elt, int lin_dtyp
   return kvhip::launch_paged_tiles(p, stream);
 }
 
-// Waits until each of `words` verdict words carries `stamp`; *refused tells
-// whether any of them refuses the call.  Nothing but verdicts is ever written
-// to these words, so a word that carries the stamp is this call's.  The words
-// arrive as the checking kernel runs, so polling them returns sooner than a
-// stream synchronisation; a kernel that has not run after 0.2 s (the stream
-// busy with earlier work) is waited for by the synchronisation.
-hipError_t await_verdict(const int64_t* report, int64_t words, int64_t stamp, hipStream_t stream, bool* refused) {
-  const auto deadline = std::chrono::steady_clock::now() + std::chrono::milliseconds(200);
-  *refused = false;
-  bool synced = false;
-  for (int64_t w = 0; w < words;) {
-    const int64_t v = __atomic_load_n(&report[w], __ATOMIC_ACQUIRE);
-    if ((v >> 1) == stamp) {
-      *refused = *refused || (v & 1) != 0;
-      ++w;
-    } else if (synced) {
-      return hipErrorUnknown;  // the kernel has ended without its verdict
-    } else if (std::chrono::steady_clock::now() > deadline) {
-      const hipError_t err = hipStreamSynchronize(stream);
-      if (err != hipSuccess) return err;
-      synced = true;
-    } else {
-      __builtin_ia32_pause();
-    }
-  }
-  return hipSuccess;
-}
-
 // Slots checked by one workgroup of the check kernel (more, once the report
 // words run out): four loads per thread.
 constexpr int64_t kCheckPerGroup = 1024;
@@ -439,7 +443,7 @@ int paged_tiles_checked(const musa_aiter_hip_paged_tiles_call& c, hipStream_t st
     p.check.report = c.report;
     err = kvhip::launch_paged_tiles(p, stream);
     if (err == hipSuccess) {
-      err = await_verdict(c.report, 1, c.stamp, stream, &refused);
+      err = kvhip::await_verdict(c.report, 1, c.stamp, stream, &refused);
       return err != hipSuccess ? err : refused ? MUSA_AITER_HIP_REFUSED : 0;
     }
     if (err != hipErrorNotSupported) return err;
@@ -453,7 +457,7 @@ int paged_tiles_checked(const musa_aiter_hip_paged_tiles_call& c, hipStream_t st
     p.check.words = shares < c.report_words ? shares : c.report_words;
     err = kvhip::launch_paged_tiles(p, stream);
     if (err == hipSuccess) {
-      err = await_verdict(c.report, p.check.words, c.stamp, stream, &refused);
+      err = kvhip::await_verdict(c.report, p.check.words, c.stamp, stream, &refused);
       return err != hipSuccess ? err : refused ? MUSA_AITER_HIP_REFUSED : 0;
     }
     if (err != hipErrorNotSupported) return err;
@@ -486,7 +490,7 @@ int paged_tiles_checked(const musa_aiter_hip_paged_tiles_call& c, hipStream_t st
   if (err != hipSuccess) return err;
   p.check.guard = c.guard;
   const hipError_t moved = kvhip::launch_paged_tiles(p, stream);
-  err = await_verdict(c.report, groups, c.stamp, stream, &refused);
+  err = kvhip::await_verdict(c.report, groups, c.stamp, stream, &refused);
   if (err != hipSuccess || refused) return err != hipSuccess ? err : MUSA_AITER_HIP_REFUSED;
   return moved;
 }
@@ -820,7 +824,7 @@ int musa_aiter_hip_block_tables_check(const int64_t* block_tables, const int64_t
                                              values, stamp, groups, as_stream(stream));
   if (err != hipSuccess) return err;
   bool refused = false;
-  err = await_verdict(report, groups, stamp, as_stream(stream), &refused);
+  err = kvhip::await_verdict(report, groups, stamp, as_stream(stream), &refused);
   if (err != hipSuccess) return err;
   out[0] = values[0];
   out[1] = values[1];
@@ -1550,7 +1554,7 @@ int musa_aiter_hip_copy_rows_paged_checked(const musa_aiter_hip_copy_rows_paged_
   p.check = kvhip::CallCheck{nullptr, c.guard, c.stamp, 0};
   const hipError_t moved = kvhip::launch_row_copy(p, as_stream(stream));
   bool refused = false;
-  err = await_verdict(c.report, groups, c.stamp, as_stream(stream), &refused);
+  err = kvhip::await_verdict(c.report, groups, c.stamp, as_stream(stream), &refused);
   if (err != hipSuccess || refused) return err != hipSuccess ? static_cast<int>(err) : MUSA_AITER_HIP_REFUSED;
   return moved;
 }

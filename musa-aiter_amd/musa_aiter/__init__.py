@@ -4,7 +4,9 @@ Importing this package gives the reference's KV transfer names (paged <->
 linear, merged, FP8 quant-store / dequant-gather, MLA flat rows, DSV4 byte
 rows, LMCache / SGLang-MP converters, LMCache host <-> device copy batches,
 SGLang HiCache transfers, layout descriptors) backed by hand-written gfx950 HIP
-kernels in ``_lib/libmusa_aiter_kv_hip.so``.
+kernels in ``_lib/libmusa_aiter_kv_hip.so``, and what serving from such caches
+needs next to them: FP8 caches with one scale per block and head (store and
+attention) and the bookkeeping of pages.
 """
 
 from musa_aiter.version import __version__, REFERENCE_API_VERSION
@@ -83,6 +85,13 @@ from musa_aiter.ops.kv_transfer import (
     native_fp8_kv_cache_abi_version,
     native_kv_transfer_abi_version,
     reset_kv_transfer_stats,
+)
+from musa_aiter.ops.kv_block_cache import kv_linear_to_paged_fp8_block, kv_paged_attention_fp8
+from musa_aiter.ops.kv_pages import (
+    kv_compact_paged_blocks,
+    kv_extend_paged_sequences,
+    kv_fork_paged_sequences,
+    kv_free_paged_sequences,
 )
 from musa_aiter.ops.lmcache_kv_transfer import (
     clear_native_lmcache_kv_transfer_cache,

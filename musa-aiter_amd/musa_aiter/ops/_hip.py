@@ -130,6 +130,16 @@ _SIGNATURES: dict[str, list] = {
                                        _c_void_p, _i64, _c_void_p],
     # (encoded, numel, table, table_len, elem_bytes, output, max_code, stream)
     "musa_aiter_hip_cachegen_decode": [_c_void_p, _i64, _c_void_p, _i64, _i32, _c_void_p, _c_void_p, _c_void_p],
+    # Operators on paged caches that are not copies (musa_aiter_kv_serving.h): packed call, stream.
+    "musa_aiter_hip_block_store": [ctypes.c_char_p, _c_void_p],
+    "musa_aiter_hip_attention": [ctypes.c_char_p, _c_void_p],
+    "musa_aiter_hip_attention_splits": [ctypes.c_char_p, _i64],
+    "musa_aiter_hip_attention_workspace": [ctypes.c_char_p],
+    "musa_aiter_hip_pages_free": [ctypes.c_char_p, _c_void_p],
+    "musa_aiter_hip_pages_fork": [ctypes.c_char_p, _c_void_p],
+    "musa_aiter_hip_pages_extend": [ctypes.c_char_p, _c_void_p],
+    "musa_aiter_hip_pages_compact": [ctypes.c_char_p, _c_void_p],
+    "musa_aiter_hip_pages_workspace": [ctypes.c_char_p, _i64],
 }
 
 _RESTYPES = {
@@ -138,6 +148,9 @@ _RESTYPES = {
     "musa_aiter_hip_cachegen_workspace_bytes": ctypes.c_int64,
     "musa_aiter_hip_graph_claim_arrays": ctypes.c_int64,
     "musa_aiter_hip_allocated_bytes": ctypes.c_int64,
+    "musa_aiter_hip_attention_splits": ctypes.c_int64,
+    "musa_aiter_hip_attention_workspace": ctypes.c_int64,
+    "musa_aiter_hip_pages_workspace": ctypes.c_int64,
 }
 
 _lock = threading.Lock()
@@ -840,4 +853,104 @@ def cachegen_decode(*, op: str, codes: torch.Tensor, table: torch.Tensor, out: t
             ptr(codes), int(codes.numel()), ptr(table), int(table.numel()), int(table.element_size()),
             ptr(out), ptr(max_code), stream_ptr(device),
         )
+    check(rc, op)
+
+
+# ----- operators on paged caches that are not copies (include/musa_aiter_kv_serving.h) ------------
+
+# musa_aiter_hip_block_store_call: linear, cache and scale pairs, slots, claims, report, guard, stamp, report words,
+# six sizes, linear strides, block and layer strides, codec and type.
+_BLOCK_STORE_CALL = struct.Struct("<6Q4Q2q6q2q4q2i")
+_BLOCK_STORE_SCAN = 256  # tokens up to which the kernel needs no claim tags
+
+
+def block_store(*, op: str, device: torch.device, linear, caches, scales, slots: torch.Tensor, sizes, strides,
+                block_strides, layer_strides, codec: int, lin_dtype: int) -> bool:
+    """The block-scaled FP8 store; False means that a slot lay past the caches and nothing was stored.
+    Captured calls are not checked: they skip such slots."""
+    with on_device(device):
+        stream = stream_ptr(device)
+        key = _stream_key(device, stream)
+        capturing = torch.cuda.is_current_stream_capturing()
+        with stream_lock(key):
+            claims, keep = 0, None
+            if sizes[1] > _BLOCK_STORE_SCAN:
+                claims, keep = claims_for(device, key, sizes[2] * sizes[5])
+            report = guard = stamp = 0
+            if not capturing:
+                checks = _check_set(device, key[1], key)
+                stamp = checks.stamp = next(_stamps)
+                report, guard = checks.report_ptr, checks.guard_ptr
+            call = _BLOCK_STORE_CALL.pack(
+                linear[0].data_ptr(), linear[1].data_ptr(), caches[0].data_ptr(), caches[1].data_ptr(),
+                scales[0].data_ptr(), scales[1].data_ptr(), slots.data_ptr(), claims, report, guard, stamp,
+                _REPORT_WORDS, *sizes, *strides, *block_strides, *layer_strides, codec, lin_dtype)
+            rc = fn("musa_aiter_hip_block_store")(call, stream)
+            del keep
+    if rc == _REFUSED:
+        return False
+    check(rc, op)
+    return True
+
+
+# musa_aiter_hip_attention_call: query, out, lse, caches, scales, tables, lens, starts, workspace, its bytes, eight
+# sizes, query strides, block strides, scale strides, table stride, window, splits, softmax scale, six flags.
+_ATTENTION_CALL = struct.Struct("<11Qq8q2q2q4q3qd6i")
+_ATTENTION_WORKSPACE = struct.Struct("<Qq")  # the workspace fields, behind ten pointers
+_ATTENTION_WORKSPACE_AT = 80
+_ATTENTION_SPLITS_AT = 80 + 16 + 8 * (8 + 2 + 2 + 4 + 2)
+
+
+def attention(*, op: str, query: torch.Tensor, out: torch.Tensor, lse: torch.Tensor | None, caches, scales,
+              tables: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor | None, sizes, window: int,
+              softmax_scale: float, longest: int, dtype: int, codec: int, fill_rows: bool) -> None:
+    """Attention over a block-scaled FP8 cache; the parts' workspace comes from torch's caching allocator."""
+    if sizes[0] == 0:
+        return
+    device = query.device
+    ks, vs = scales
+    call = bytearray(_ATTENTION_CALL.pack(
+        query.data_ptr(), out.data_ptr(), _data(lse), caches[0].data_ptr(), caches[1].data_ptr(), ks.data_ptr(),
+        vs.data_ptr(), tables.data_ptr(), lens.data_ptr(), _data(starts), 0, 0, *sizes, query.stride(0),
+        query.stride(1), caches[0].stride(0), caches[1].stride(0), ks.stride(0), vs.stride(0), ks.stride(1),
+        vs.stride(1), tables.stride(0), window, 1, softmax_scale, dtype, codec, tables.dtype is torch.int64,
+        lens.dtype is torch.int64, starts is not None and starts.dtype is torch.int64, fill_rows))
+    with on_device(device):
+        workspace = None
+        splits = fn("musa_aiter_hip_attention_splits")(bytes(call), longest)
+        if splits > 1:
+            struct.pack_into("<q", call, _ATTENTION_SPLITS_AT, splits)
+            size = fn("musa_aiter_hip_attention_workspace")(bytes(call))
+            workspace = torch.empty(size, dtype=torch.uint8, device=device)
+            _ATTENTION_WORKSPACE.pack_into(call, _ATTENTION_WORKSPACE_AT, workspace.data_ptr(), size)
+        rc = fn("musa_aiter_hip_attention")(bytes(call), stream_ptr(device))
+        del workspace
+    check(rc, op)
+
+
+# musa_aiter_hip_pages_call: tables, lens, refs, rows, slots, result, workspace, its bytes, caches, scales, six sizes,
+# layers, block bytes, block and layer strides, scale values, two flags.
+_PAGES_CALL = struct.Struct("<7Qq4Q6q2q4qq2i")
+_PAGES_WORKSPACE_AT = 48
+
+
+def pages(kind: str, *, op: str, device: torch.device, tables: torch.Tensor, lens: torch.Tensor | None,
+          refs: torch.Tensor, rows: torch.Tensor | None, block_size: int, slots: torch.Tensor | None = None,
+          result: torch.Tensor | None = None, max_new: int = 0, caches=(None, None), scales=(None, None),
+          layers: int = 0, block_bytes: int = 0, block_strides=(0, 0), layer_strides=(0, 0),
+          scale_values: int = 0) -> None:
+    """One of the page operations ``free``, ``fork``, ``extend`` and ``compact``."""
+    call = bytearray(_PAGES_CALL.pack(
+        tables.data_ptr(), _data(lens), refs.data_ptr(), _data(rows), _data(slots), _data(result), 0, 0,
+        _data(caches[0]), _data(caches[1]), _data(scales[0]), _data(scales[1]), tables.shape[0], tables.shape[1],
+        tables.stride(0), refs.shape[0], block_size, max_new, layers, block_bytes, *block_strides, *layer_strides,
+        scale_values, tables.dtype is torch.int64, rows is not None and rows.dtype is torch.int64))
+    with on_device(device):
+        workspace = None
+        if kind != "free":
+            size = fn("musa_aiter_hip_pages_workspace")(bytes(call), ("fork", "extend", "compact").index(kind))
+            workspace = torch.empty(size, dtype=torch.uint8, device=device)
+            struct.pack_into("<Qq", call, _PAGES_WORKSPACE_AT, workspace.data_ptr(), size)
+        rc = fn("musa_aiter_hip_pages_" + kind)(bytes(call), stream_ptr(device))
+        del workspace
     check(rc, op)

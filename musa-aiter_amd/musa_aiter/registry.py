@@ -1,7 +1,8 @@
 """Operator capability registry (API of the reference's musa_aiter/registry.py:8-56).
 
-Only the KV-cache movement family is registered: it is the path this package
-implements.  Every row lists the single backend label ``rocm-hip`` (the gfx950
+Registered are the KV-cache movement family (``kvcache``), the path of the
+reference that this package implements, and its own families ``kvblock`` and
+``kvpages`` next to it.  Every row lists the single backend label ``rocm-hip`` (the gfx950
 HIP kernels behind ``libmusa_aiter_kv_hip.so``), which is what
 ``python -m musa_aiter.cli list-ops --family kvcache`` prints.  Devices are
 torch device types: ROCm tensors report ``cuda``.
@@ -155,3 +156,20 @@ _kv("hicache_transfer_kv_per_layer_direct_pf_lf", "hip-native", _HICACHE,
     "SGLang direct HiCache page-first pages -> one layer-first layer.")
 _kv("hicache_transfer_kv_all_layer_direct_lf_pf", "hip-native", _HICACHE,
     "SGLang direct HiCache layer-first rows -> all-layer page-first pages, one launch.")
+
+
+def _serving(name: str, family: str, dtypes: tuple[str, ...], description: str) -> None:
+    register(OperatorCapability(name, family, "hip-native", dtypes, DEVICES, (BACKEND,), description, (), VENDOR))
+
+
+# FP8 caches with one scale per block and head, and their pages (no reference counterpart, families of their own).
+_serving("kv_linear_to_paged_fp8_block", "kvblock", ("float16", "bfloat16", "float32"),
+         "Linear KV -> paged FP8 cache quantize scatter that keeps one scale per block and head.")
+_serving("kv_paged_attention_fp8", "kvblock", ("float16", "bfloat16", "float32"),
+         "Causal attention (decode, draft and prompt rows) over a paged FP8 cache with one scale per block and head.")
+_PAGES = ("int32", "int64")
+_serving("kv_extend_paged_sequences", "kvpages", _PAGES,
+         "Pages and slots for new tokens on the device; a shared partial page is copied first.")
+_serving("kv_fork_paged_sequences", "kvpages", _PAGES, "Rows take over other rows' pages by reference count.")
+_serving("kv_free_paged_sequences", "kvpages", _PAGES, "Rows are cut or ended and their pages released.")
+_serving("kv_compact_paged_blocks", "kvpages", _PAGES, "Pages in use move to the front of the cache; tables follow.")
