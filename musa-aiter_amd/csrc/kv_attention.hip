@@ -44,11 +44,40 @@ __device__ __forceinline__ SeqRows seq_rows(const AttnCall& c, int64_t b) {
   return {lo, hi - lo};
 }
 
-// Cached tokens of sequence b that its table has room for.
+// The sequence whose row t is, its first row and number of rows (seq -1: none); the same in all lanes.
+struct RowSeq {
+  int64_t seq, first, count;
+};
+
+__device__ __forceinline__ RowSeq row_sequence(const AttnCall& c, int64_t t) {
+  if (c.starts == nullptr) return t < c.batch ? RowSeq{t, t, 1} : RowSeq{-1, 0, 0};
+  for (int64_t b0 = 0; b0 < c.batch; b0 += kWave) {
+    SeqRows r{0, 0};
+    if (b0 + lane_id() < c.batch) r = seq_rows(c, b0 + lane_id());
+    const uint64_t hit = ballot(t >= r.first && t < r.first + r.count);
+    if (hit == 0) continue;
+    const int src = __builtin_ctzll(hit);
+    return {b0 + src, readlane64(r.first, src), readlane64(r.count, src)};
+  }
+  return {-1, 0, 0};
+}
+
 __device__ __forceinline__ int64_t seq_len(const AttnCall& c, int64_t b) { return int_at(c.lens, b, c.wide_lens); }
 
 __device__ __forceinline__ int64_t table_block(const AttnCall& c, int64_t b, int64_t j) {
   return int_at(c.tables, b * c.table_stride + j, c.wide_tables);
+}
+
+// A query's 16-bit value, fp16 denormals included whatever the mode register says about them.
+template <int DT>
+__device__ __forceinline__ float query_value(uint16_t bits) {
+  if constexpr (DT == kLinBF16) {
+    return bf16_bits_to_f32(bits);
+  } else {
+    const uint32_t a = static_cast<uint32_t>(bits & 0x7FFFu) << 13;
+    const uint32_t top = (bits & 0x7C00u) == 0x7C00u ? 0x7F800000u : 0u;  // infinities and NaN
+    return __uint_as_float(__float_as_uint(__uint_as_float(a) * 0x1p112f) | top | static_cast<uint32_t>(bits & 0x8000u) << 16);
+  }
 }
 
 template <int DT>
@@ -104,34 +133,15 @@ __global__ __launch_bounds__(kBlockThreads) void attention_any_kernel(const Attn
   const int lane = lane_id(), wave = wave_in_block();
   const int64_t bs = c.block_size;
 
-  // The sequence of this row.
-  int64_t seq = -1, pos = -1, len = 0;
-  if (c.starts == nullptr) {
-    seq = t < c.batch ? t : -1;
-    if (seq >= 0) {
-      len = seq_len(c, seq);
-      pos = len - 1;
-    }
-  } else {
-    for (int64_t b0 = 0; b0 < c.batch && seq < 0; b0 += kWave) {
-      const int64_t b = b0 + lane;
-      SeqRows r{0, 0};
-      if (b < c.batch) r = seq_rows(c, b);
-      const uint64_t hit = ballot(r.count > 0 && t >= r.first && t < r.first + r.count);
-      if (hit != 0) {
-        const int src = __builtin_ctzll(hit);
-        seq = b0 + src;
-        len = seq_len(c, seq);
-        pos = len - readlane64(r.count, src) + (t - readlane64(r.first, src));
-      }
-    }
-  }
+  const RowSeq row = row_sequence(c, t);
+  const int64_t seq = row.seq;
   if (seq < 0) {
     if (!c.fill_rows || split != 0) return;
     for (int64_t d = threadIdx.x; d < c.head_dim; d += kBlockThreads) store_o<DT>(c.out, rh * c.head_dim + d, 0.0f);
     if (c.lse != nullptr && threadIdx.x == 0) c.lse[rh] = -__builtin_inff();
     return;
   }
+  const int64_t pos = seq_len(c, seq) - row.count + (t - row.first);
   const int64_t group = c.heads / c.kv_heads, head = hq / group;
   for (int64_t d = threadIdx.x; d < c.head_dim; d += kBlockThreads)
     q[d] = load_q<DT>(c.query, t * c.query_row_stride + hq * c.query_head_stride + d);
@@ -214,23 +224,587 @@ __global__ __launch_bounds__(kBlockThreads) void attention_any_kernel(const Attn
   }
 }
 
+// ----- matrix-core form ---------------------------------------------------------------------------
+// A wave takes 64 cached tokens and 16 * NT query rows (row = position and head within the kv head's group) at
+// a time: S^T = K Q^T, then O^T += V^T P^T, with 16x16x32 matrix instructions.  Everything stays in the lane
+// that loaded it.  With x = lane % 16 and g = lane / 16:
+//   * K: lane (x, g) loads the 4 tokens 16 (x / 4) + 4 (x % 4) .. + 3 of rows d = 4 l + g (one dword each: 16
+//     lanes and 4 rows make 64-byte runs).  Byte i of the dwords of 8 rows is the A operand of the product for
+//     tokens {4 x + i}, so four products (i = 0..3) cover the 64 tokens.
+//   * Their results give lane (x, g) the scores of query row x with tokens 16 g + 4 r + i: the 16 tokens of one
+//     group, which lie in one block (block sizes are multiples of 16), so scales and masks are per lane.
+//   * V: lane (x, g) loads the 16 tokens of group g for d = 16 l + x (16 bytes).  Its bytes and the lane's
+//     probabilities are the operands of V^T P^T in the same token order: no value crosses lanes but the
+//     running maximum.
+// Codes become 16-bit floats by shifts: E4M3 as fp16 with the value times 2^-8 (sign, 4 exponent and 3 mantissa
+// bits fall on fp16's fields; the all-ones code is the ordinary 480 * 2^-8), E5M2 as bf16 times 2^-112.  Codes of
+// exponent 0 are zeros: for fp16 a multiplication by one flushes them, with the mode register's fp16 denormals
+// off; for bf16 their bits are masked.  Query rows are scaled by a power of two so that 16 bits hold them (two
+// summands of bf16 hold an fp16 query).  Probabilities times value scale are rounded to 11 bits (8 + 8 bits in
+// two bf16 summands, 11 + 11 in two fp16 summands where the output is fp16 and one rounding would show).
+// The value scale of a block enters the running maximum, m = max(s_j + log2 vs_j), so that the weights fit fp16
+// whatever the scales are; l = sum 2^(s_j - m) needs no such care in fp32.
+constexpr int kWaveTokens = 64;
+
+using f32x4 = float __attribute__((ext_vector_type(4)));
+using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
+using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
+using f16x2 = _Float16 __attribute__((ext_vector_type(2)));
+using bf16x2 = __bf16 __attribute__((ext_vector_type(2)));
+using f32x2 = float __attribute__((ext_vector_type(2)));
+using i16x2 = short __attribute__((ext_vector_type(2)));
+
+template <int CODEC>
+struct Mma;
+
+template <>
+struct Mma<kE4M3> {
+  static constexpr int kCodeShift = 8;     // value = stored * 2^8
+  static constexpr int kQueryTop = 14;     // query rows are scaled to [2^14, 2^15)
+  static constexpr int kWeightTop = 14;    // probabilities times value scale to at most 2^14
+  uint32_t one;                            // 1.0 twice, from behind the change of the mode register
+
+  // fp16 denormals off: the products by `one` (v_pk_mul_f16) then flush what exponent-0 codes become.  None can
+  // be moved in front of the change, which `one` comes out of, or be left out, as the compiler does not know it.
+  // (The products are no inline asm: an asm result that a matrix instruction reads would miss its wait states.)
+  __device__ __forceinline__ Mma() {
+    asm volatile("s_setreg_imm32_b32 hwreg(HW_REG_MODE, 6, 2), 0\n\ts_nop 3\n\tv_mov_b32 %0, 0x3c003c00" : "=v"(one));
+  }
+  // Denormals on again.  The outputs' conversions stay behind it: f32_to_f16_bits holds a volatile asm too.
+  __device__ __forceinline__ void done() const {
+    asm volatile("s_setreg_imm32_b32 hwreg(HW_REG_MODE, 6, 2), 3\n\ts_nop 3" ::);
+  }
+  __device__ __forceinline__ uint32_t prepare(uint32_t w) const { return w; }
+  // Two codes in the high bytes of the halves of w.
+  __device__ __forceinline__ uint32_t pair(uint32_t w) const {
+    const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, w) >> i16x2{1, 1}) & 0xBF80BF80u;
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, h) * __builtin_bit_cast(f16x2, one));
+  }
+  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+  }
+  static __device__ __forceinline__ f32x2 unpack(uint32_t v) {
+    return __builtin_convertvector(__builtin_bit_cast(f16x2, v), f32x2);
+  }
+};
+
+template <>
+struct Mma<kE5M2> {
+  static constexpr int kCodeShift = 112;
+  static constexpr int kQueryTop = 100;
+  static constexpr int kWeightTop = 40;
+  __device__ __forceinline__ void done() const {}
+  __device__ __forceinline__ uint32_t prepare(uint32_t w) const {  // zeros for exponent-0 codes
+    const uint32_t m = ((w & 0x7C7C7C7Cu) + 0x7C7C7C7Cu) & 0x80808080u;
+    return w & ((m - (m >> 7)) | 0x80808080u);
+  }
+  __device__ __forceinline__ uint32_t pair(uint32_t w) const {
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, w) >> i16x2{3, 3}) & 0x8FE08FE0u;
+  }
+  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+  }
+  static __device__ __forceinline__ f32x2 unpack(uint32_t v) {
+    return f32x2{__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)};
+  }
+};
+
+// Summands that hold a query value and a probability (see above).
+template <int CODEC, int DT>
+constexpr int kQueryParts = CODEC == kE5M2 && DT == kLinF16 ? 2 : 1;
+template <int CODEC, int DT>
+constexpr int kWeightParts = CODEC == kE5M2 || DT == kLinF16 ? 2 : 1;
+
+// Maximum and sum over the four lane groups of 16.
+__device__ __forceinline__ float groups_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float groups_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// Sizes as 32-bit numbers: rows * heads and the positions of a table row stay far below 2^31 (checked by the
+// C entry), and registers are what this kernel has least of.
+struct RowsArgs {
+  AttnCall c;
+  int32_t batch, heads, hd, bs, num_blocks, room;  // room: positions that a table row has place for
+  int32_t group;        // heads per kv head
+  int32_t block_shift;  // log2(block_size / 16), or -1
+  int32_t seq_tiles;    // row tiles of every sequence (no row table)
+  int32_t window, splits;
+};
+
+constexpr int32_t kMostRoom = 1 << 29;
+// Lengths past it see what a row of kMostRoom positions would show them.
+constexpr int32_t kMostLen = 3 << 29;
+
+// The row tile of a workgroup: rows [first, first + count) of sequence `seq` from (position, head) row `base`.
+struct RowTile {
+  int32_t seq, first, count, base;
+};
+
+// Finds the `index`-th tile of `size` rows over all sequences (seq -1: past the last).
+__device__ __forceinline__ RowTile find_tile(const RowsArgs& a, int32_t index, int size) {
+  const AttnCall& c = a.c;
+  if (c.starts == nullptr) {
+    const int32_t seq = index / a.seq_tiles;
+    if (seq >= a.batch) return {-1, 0, 0, 0};
+    return {seq, seq, 1, (index - seq * a.seq_tiles) * size};
+  }
+  int32_t before = 0;
+  for (int32_t b0 = 0; b0 < a.batch; b0 += kWave) {
+    const int32_t b = b0 + lane_id();
+    SeqRows r{0, 0};
+    if (b < a.batch) r = seq_rows(c, b);
+    const int32_t first = static_cast<int32_t>(r.first), count = static_cast<int32_t>(r.count);
+    const int32_t tiles = (count * a.group + size - 1) / size;
+    int32_t upto = tiles;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const int32_t y = __shfl_up(upto, o);
+      if (lane_id() >= o) upto += y;
+    }
+    const uint64_t hit = ballot(before + upto > index);
+    if (hit != 0) {
+      const int src = __builtin_ctzll(hit);
+      const int32_t in_front = before + __builtin_amdgcn_readlane(upto - tiles, src);
+      return {b0 + src, __builtin_amdgcn_readlane(first, src), __builtin_amdgcn_readlane(count, src),
+              (index - in_front) * size};
+    }
+    before += __builtin_amdgcn_readlane(upto, kWave - 1);
+  }
+  return {-1, 0, 0, 0};
+}
+
+// Zeroes this worker's share of the rows that belong to no sequence.
+template <int DT>
+__device__ __forceinline__ void fill_loose_rows(const AttnCall& c, int64_t worker, int64_t workers) {
+  for (int64_t t = worker; t < c.rows; t += workers) {
+    if (row_sequence(c, t).seq >= 0) continue;
+    for (int64_t d = threadIdx.x; d < c.heads * c.head_dim; d += kBlockThreads)
+      store_o<DT>(c.out, t * c.heads * c.head_dim + d, 0.0f);
+    if (c.lse != nullptr)
+      for (int64_t h = threadIdx.x; h < c.heads; h += kBlockThreads) c.lse[t * c.heads + h] = -__builtin_inff();
+  }
+}
+
+// Query rows as B operands: element j of step s of lane (x, g) is d = 32 s + 4 j + g of row x.
+template <int HDP, bool EXACT, int CODEC, int DT>
+struct QueryTile {
+  u32x4 q[kQueryParts<CODEC, DT>][HDP / 32];
+  float factor;  // scores times this (and the key scale) are in base 2
+
+  // `row` is readable; without `mine` the row is zeros.
+  __device__ __forceinline__ void load(const RowsArgs& a, const uint16_t* row, bool mine) {
+    const int g = lane_id() >> 4;
+    float most = 0.0f;
+    uint16_t raw[HDP / 4];
+#pragma unroll
+    for (int l = 0; l < HDP / 4; ++l) {
+      const int d = 4 * l + g;
+      raw[l] = row[EXACT ? d : min(d, a.hd - 1)];
+      if (!mine || (!EXACT && d >= a.hd)) raw[l] = 0;
+    }
+#pragma unroll
+    for (int l = 0; l < HDP / 4; ++l) most = fmaxf(most, fabsf(query_value<DT>(raw[l])));
+    most = groups_max(most);
+    const bool fine = most > 0.0f && most < __builtin_inff();
+    const int up = fine ? Mma<CODEC>::kQueryTop - ilogbf(most) : 0;
+    factor = __builtin_ldexpf(static_cast<float>(a.c.softmax_scale) * kLog2e, Mma<CODEC>::kCodeShift - up);
+#pragma unroll
+    for (int l = 0; l < HDP / 4; l += 2) {
+      float a = __builtin_ldexpf(query_value<DT>(raw[l]), up), b = __builtin_ldexpf(query_value<DT>(raw[l + 1]), up);
+      for (int part = 0; part < kQueryParts<CODEC, DT>; ++part) {
+        const uint32_t v = Mma<CODEC>::pack(a, b);
+        q[part][l / 8][l % 8 / 2] = v;
+        const f32x2 took = Mma<CODEC>::unpack(v);
+        a -= took[0];
+        b -= took[1];
+      }
+    }
+  }
+};
+
+// Table entry of the 16-token group that begins at `token` (multiple of 16), or -1; *inside: token in its block.
+__device__ __forceinline__ int32_t group_block(const RowsArgs& a, const uint8_t* row, int32_t token, int32_t end,
+                                               int32_t* inside) {
+  const uint32_t n16 = static_cast<uint32_t>(token) >> 4, b16 = static_cast<uint32_t>(a.bs) >> 4;
+  const uint32_t j = a.block_shift >= 0 ? n16 >> a.block_shift : n16 / b16;
+  *inside = static_cast<int32_t>((n16 - j * b16) << 4);
+  if (token >= end) return -1;
+  const int64_t blk = int_at(row, j, a.c.wide_tables);
+  return blk >= 0 && blk < a.num_blocks ? static_cast<int32_t>(blk) : -1;
+}
+
+struct GroupIds {
+  int32_t k, v;          // blocks of the groups whose keys and values the lane loads
+  int32_t k_in, v_in;
+};
+
+__device__ __forceinline__ GroupIds tile_ids(const RowsArgs& a, const uint8_t* row, int32_t token, int32_t end) {
+  const int x = lane_id() & 15, g = lane_id() >> 4;
+  GroupIds ids;
+  ids.k = group_block(a, row, token + 16 * (x >> 2), end, &ids.k_in);
+  ids.v = group_block(a, row, token + 16 * g, end, &ids.v_in);
+  return ids;
+}
+
+__device__ __forceinline__ uint32_t load4(const uint8_t* p) {
+  return *reinterpret_cast<const KVHIP_GLOBAL uint32_t*>(reinterpret_cast<uint64_t>(p));
+}
+
+// A uniform value that the compiler takes for a new one, so that what follows from it is computed again for
+// every tile: held over the loop, the rows' offsets take a register per load, and the registers ran out.
+__device__ __forceinline__ int not_hoisted(int v) {
+  asm volatile("" : "+s"(v));
+  return v;
+}
+
+// DIMS rows of the keys of 64 tokens: dword l is row d = first + 4 l + g of the lane's 4 tokens.  A group without a block reads block
+// 0, which every cache has; its scores are masked.  Without EXACT rows past head_dim read the last one: the
+// query is zero there.
+template <int DIMS, bool EXACT>
+__device__ __forceinline__ void load_keys(const RowsArgs& a, int64_t head_off, const GroupIds& ids, int first,
+                                          uint32_t* k) {
+  const AttnCall& c = a.c;
+  const int x = lane_id() & 15, g = lane_id() >> 4;
+  const int32_t bs = a.bs;
+  const uint8_t* p = static_cast<const uint8_t*>(c.cache[0]) + static_cast<int64_t>(ids.k < 0 ? 0 : ids.k) *
+                     c.cache_block_stride[0] + head_off + ids.k_in + 4 * (x & 3);
+  if constexpr (EXACT) {
+    p += (first + g) * bs;
+#pragma unroll
+    for (int l = 0; l < DIMS / 4; ++l, p += 4 * bs) k[l] = load4(p);
+  } else {
+    const int last = a.hd - 1, step = not_hoisted(bs);
+#pragma unroll
+    for (int l = 0; l < DIMS / 4; ++l) k[l] = load4(p + min(first + 4 * l + g, last) * step);
+  }
+}
+
+// Scales of the lane's group g.
+struct GroupScales {
+  float ks, vs;
+  bool seen;  // the group has a block in the cache
+};
+
+__device__ __forceinline__ GroupScales load_scales(const AttnCall& c, int32_t head, const GroupIds& ids) {
+  const int64_t blk = ids.v < 0 ? 0 : ids.v;
+  return {c.scale[0][blk * c.scale_block_stride[0] + head * c.scale_head_stride[0]],
+          c.scale[1][blk * c.scale_block_stride[1] + head * c.scale_head_stride[1]], ids.v >= 0};
+}
+
+// DIMS rows of the values of 64 tokens: piece l is row d = first + 16 l + x of the 16 tokens of group g (rows past
+// head_dim as above: outputs past it are not stored).
+template <int DIMS, bool EXACT>
+__device__ __forceinline__ void load_values(const RowsArgs& a, int64_t head_off, const GroupIds& ids, int first,
+                                            u32x4* v) {
+  const AttnCall& c = a.c;
+  const int x = lane_id() & 15;
+  const int32_t bs = a.bs;
+  const int64_t blk = ids.v < 0 ? 0 : ids.v;
+  const uint8_t* p = static_cast<const uint8_t*>(c.cache[1]) + blk * c.cache_block_stride[1] + head_off + ids.v_in;
+  if constexpr (EXACT) {
+    p += (first + x) * bs;
+#pragma unroll
+    for (int l = 0; l < DIMS / 16; ++l, p += 16 * bs) v[l] = ld16_cached(p);
+  } else {
+    const int last = a.hd - 1, step = not_hoisted(bs);
+#pragma unroll
+    for (int l = 0; l < DIMS / 16; ++l) v[l] = ld16_cached(p + min(first + 16 * l + x, last) * step);
+  }
+}
+
+// Running state of 16 query rows: lane (x, g) holds row x, dims 16 l + 4 g + r, and its own tokens' share of l.
+template <int HDP>
+struct RowState {
+  f32x4 acc[HDP / 16];
+  float m, l;
+};
+
+// Positions [lo, hi) that a row sees.
+struct Sight {
+  int32_t lo, hi;
+};
+
+// Adds DIMS dims' part, from step FIRST on, of the scores of 16 * NT rows with 64 tokens, before scaling: element r
+// of product i is token 16 g + 4 r + i.
+template <int FIRST, int DIMS, int HDP, bool EXACT, int NT, int CODEC, int DT>
+__device__ __forceinline__ void key_products(const Mma<CODEC>& mma, const uint32_t* k,
+                                             const QueryTile<HDP, EXACT, CODEC, DT>* q, f32x4 (*score)[4]) {
+#pragma unroll
+  for (int step = 0; step < DIMS / 32; ++step) {
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = mma.prepare(k[8 * step + j]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u32x4 a;
+      // Bytes i of rows j and j + 1 into the high bytes of the halves.
+      const uint32_t sel = 0x000C000Cu | (static_cast<uint32_t>(i) << 8) | (static_cast<uint32_t>(4 + i) << 24);
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) a[j / 2] = mma.pair(__builtin_amdgcn_perm(w[j + 1], w[j], sel));
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int part = 0; part < kQueryParts<CODEC, DT>; ++part)
+          score[n][i] = Mma<CODEC>::mma(a, q[n].q[part][FIRST + step], score[n][i]);
+    }
+  }
+}
+
+// One step of the running softmax: scores in, weights (probability * value scale) out; rescales the state where
+// the maximum grew.
+template <int HDP, int CODEC>
+__device__ __forceinline__ void soften(f32x4* score, float factor, const GroupScales& scales, bool masked,
+                                       int32_t token, const Sight& sight, RowState<HDP>& s) {
+  const float f = factor * scales.ks, vs = scales.vs;
+  const bool seen = scales.seen;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) score[i] *= f;
+  if (masked) {
+    const int first = token + 16 * (lane_id() >> 4);
+    const int lo = sight.lo - first, hi = seen ? sight.hi - first : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (4 * r + i < lo || 4 * r + i >= hi) score[i][r] = -__builtin_inff();
+  }
+  float most = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) most = fmaxf(most, score[i][r]);
+  const float lift = __builtin_amdgcn_fmed3f(__builtin_amdgcn_logf(vs), -100.0f, 100.0f);
+  const float top = fmaxf(s.m, groups_max(most + lift));
+  const float ref = top == -__builtin_inff() ? 0.0f : top;
+  if (ballot(top > s.m) != 0) {
+    const float fade = __builtin_amdgcn_exp2f(s.m - ref);
+    s.l *= fade;
+#pragma unroll
+    for (int l = 0; l < HDP / 16; ++l) s.acc[l] *= fade;
+    s.m = top;
+  }
+  const float weight = seen ? __builtin_ldexpf(vs, Mma<CODEC>::kWeightTop) : 0.0f;
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float p = __builtin_amdgcn_exp2f(score[i][r] - ref);
+      sum += p;
+      score[i][r] = p * weight;
+    }
+  s.l += sum;
+}
+
+// Weights as B operands of step `step`: tokens (0, 2), (1, 3) of the group's dword 2 step, then of the next one.
+template <int CODEC, int DT>
+__device__ __forceinline__ void pack_weights(const f32x4* score, int step, u32x4* p) {
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    const int r = 2 * step + (h >> 1), i = h & 1;
+    float a = score[i][r], b = score[i + 2][r];
+#pragma unroll
+    for (int part = 0; part < kWeightParts<CODEC, DT>; ++part) {
+      p[part][h] = Mma<CODEC>::pack(a, b);
+      const f32x2 took = Mma<CODEC>::unpack(p[part][h]);
+      a -= took[0];
+      b -= took[1];
+    }
+  }
+}
+
+// Adds weights times values to the state's dims from 16 * FIRST on.
+template <int FIRST, int DIMS, int HDP, int NT, int CODEC, int DT>
+__device__ __forceinline__ void value_products(const Mma<CODEC>& mma, const u32x4* v,
+                                               u32x4 (*p)[2][kWeightParts<CODEC, DT>], RowState<HDP>* state) {
+#pragma unroll
+  for (int step = 0; step < 2; ++step) {
+#pragma unroll
+    for (int l = 0; l < DIMS / 16; ++l) {
+      u32x4 a;
+#pragma unroll
+      for (int h = 0; h < 4; h += 2) {
+        const uint32_t w = mma.prepare(v[l][2 * step + (h >> 1)]);
+        a[h] = mma.pair(w << 8);
+        a[h + 1] = mma.pair(w);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int part = 0; part < kWeightParts<CODEC, DT>; ++part)
+          state[n].acc[FIRST + l] = Mma<CODEC>::mma(a, p[n][step][part], state[n].acc[FIRST + l]);
+    }
+  }
+}
+
+// One workgroup per (row tile, kv head, part): its four waves take turns at the part's 64-token tiles and join
+// what they have in LDS, 128 dims at a time.  A wave loads the next tile's keys once this tile's are used up and
+// its values behind this tile's, so either the one or the other is on its way all the time.
+constexpr int kJoinDims = 128;
+constexpr int kJoinStride = kJoinDims + 4;
+
+template <int HDP, bool EXACT, int NT, int CODEC, int DT>
+__global__ __launch_bounds__(kBlockThreads, HDP * NT <= 128 ? 2 : 1)
+void attention_rows_kernel(const RowsArgs a) {
+  const AttnCall& c = a.c;
+  constexpr int kRows = 16 * NT;
+  const int32_t head = blockIdx.y, split = blockIdx.z;
+  const RowTile tile = find_tile(a, blockIdx.x, kRows);
+  if (c.starts != nullptr && c.fill_rows && head == 0 && split == 0) fill_loose_rows<DT>(c, blockIdx.x, gridDim.x);
+  if (tile.seq < 0) return;
+  const int x = lane_id() & 15, wave = wave_in_block();
+  const int64_t said = seq_len(c, tile.seq);
+  const int32_t len = said < 0 ? 0 : said < kMostLen ? static_cast<int32_t>(said) : kMostLen;
+  const int32_t group = a.group, in_seq = tile.count * group;
+  const int32_t before = len - tile.count;  // position of the sequence's first row
+  const Mma<CODEC> mma;
+
+  // Rows and what they see.
+  QueryTile<HDP, EXACT, CODEC, DT> q[NT];
+  RowState<HDP> state[NT];
+  Sight sight[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int32_t r = tile.base + 16 * n + x;
+    const bool mine = r < in_seq;
+    const int32_t i = mine ? r / group : 0, h = mine ? r - i * group : 0;
+    const int32_t pos = before + i;
+    q[n].load(a, static_cast<const uint16_t*>(c.query) + (tile.first + i) * c.query_row_stride +
+                     (head * group + h) * c.query_head_stride, mine);
+    sight[n].hi = mine ? min(pos + 1, a.room) : 0;
+    sight[n].lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
+    state[n].m = -__builtin_inff();
+    state[n].l = 0.0f;
+#pragma unroll
+    for (int l = 0; l < HDP / 16; ++l) state[n].acc[l] = f32x4{0, 0, 0, 0};
+  }
+  const int32_t pos_lo = before + tile.base / group, pos_hi = before + (min(tile.base + kRows, in_seq) - 1) / group;
+  const int32_t end = min(pos_hi + 1, a.room);
+  const int32_t begin = a.window > 0 ? max(pos_lo - a.window + 1, 0) : 0;
+  // Tiles inside [all_lo, all_hi) are seen whole by every row.
+  const int32_t all_lo = a.window > 0 ? max(pos_hi - a.window + 1, 0) : 0;
+  const Span span = part_span(begin, end, split, a.splits);
+  const int32_t last = static_cast<int32_t>(span.hi), all_hi = min(pos_lo + 1, last);
+  const int64_t head_off = static_cast<int64_t>(head) * a.hd * a.bs;
+  const uint8_t* row = static_cast<const uint8_t*>(c.tables) +
+                       tile.seq * c.table_stride * (c.wide_tables ? 8 : 4);
+
+  constexpr int32_t kStep = kWavesPerBlock * kWaveTokens;
+  int32_t token = static_cast<int32_t>(span.lo) + wave * kWaveTokens;
+  if (token < last) {
+    // 256 dims go in two halves through the same registers.
+    constexpr int kDims = HDP <= 128 ? HDP : HDP / 2;
+    uint32_t k[kDims / 4];
+    u32x4 v[kDims / 16];
+    GroupIds ids = tile_ids(a, row, token, last);
+    load_keys<kDims, EXACT>(a, head_off, ids, 0, k);
+    load_values<kDims, EXACT>(a, head_off, ids, 0, v);
+    for (;;) {
+      const GroupScales scales = load_scales(c, head, ids);
+      const int32_t next = token + kStep;
+      const GroupIds next_ids = tile_ids(a, row, next, last);
+      f32x4 score[NT][4] = {};
+      key_products<0, kDims, HDP, EXACT, NT, CODEC, DT>(mma, k, q, score);
+      if constexpr (HDP > kDims) {
+        load_keys<kDims, EXACT>(a, head_off, ids, kDims, k);
+        key_products<kDims / 32, kDims, HDP, EXACT, NT, CODEC, DT>(mma, k, q, score);
+      }
+      if (next < last) load_keys<kDims, EXACT>(a, head_off, next_ids, 0, k);
+      const bool masked = token < all_lo || token + kWaveTokens > all_hi || ballot(!scales.seen) != 0;
+      u32x4 p[NT][2][kWeightParts<CODEC, DT>];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        soften<HDP, CODEC>(score[n], q[n].factor, scales, masked, token, sight[n], state[n]);
+        pack_weights<CODEC, DT>(score[n], 0, p[n][0]);
+        pack_weights<CODEC, DT>(score[n], 1, p[n][1]);
+      }
+      value_products<0, kDims, HDP, NT, CODEC, DT>(mma, v, p, state);
+      if constexpr (HDP > kDims) {
+        load_values<kDims, EXACT>(a, head_off, ids, kDims, v);
+        value_products<kDims / 16, kDims, HDP, NT, CODEC, DT>(mma, v, p, state);
+      }
+      if (next >= last) break;
+      load_values<kDims, EXACT>(a, head_off, next_ids, 0, v);
+      ids = next_ids;
+      token = next;
+    }
+  }
+
+  mma.done();
+
+  // The four waves' results of a row are joined by the thread that stores them.
+  __shared__ float joined[kWavesPerBlock][16][kJoinStride];
+  __shared__ float ml[kWavesPerBlock][16][2];
+  constexpr int kChunk = HDP < kJoinDims ? HDP : kJoinDims;
+  const float back = __builtin_ldexpf(1.0f, Mma<CODEC>::kCodeShift - Mma<CODEC>::kWeightTop);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float l = groups_sum(state[n].l);
+#pragma unroll
+    for (int d0 = 0; d0 < HDP; d0 += kChunk) {
+      __syncthreads();
+      if (lane_id() < 16) {
+        ml[wave][x][0] = state[n].m;
+        ml[wave][x][1] = l;
+      }
+#pragma unroll
+      for (int k = 0; k < kChunk / 16; ++k)
+        *reinterpret_cast<f32x4*>(&joined[wave][x][16 * k + 4 * (lane_id() >> 4)]) = state[n].acc[d0 / 16 + k];
+      __syncthreads();
+      const int at = threadIdx.x >> 4;
+      const int32_t r = tile.base + 16 * n + at;
+      if (r >= in_seq) continue;
+      const int32_t i = r / group;
+      const int64_t rh = static_cast<int64_t>(tile.first + i) * a.heads + head * group + (r - i * group);
+      float top = ml[0][at][0];
+#pragma unroll
+      for (int w = 1; w < kWavesPerBlock; ++w) top = fmaxf(top, ml[w][at][0]);
+      const float ref = top == -__builtin_inff() ? 0.0f : top;
+      float fade[kWavesPerBlock], sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWavesPerBlock; ++w) {
+        fade[w] = __builtin_amdgcn_exp2f(ml[w][at][0] - ref);
+        sum += ml[w][at][1] * fade[w];
+      }
+      for (int k = threadIdx.x & 15; k < kChunk; k += 16) {
+        float o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWavesPerBlock; ++w) o += joined[w][at][k] * fade[w];
+        o *= back;
+        if (!EXACT && d0 + k >= a.hd) continue;
+        if (a.splits > 1) part_acc(c, split, rh)[d0 + k] = o;
+        else store_o<DT>(c.out, rh * a.hd + d0 + k, sum == 0.0f ? 0.0f : o / sum);
+      }
+      if (d0 == 0 && (threadIdx.x & 15) == 0) {
+        if (a.splits > 1) {
+          part_ml(c, split, rh)[0] = top;
+          part_ml(c, split, rh)[1] = sum;
+        } else if (c.lse != nullptr) {
+          c.lse[rh] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * kLn2;
+        }
+      }
+    }
+  }
+}
+
 // ----- joining the parts: one wave per (row, head) -------------------------------------------------
 template <int DT>
 __global__ __launch_bounds__(kBlockThreads) void attention_join_kernel(const AttnCall c) {
   const int64_t rh = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave_in_block();
   if (rh >= c.rows * c.heads) return;
   const int64_t t = rh / c.heads;
-  if (c.starts != nullptr) {  // rows of no sequence have no parts
-    bool mine = false;
-    for (int64_t b0 = 0; b0 < c.batch && !mine; b0 += kWave) {
-      SeqRows r{0, 0};
-      if (b0 + lane_id() < c.batch) r = seq_rows(c, b0 + lane_id());
-      mine = ballot(t >= r.first && t < r.first + r.count) != 0;
-    }
-    if (!mine) return;
-  } else if (t >= c.batch) {
-    return;
-  }
+  if (row_sequence(c, t).seq < 0) return;  // no parts
   float top = -__builtin_inff();
   for (int64_t s = 0; s < c.splits; ++s) top = fmaxf(top, part_ml(c, s, rh)[0]);
   const float ref = top == -__builtin_inff() ? 0.0f : top;
@@ -260,19 +834,88 @@ hipError_t launch_any(const AttnCall& c, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// Whether the matrix-core form takes the call: 16-bit queries, up to 256 dims, 16-token groups that lie in one
+// block and begin at multiples of 16 bytes.
+bool takes_rows(const AttnCall& c) {
+  if (c.dtype == kLinF32 || c.head_dim > 256 || c.block_size % 16 != 0) return false;
+  uint64_t all = 0;
+  for (int kv = 0; kv < 2; ++kv)
+    all |= reinterpret_cast<uint64_t>(c.cache[kv]) | static_cast<uint64_t>(c.cache_block_stride[kv]);
+  return all % 16 == 0;
+}
+
+// 16-row tiles that a wave holds: 2 where the rows of a sequence fill more than one on average and two fit the
+// registers.
+int row_tiles(const AttnCall& c) {
+  if (c.head_dim > 128) return 1;
+  const int64_t group = c.heads / c.kv_heads;
+  const int64_t rows = c.starts == nullptr ? 1 : c.batch > 0 ? (c.rows + c.batch - 1) / c.batch : 1;
+  return rows * group <= 16 ? 1 : 2;
+}
+
+int64_t tiles_bound(const AttnCall& c, int size) {
+  const int64_t group = c.heads / c.kv_heads;
+  if (c.starts == nullptr) return c.batch * ((group + size - 1) / size);
+  return c.rows * group / size + c.batch;
+}
+
+template <int HDP, bool EXACT, int NT, int CODEC, int DT>
+hipError_t launch_rows_as(const AttnCall& c, hipStream_t stream) {
+  RowsArgs a{};
+  a.c = c;
+  a.batch = static_cast<int32_t>(c.batch);
+  a.heads = static_cast<int32_t>(c.heads);
+  a.hd = static_cast<int32_t>(c.head_dim);
+  a.bs = static_cast<int32_t>(c.block_size);
+  a.num_blocks = static_cast<int32_t>(c.num_blocks);
+  a.room = static_cast<int32_t>(c.max_blocks * c.block_size);
+  a.window = static_cast<int32_t>(c.window < kMostRoom ? c.window : kMostRoom);
+  a.splits = static_cast<int32_t>(c.splits);
+  a.group = static_cast<int32_t>(c.heads / c.kv_heads);
+  const int64_t b16 = c.block_size / 16;
+  a.block_shift = (b16 & (b16 - 1)) == 0 ? __builtin_ctzll(b16) : -1;
+  a.seq_tiles = (a.group + 16 * NT - 1) / (16 * NT);
+  int64_t tiles = tiles_bound(c, 16 * NT);
+  if (tiles < 1) tiles = 1;  // rows of no sequence are still to be filled
+  const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>(c.kv_heads), static_cast<uint32_t>(c.splits));
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_rows_kernel<HDP, EXACT, NT, CODEC, DT>), grid, dim3(kBlockThreads), 0,
+                     stream, a);
+  return hipGetLastError();
+}
+
+template <int DT, int CODEC, int NT>
+hipError_t launch_rows(const AttnCall& c, hipStream_t stream) {
+  if (c.head_dim == 64) return launch_rows_as<64, true, NT, CODEC, DT>(c, stream);
+  if (c.head_dim < 64) return launch_rows_as<64, false, NT, CODEC, DT>(c, stream);
+  if (c.head_dim == 96) return launch_rows_as<96, true, NT, CODEC, DT>(c, stream);
+  if (c.head_dim == 128) return launch_rows_as<128, true, NT, CODEC, DT>(c, stream);
+  if (c.head_dim < 128) return launch_rows_as<128, false, NT, CODEC, DT>(c, stream);
+  if (c.head_dim == 256) return launch_rows_as<256, true, 1, CODEC, DT>(c, stream);
+  return launch_rows_as<256, false, 1, CODEC, DT>(c, stream);
+}
+
+template <int DT, int CODEC>
+hipError_t launch_typed(const AttnCall& c, hipStream_t stream) {
+  if constexpr (DT != kLinF32)
+    if (takes_rows(c))
+      return row_tiles(c) == 1 ? launch_rows<DT, CODEC, 1>(c, stream) : launch_rows<DT, CODEC, 2>(c, stream);
+  return launch_any<DT, CODEC>(c, stream);
+}
+
 template <int DT>
 hipError_t launch_dtype(const AttnCall& c, hipStream_t stream) {
-  const hipError_t err = c.codec == kE4M3 ? launch_any<DT, kE4M3>(c, stream) : launch_any<DT, kE5M2>(c, stream);
+  const hipError_t err = c.codec == kE4M3 ? launch_typed<DT, kE4M3>(c, stream) : launch_typed<DT, kE5M2>(c, stream);
   if (err != hipSuccess || c.splits == 1) return err;
   return launch_join<DT>(c, stream);
 }
 
 }  // namespace
 
+// Parts: enough workgroups for two per CU and then some, none below 256 tokens (a workgroup's four waves).
 int64_t attention_splits(const AttnCall& c, int64_t longest) {
-  const int64_t groups = c.rows * c.heads;
-  int64_t splits = groups > 0 ? 1024 / groups : 1;
-  const int64_t most = longest / 256;
+  const int64_t groups = takes_rows(c) ? tiles_bound(c, 16 * row_tiles(c)) * c.kv_heads : c.rows * c.heads;
+  int64_t splits = groups > 0 ? (1024 + groups - 1) / groups : 1;
+  const int64_t most = (longest + 255) / 256;
   splits = splits < most ? splits : most;
   return splits < 1 ? 1 : splits > 64 ? 64 : splits;
 }

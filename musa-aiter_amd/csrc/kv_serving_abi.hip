@@ -89,7 +89,8 @@ int block_store(const musa_aiter_hip_block_store_call& c, hipStream_t stream) {
 bool attention_sizes_ok(const musa_aiter_hip_attention_call& c) {
   return extent(c.rows, 0) && extent(c.batch, 0) && extent(c.heads, 1) && extent(c.kv_heads, 1) &&
          extent(c.head_dim, 1) && extent(c.block_size, 1) && extent(c.num_blocks, 1) && extent(c.max_blocks, 0) &&
-         c.heads % c.kv_heads == 0 && c.heads <= 65535 && c.head_dim <= 512 && c.window >= 0;
+         c.heads % c.kv_heads == 0 && c.heads <= 65535 && c.head_dim <= 512 && c.window >= 0 &&
+         c.rows * c.heads < kMaxExtent && c.max_blocks * c.block_size <= kMaxExtent / 4;
 }
 
 int attention(const musa_aiter_hip_attention_call& c, hipStream_t stream) {

@@ -235,6 +235,8 @@ def kv_paged_attention_fp8(
         raise ValueError(f"{op}: all tensors must be on the same device")
     _check_scales(op, k_scales, "k_scales", (nb, nh), device)
     _check_scales(op, v_scales, "v_scales", (nb, nh), device)
+    if rows * heads >= 1 << 31 or int(block_tables.shape[1]) * bs > 1 << 29:
+        raise ValueError(f"{op}: at most 2**31 - 1 rows times heads and 2**29 positions per sequence")
     if window is not None and window < 1:
         raise ValueError(f"{op}: window must be positive")
     if max_seq_len is not None and max_seq_len < 0:

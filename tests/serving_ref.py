@@ -68,17 +68,19 @@ def block_store(new: np.ndarray, cache: np.ndarray, scales: np.ndarray, slots: n
 
 
 def attention(query, key, value, tables, lens, k_scales, v_scales, fmt, *, starts=None, scale=None, window=None):
-    """float64 (out [T, Hq, D], lse [T, Hq], weight [T, Hq, D], spread [T, Hq]) of float64 query and uint8 caches.
+    """float64 (out [T, Hq, D], lse [T, Hq], weight [T, Hq, D], spread [T, Hq], faint [T, Hq, D]) of float64 query and
+    uint8 caches.
 
-    weight is sum_j p_j |v_jd| and spread the largest sum_d |q_d k_jd| * |scale| that a row meets: what the error
-    of a computation in fewer bits grows with.  Rows of no sequence are NaN."""
+    weight is sum_j p_j |v_jd|, spread the largest sum_d |q_d k_jd| * |scale| that a row meets, and faint
+    max_j(p_j vs_j) * sum_j |code_jd|: what the error of a computation in fewer bits grows with.  Rows of no
+    sequence are NaN."""
     table = decode_table(fmt)
     rows, heads, hd = query.shape
     nb, nh, _, bs = key.shape
     scale = hd ** -0.5 if scale is None else scale
     starts = list(range(len(lens) + 1)) if starts is None else list(starts)
     out, lse = np.full(query.shape, np.nan), np.full((rows, heads), np.nan)
-    weight, spread = np.zeros(query.shape), np.zeros((rows, heads))
+    weight, spread, faint = np.zeros(query.shape), np.zeros((rows, heads)), np.zeros(query.shape)
     for b, n in enumerate(lens):
         lo, hi = starts[b], starts[b + 1]
         room = min(max(int(n), 0), tables.shape[1] * bs)
@@ -88,7 +90,8 @@ def attention(query, key, value, tables, lens, k_scales, v_scales, fmt, *, start
         safe = np.where(there, blk, 0)
         for h in range(nh):
             k = table[key[safe, h, :, off]] * k_scales[safe, h][:, None]
-            v = table[value[safe, h, :, off]] * v_scales[safe, h][:, None]
+            codes, vs = table[value[safe, h, :, off]], v_scales[safe, h]
+            v = codes * vs[:, None]
             for t in range(lo, hi):
                 pos = int(n) - (hi - lo) + (t - lo)
                 j = np.arange(room)
@@ -103,8 +106,9 @@ def attention(query, key, value, tables, lens, k_scales, v_scales, fmt, *, start
                     p /= p.sum()
                     out[t, g] = p @ v[seen]
                     weight[t, g] = p @ np.abs(v[seen])
+                    faint[t, g] = (p * vs[seen]).max() * np.abs(codes[seen]).sum(axis=0)
                     spread[t, g] = (np.abs(k[seen]) @ np.abs(query[t, g])).max() * abs(scale)
-    return out, lse, weight, spread
+    return out, lse, weight, spread, faint
 
 
 class Pages:

@@ -5,7 +5,10 @@ rounded: the output once (half a step of its type relative to it), every weight 
 (2^-11 relative each, so 2^-11 * sum_j p_j |v_jd| in all), and the scores in float32.  A score is a sum of head_dim
 products: its error is at most (head_dim + 8) * 2^-24 times the sum of their sizes (`spread`), it is taken times
 log2(e) and to the power of two in float32 (2^-22 more, relative), and an error d of all scores changes p_j by at
-most e^(2 d) - 1.  The accumulations over the tokens add (tokens + 8) * 2^-24 * sum_j p_j |v_jd|.
+most e^(2 d) - 1.  The accumulations over the tokens add (tokens + 8) * 2^-24 * sum_j p_j |v_jd|.  Weights p_j vs_j
+are held in 16 bits, scaled so that the largest is 2^14: one below fp16's smallest normal value, 2^-14, may be lost
+(for an fp16 output in two summands the same holds for the sum), which adds 2^-28 * max_j(p_j vs_j) * |code_jd| for
+every token (`faint`).
 """
 
 from __future__ import annotations
@@ -63,7 +66,7 @@ class Case:
                              window=self.window)
 
     def check(self, out, lse=None, scale=None, only=None):
-        want, want_lse, weight, spread = self.expect(scale)
+        want, want_lse, weight, spread, faint = self.expect(scale)
         got = out.double().cpu().numpy()
         hd, tokens = want.shape[2], int(self.lens.max(initial=1))
         mine = ~np.isnan(want_lse)
@@ -71,7 +74,7 @@ class Case:
             mine &= only
         noise = (hd + 8) * 2.0 ** -24 * spread + 2.0 ** -22 * (1 + np.where(np.isfinite(want_lse), np.abs(want_lse), 0))
         bound = torch.finfo(self.dtype).eps / 2 * np.abs(want) + weight * (
-            2.0 ** -11 * (1 + 2.0 ** -8) + np.expm1(2 * noise) + (tokens + 8) * 2.0 ** -24)[..., None] + 2.0 ** -40
+            2.0 ** -11 * (1 + 2.0 ** -8) + np.expm1(2 * noise) + (tokens + 8) * 2.0 ** -24)[..., None] + 2.0 ** -28 * (1 + 2.0 ** -8) * faint + 2.0 ** -40
         if self.dtype is torch.float16:
             bound += 2.0 ** -25  # half a step of the smallest values
         off = np.abs(got - want)[mine] - bound[mine]
@@ -221,13 +224,29 @@ def test_scales_of_every_size(dtype, fmt):
     case.check(*_go(case))
 
 
-def test_large_and_small_queries_and_softmax_scale():
-    for size, scale in ((1e4, 1e-4), (1e-6, 1e5), (3.0, 0.0), (1.0, -0.2), (1e30, 1e-31)):
-        case = Case(lens=[40, 130], heads=4, kv_heads=2, seed=12)
-        case.query = (case.query.float() * size).to(torch.bfloat16)
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("dtype,size,scale", [("bf16", 1e4, 1e-4), ("bf16", 1e-6, 1e5), ("bf16", 3.0, 0.0),
+                                              ("bf16", 1.0, -0.2), ("bf16", 1e30, 1e-31), ("fp16", 2e-7, 1e5),
+                                              ("fp16", 1e-5, 1e4), ("fp16", 1e4, 1e-4), ("fp32", 1e-30, 1e29)])
+def test_large_and_small_queries_and_softmax_scale(fmt, dtype, size, scale):
+    for hd in (64, 128):
+        case = Case(lens=[40, 130], heads=4, kv_heads=2, hd=hd, seed=12, dtype=dtype, fmt=fmt)
+        case.query = (case.query.float() * size).to(case.dtype)
         args, kw = case.args()
         out, lse = musa_aiter.kv_paged_attention_fp8(*args, **kw, softmax_scale=scale, return_lse=True)
         case.check(out, lse, scale=scale)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 96])
+@pytest.mark.parametrize("longest", [40, 2000])
+def test_outputs_of_the_smallest_fp16_values(hd, longest):
+    case = Case(lens=[40, 2000, 1], heads=4, kv_heads=2, hd=hd, seed=21, dtype="fp16", size=1.0)
+    for s in case.scales[1:]:
+        s *= 1e-5
+    args, kw = case.args()
+    out, lse = musa_aiter.kv_paged_attention_fp8(*args, **kw, return_lse=True, max_seq_len=longest)
+    got = case.check(out, lse)
+    assert ((got != 0) & (np.abs(got) < 2.0 ** -14)).any()
 
 
 def test_nan_and_infinite_queries_stay_in_their_rows():
