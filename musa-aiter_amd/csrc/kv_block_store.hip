@@ -8,9 +8,16 @@
 //   encode(decode(code) * s_old / s)
 // all in fp32 with one rounding per operation, so the result does not depend on how the work is cut.
 //
-// The tokens of a block may stand anywhere in the call.  One wave has one (block, plane, head, layer): the
-// block's leader, the token that owns the lowest written column, names the block, and the columns' tokens come
-// from the claim tags of the call (or, for few tokens, from the slots themselves, read by every workgroup).
+// The tokens of a block may stand anywhere in the call.  A block's leader, the token that owns its lowest written
+// column, names the block once; which token writes a column comes from the claim tags of the call or, for up to
+// kStoreScanTokens tokens, from the slots themselves, which every workgroup reads (one launch, no tags).
+//
+// A unit is one (block, plane, head, layer), done by one wave.  Where rows and blocks allow it (16-token groups
+// of columns, 8-dim pieces, 16-byte addresses) the wave loads 16-byte pieces of 4 tokens at a time, lane (tg, pc)
+// the tokens of columns 4 tg .. 4 tg + 3 and dims 8 pc .. 8 pc + 7, so that four codes of a dim are one dword of
+// the cache; two exchanges between the four lanes of a piece (v_permlane32_swap, v_permlane16_swap) then give
+// every lane whole 16-column rows of two dims.  Other shapes go element by element.
+// What bounds it: few tokens, latency (a token's row, its block's scale, the stores); many, memory.
 #include "kv_serving.h"
 
 namespace kvhip {
@@ -21,21 +28,8 @@ constexpr float kCodecMax = CODEC == kE4M3 ? 448.0f : 57344.0f;
 
 struct StoreArgs {
   BlockStoreParams p;
+  int32_t window;  // tokens per workgroup (claims form)
 };
-
-// Token that writes column `col` of `block`, or -1.
-__device__ __forceinline__ int64_t column_token(const BlockStoreParams& p, const int64_t* scan, int64_t block,
-                                                int64_t col) {
-  const int64_t slot = block * p.block_size + col;
-  if (p.owner != nullptr) {
-    const uint64_t tag = p.owner[slot];
-    return static_cast<uint32_t>(tag >> 32) == p.epoch ? static_cast<int64_t>(tag & 0xFFFFFFFFu) - 1 : -1;
-  }
-  int64_t found = -1;
-  for (int64_t t = 0; t < p.num_tokens; ++t)
-    if (scan[t] == slot) found = t;
-  return found;
-}
 
 template <int LDT>
 __device__ __forceinline__ float load_lin(const void* base, int64_t i) {
@@ -49,77 +43,305 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
-// One wave per (token, plane, head, layer); waves whose token leads no block end at once.
-template <int CODEC, int LDT>
-__global__ __launch_bounds__(kBlockThreads) void block_store_kernel(const StoreArgs a) {
-  const BlockStoreParams& p = a.p;
-  __shared__ int64_t scan[kStoreScanTokens];
-  __shared__ int refused;
-  if (refused_ahead(p.check)) return;
-  const int64_t slots_all = p.num_blocks * p.block_size;
-  if (p.owner == nullptr) {
-    if (threadIdx.x == 0) refused = 0;
-    __syncthreads();
-    for (int64_t t = threadIdx.x; t < p.num_tokens; t += kBlockThreads) {
-      const int64_t s = p.slots[t];
-      scan[t] = s;
-      if (s >= slots_all) refused = 1;
-    }
-    __syncthreads();
-    if (p.check.report != nullptr) {
-      if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0)
-        __hip_atomic_store(p.check.report, 2 * p.check.stamp + refused, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-      if (refused) return;
-    }
+// Which token writes a column of the block, or -1.
+struct TagColumns {
+  const uint64_t* tags;  // of the block's first column
+  uint32_t epoch;
+  __device__ __forceinline__ int32_t operator()(int64_t col) const {
+    const uint64_t tag = tags[col];
+    return static_cast<uint32_t>(tag >> 32) == epoch ? static_cast<int32_t>(tag & 0xFFFFFFFFu) - 1 : -1;
   }
-  const int64_t t = blockIdx.x;
-  const int64_t unit = static_cast<int64_t>(blockIdx.y) * kWavesPerBlock + wave_in_block();
-  if (unit >= 2 * p.num_heads) return;
-  const int64_t layer = blockIdx.z;
-  const int kv = static_cast<int>(unit & 1);
-  const int64_t head = unit >> 1;
-  const int64_t slot = p.slots[t];
-  if (slot < 0 || slot >= slots_all) return;
-  const int64_t block = slot / p.block_size, bs = p.block_size;
-  // Leader: this token owns its column, and no lower column is written.
-  bool leads = true;
-  for (int64_t c0 = 0; c0 <= slot - block * bs && leads; c0 += kWave) {
-    const int64_t col = c0 + lane_id();
-    const int64_t owner = col <= slot - block * bs ? column_token(p, scan, block, col) : -1;
-    leads = ballot(col < slot - block * bs ? owner >= 0 : col == slot - block * bs && owner != t) == 0;
-  }
-  if (!leads) return;
+};
+struct MapColumns {
+  const int32_t* map;  // LDS, token + 1 or 0
+  __device__ __forceinline__ int32_t operator()(int64_t col) const { return map[col] - 1; }
+};
 
-  const void* lin = p.lin[kv];
-  const int64_t lin0 = layer * p.lin_layer_stride + head * p.head_dim;
-  uint8_t* codes = p.cache[kv] + layer * p.layer_stride[kv] + block * p.block_stride[kv] + head * p.head_dim * bs;
-  float* scale = p.scale[kv] + (layer * p.num_blocks + block) * p.num_heads + head;
+struct Unit {
+  const uint8_t* lin;  // the head's first element of token 0
+  int64_t token_bytes;
+  uint8_t* codes;      // [head_dim][block_size]
+  float* scale;
+  int64_t hd, bs;
+};
+
+__device__ __forceinline__ Unit unit_of(const BlockStoreParams& p, int elt, int64_t block, int64_t layer, int64_t head,
+                                        int kv) {
+  Unit u;
+  u.lin = static_cast<const uint8_t*>(p.lin[kv]) + (layer * p.lin_layer_stride + head * p.head_dim) * elt;
+  u.token_bytes = p.lin_token_stride * elt;
+  u.codes = p.cache[kv] + layer * p.layer_stride[kv] + block * p.block_stride[kv] + head * p.head_dim * p.block_size;
+  u.scale = p.scale[kv] + (layer * p.num_blocks + block) * p.num_heads + head;
+  u.hd = p.head_dim;
+  u.bs = p.block_size;
+  return u;
+}
+
+template <int CODEC>
+__device__ __forceinline__ float new_scale(float most, float before, bool anew) {
+  const float now = fmaxf(div_rn(most, kCodecMax<CODEC>), kScaleFloor);
+  return anew ? now : fmaxf(now, before);
+}
+
+// ----- element by element -----------------------------------------------------------------------
+template <int CODEC, int LDT, typename COLUMNS>
+__device__ __forceinline__ void store_unit(const Unit& u, const COLUMNS& token_of) {
+  constexpr int kElt = LDT == kLinF32 ? 4 : 2;
   float most = 0.0f;
-  for (int64_t col = 0; col < bs; ++col) {
-    const int64_t tok = column_token(p, scan, block, col);
+  for (int64_t col = 0; col < u.bs; ++col) {
+    const int64_t tok = token_of(col);
     if (tok < 0) continue;
-    for (int64_t d = lane_id(); d < p.head_dim; d += kWave) {
-      const float x = fabsf(load_lin<LDT>(lin, lin0 + tok * p.lin_token_stride + d));
+    for (int64_t d = lane_id(); d < u.hd; d += kWave) {
+      const float x = fabsf(load_lin<LDT>(u.lin + tok * u.token_bytes, d));
       most = fmaxf(most, x < __builtin_inff() ? x : 0.0f);
     }
   }
   most = wave_max(most);
-  const float before = *scale;
-  const bool anew = slot == block * bs || scale_refused(before);
-  float now = fmaxf(div_rn(most, kCodecMax<CODEC>), kScaleFloor);
-  if (!anew) now = fmaxf(now, before);
-  for (int64_t col = 0; col < bs; ++col) {
-    const int64_t tok = column_token(p, scan, block, col);
+  const float before = *u.scale;
+  const bool anew = token_of(0) >= 0 || scale_refused(before);
+  const float now = new_scale<CODEC>(most, before, anew);
+  for (int64_t col = 0; col < u.bs; ++col) {
+    const int64_t tok = token_of(col);
     if (tok < 0 && !anew && now == before) continue;
-    for (int64_t d = lane_id(); d < p.head_dim; d += kWave) {
-      uint8_t* at = codes + d * bs + col;
+    for (int64_t d = lane_id(); d < u.hd; d += kWave) {
+      uint8_t* at = u.codes + d * u.bs + col;
       uint32_t code = 0;
-      if (tok >= 0) code = fp8_encode<CODEC>(div_rn(load_lin<LDT>(lin, lin0 + tok * p.lin_token_stride + d), now));
+      if (tok >= 0) code = fp8_encode<CODEC>(div_rn(load_lin<LDT>(u.lin + tok * u.token_bytes, d), now));
       else if (!anew) code = fp8_encode<CODEC>(div_rn(fp8_decode<CODEC>(*at) * before, now));
       *at = static_cast<uint8_t>(code);
     }
   }
-  if (lane_id() == 0) *scale = now;
+  static_assert(kElt == 4 || kElt == 2, "");
+  if (lane_id() == 0) *u.scale = now;
+}
+
+// ----- by 16-byte pieces ------------------------------------------------------------------------
+template <int LDT>
+struct Piece {  // 8 dims of a token
+  u32x4 raw[LDT == kLinF32 ? 2 : 1];
+  __device__ __forceinline__ float at(int j) const {
+    if constexpr (LDT == kLinF32) return __uint_as_float(raw[j >> 2][j & 3]);
+    else return lin_to_f32<LDT>(elem16(raw[0], j));
+  }
+};
+
+// The pieces of dims 128 `chunk` + 8 pc .. + 7 of the lane's four columns of group `group`; absent tokens are 0.
+template <int LDT>
+__device__ __forceinline__ void load_pieces(const Unit& u, const int32_t* tok, int chunk, Piece<LDT>* x) {
+  const int64_t d = 128 * chunk + 8 * (lane_id() & 15);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = Piece<LDT>{};
+    if (tok[i] >= 0 && d < u.hd) {
+      const uint8_t* p = u.lin + tok[i] * u.token_bytes + d * (LDT == kLinF32 ? 4 : 2);
+      x[i].raw[0] = ld16_cached(p);
+      if constexpr (LDT == kLinF32) x[i].raw[1] = ld16_cached(p + 16);
+    }
+  }
+}
+
+// Tokens of the lane's four columns of a group; returns which of its 16 columns are written.
+template <typename COLUMNS>
+__device__ __forceinline__ uint32_t group_tokens(const COLUMNS& token_of, int64_t group, int32_t* tok) {
+  const int32_t mine = token_of(16 * group + (lane_id() & 15));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) tok[i] = __shfl(mine, 4 * (lane_id() >> 4) + i);
+  return static_cast<uint32_t>(ballot(mine >= 0)) & 0xFFFFu;
+}
+
+template <int LDT>
+__device__ __forceinline__ void most_of(const Piece<LDT>* x, float* most, bool* odd) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v = fabsf(x[i].at(j));
+      const bool finite = v < __builtin_inff();
+      *odd |= !finite;
+      *most = fmaxf(*most, finite ? v : 0.0f);
+    }
+}
+
+// Bytes of columns 4 k .. 4 k + 3 that are written, as a mask of the dword.
+__device__ __forceinline__ uint32_t column_bytes(uint32_t written, int k) {
+  return (((written >> (4 * k) & 15u) * 0x00204081u) & 0x01010101u) * 0xFFu;
+}
+
+// The four lanes of a piece trade their dwords: in, dword j holds dim j of the lane's columns; out, row r holds
+// the 16 columns of dim 2 tg + r.
+__device__ __forceinline__ void trade(uint32_t* w, u32x4* row) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const auto s = __builtin_amdgcn_permlane32_swap(w[j], w[j + 4], false, false);
+    w[j] = s[0];
+    w[j + 4] = s[1];
+  }
+#pragma unroll
+  for (int j = 0; j < 8; j += 4)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const auto s = __builtin_amdgcn_permlane16_swap(w[j + r], w[j + 2 + r], false, false);
+      row[r][j / 2] = s[0];
+      row[r][j / 2 + 1] = s[1];
+    }
+}
+
+template <int CODEC>
+__device__ __forceinline__ uint32_t recode(uint32_t w, float before, float now) {
+  uint32_t out = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    out |= fp8_encode<CODEC>(div_rn(fp8_decode<CODEC>(w >> (8 * k) & 0xFFu) * before, now)) << (8 * k);
+  return out;
+}
+
+// HOLD: the block is one group of at most 128 dims, whose pieces stay in registers between the two passes; else
+// the second pass reads them again.
+template <int CODEC, int LDT, bool HOLD, typename COLUMNS>
+__device__ __forceinline__ void store_unit_pieces(const Unit& u, const COLUMNS& token_of) {
+  const int groups = HOLD ? 1 : static_cast<int>(u.bs >> 4), chunks = HOLD ? 1 : static_cast<int>((u.hd + 127) >> 7);
+  const float before = *u.scale;
+  float most = 0.0f;
+  bool odd = false;
+  int32_t tok[4];
+  uint32_t written = 0;
+  Piece<LDT> x[4];
+  for (int g = 0; g < groups; ++g) {
+    written = group_tokens(token_of, g, tok);
+    if (written == 0) continue;
+    for (int ch = 0; ch < chunks; ++ch) {
+      load_pieces<LDT>(u, tok, ch, x);
+      most_of<LDT>(x, &most, &odd);
+    }
+  }
+  most = wave_max(most);
+  const bool anew = token_of(0) >= 0 || scale_refused(before);
+  const float now = new_scale<CODEC>(most, before, anew);
+  const bool same = !anew && now == before;
+  // The quotient with one hoisted reciprocal is exact for scales in [2^-60, 2^60) and every finite value: a value
+  // so small that its residuals underflow has a quotient below 2^-40, which is flushed either way.
+  const bool exact = ballot(odd) == 0 && now < 0x1p60f;
+  const float r = div_rn(1.0f, now);
+  const int tg = lane_id() >> 4, pc = lane_id() & 15;
+  for (int g = 0; g < groups; ++g) {
+    if (!HOLD) written = group_tokens(token_of, g, tok);
+    if (written == 0 && same) continue;
+    for (int ch = 0; ch < chunks; ++ch) {
+      if (!HOLD) load_pieces<LDT>(u, tok, ch, x);
+      uint32_t w[8];
+      u32x4 row[2];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (exact) {
+          constexpr bool kNarrow = LDT != kLinF32;
+          w[j] = fp8_pack4_hw<CODEC>(quot_fast<kNarrow>(x[0].at(j), now, r), quot_fast<kNarrow>(x[1].at(j), now, r),
+                                     quot_fast<kNarrow>(x[2].at(j), now, r), quot_fast<kNarrow>(x[3].at(j), now, r));
+        } else {
+          w[j] = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[j] |= fp8_encode<CODEC>(div_rn(x[i].at(j), now)) << (8 * i);
+        }
+      }
+      trade(w, row);
+      const int64_t d = 128 * ch + 8 * pc + 2 * tg;
+      if (d >= u.hd) continue;
+      uint8_t* at = u.codes + d * u.bs + 16 * g;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (written != 0xFFFFu) {
+          u32x4 old = {0, 0, 0, 0};
+          if (!anew) old = ld16_cached(at + k * u.bs);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t m = column_bytes(written, q);
+            if (!anew && !same) old[q] = recode<CODEC>(old[q], before, now);
+            row[k][q] = (row[k][q] & m) | (old[q] & ~m);
+          }
+        }
+        st16_cached(at + k * u.bs, row[k]);
+      }
+    }
+  }
+  if (lane_id() == 0) *u.scale = now;
+}
+
+enum StoreForm : int { kElements = 0, kPieces = 1, kHeldPieces = 2 };
+
+template <int CODEC, int LDT, int FORM, typename COLUMNS>
+__device__ __forceinline__ void store_one(const BlockStoreParams& p, int64_t block, int64_t layer, int64_t unit,
+                                          const COLUMNS& token_of) {
+  const Unit u = unit_of(p, LDT == kLinF32 ? 4 : 2, block, layer, unit >> 1, static_cast<int>(unit & 1));
+  if constexpr (FORM == kElements) store_unit<CODEC, LDT>(u, token_of);
+  else store_unit_pieces<CODEC, LDT, FORM == kHeldPieces>(u, token_of);
+}
+
+// Few tokens: one workgroup per (token, four units, layer), which makes its block's columns from all the slots.
+template <int CODEC, int LDT, int FORM>
+__global__ __launch_bounds__(kBlockThreads) void block_store_scan_kernel(const StoreArgs a) {
+  const BlockStoreParams& p = a.p;
+  __shared__ int32_t map[kStoreScanColumns];
+  __shared__ int refused, lowest;
+  const int64_t bs = p.block_size, slots_all = p.num_blocks * bs;
+  const int64_t slot = p.slots[blockIdx.x];
+  const int64_t block = slot < 0 ? -1 : slot / bs;
+  const int64_t mine = threadIdx.x < p.num_tokens ? p.slots[threadIdx.x] : -1;
+  if (threadIdx.x == 0) {
+    refused = 0;
+    lowest = kStoreScanColumns;
+  }
+  for (int c = threadIdx.x; c < bs; c += kBlockThreads) map[c] = 0;
+  __syncthreads();
+  if (mine >= slots_all) refused = 1;
+  if (block >= 0 && mine >= block * bs && mine < (block + 1) * bs) {
+    const int col = static_cast<int>(mine - block * bs);
+    atomicMax(&map[col], static_cast<int>(threadIdx.x) + 1);
+    atomicMin(&lowest, col);
+  }
+  __syncthreads();
+  if (p.check.report != nullptr) {
+    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0)
+      __hip_atomic_store(p.check.report, 2 * p.check.stamp + refused, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    if (refused) return;
+  }
+  if (block < 0 || slot >= slots_all) return;
+  if (slot - block * bs != lowest || map[lowest] != static_cast<int>(blockIdx.x) + 1) return;
+  const int64_t unit = static_cast<int64_t>(blockIdx.y) * kWavesPerBlock + wave_in_block();
+  if (unit < 2 * p.num_heads) store_one<CODEC, LDT, FORM>(p, block, blockIdx.z, unit, MapColumns{map});
+}
+
+// Many tokens: one workgroup per (window of tokens, share of the units, layer).
+constexpr int kMostWindow = 64;
+
+template <int CODEC, int LDT, int FORM>
+__global__ __launch_bounds__(kBlockThreads) void block_store_tags_kernel(const StoreArgs a) {
+  const BlockStoreParams& p = a.p;
+  __shared__ int64_t leads[kMostWindow];
+  __shared__ int count;
+  if (refused_ahead(p.check)) return;
+  const int64_t bs = p.block_size;
+  if (threadIdx.x == 0) count = 0;
+  __syncthreads();
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * a.window + threadIdx.x;
+  if (static_cast<int>(threadIdx.x) < a.window && t < p.num_tokens) {
+    const int64_t slot = p.slots[t];
+    if (slot >= 0 && slot < p.num_blocks * bs) {
+      const int64_t block = slot / bs, col = slot - block * bs;
+      const TagColumns token_of{p.owner + block * bs, p.epoch};
+      bool lead = true;
+      for (int64_t c = 0; c < col && lead; ++c) lead = token_of(c) < 0;
+      if (lead && token_of(col) == t) leads[atomicAdd(&count, 1)] = block;
+    }
+  }
+  __syncthreads();
+  // The units of this workgroup's share of every block it leads, a wave each.
+  const int64_t share = (2 * p.num_heads + gridDim.y - 1) / gridDim.y;
+  const int64_t first = blockIdx.y * share;
+  const int64_t units = first + share < 2 * p.num_heads ? share : 2 * p.num_heads - first;
+  if (units <= 0) return;
+  for (int64_t i = wave_in_block(); i < count * units; i += kWavesPerBlock) {
+    const int64_t b = i / units, block = uniform64(leads[b]);
+    store_one<CODEC, LDT, FORM>(p, block, blockIdx.z, first + (i - b * units), TagColumns{p.owner + block * bs, p.epoch});
+  }
 }
 
 __global__ __launch_bounds__(kBlockThreads) void block_tag_reset_kernel(const int64_t* slots, int64_t n,
@@ -133,14 +355,40 @@ __global__ __launch_bounds__(kBlockThreads) void block_tag_reset_kernel(const in
   owner[s / bs * bs + (i - t * bs)] = 0;
 }
 
+template <int CODEC, int LDT, int FORM>
+hipError_t launch_form(const BlockStoreParams& p, hipStream_t stream) {
+  StoreArgs a{p, 0};
+  const uint32_t layers = static_cast<uint32_t>(p.num_layers);
+  if (p.owner == nullptr) {
+    const dim3 grid(static_cast<uint32_t>(p.num_tokens),
+                    static_cast<uint32_t>((2 * p.num_heads + kWavesPerBlock - 1) / kWavesPerBlock), layers);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(block_store_scan_kernel<CODEC, LDT, FORM>), grid, dim3(kBlockThreads), 0,
+                       stream, a);
+    return hipGetLastError();
+  }
+  // Windows as wide as leaves the chip enough workgroups: the tokens of a window may each lead a block.
+  a.window = kMostWindow;
+  while (a.window > kWavesPerBlock && p.num_tokens < int64_t{128} * a.window) a.window /= 2;
+  const int64_t windows = (p.num_tokens + a.window - 1) / a.window;
+  const int64_t shares = (2 * p.num_heads + kWavesPerBlock - 1) / kWavesPerBlock;
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(block_store_tags_kernel<CODEC, LDT, FORM>),
+                     dim3(static_cast<uint32_t>(windows), static_cast<uint32_t>(shares), layers), dim3(kBlockThreads),
+                     0, stream, a);
+  return hipGetLastError();
+}
+
 template <int CODEC, int LDT>
 hipError_t launch_typed(const BlockStoreParams& p, hipStream_t stream) {
-  const StoreArgs a{p};
-  const dim3 grid(static_cast<uint32_t>(p.num_tokens),
-                  static_cast<uint32_t>((2 * p.num_heads + kWavesPerBlock - 1) / kWavesPerBlock),
-                  static_cast<uint32_t>(p.num_layers));
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(block_store_kernel<CODEC, LDT>), grid, dim3(kBlockThreads), 0, stream, a);
-  return hipGetLastError();
+  const int64_t elt = LDT == kLinF32 ? 4 : 2;
+  uint64_t all = static_cast<uint64_t>(p.lin_token_stride * elt) | static_cast<uint64_t>(p.head_dim * elt) |
+                 static_cast<uint64_t>(p.num_layers > 1 ? p.lin_layer_stride * elt : 0) |
+                 static_cast<uint64_t>(p.block_size);
+  for (int kv = 0; kv < 2; ++kv)
+    all |= reinterpret_cast<uint64_t>(p.lin[kv]) | reinterpret_cast<uint64_t>(p.cache[kv]) |
+           static_cast<uint64_t>(p.block_stride[kv]) | static_cast<uint64_t>(p.num_layers > 1 ? p.layer_stride[kv] : 0);
+  if (all % 16 != 0 || p.head_dim % 8 != 0) return launch_form<CODEC, LDT, kElements>(p, stream);
+  if (p.block_size == 16 && p.head_dim <= 128) return launch_form<CODEC, LDT, kHeldPieces>(p, stream);
+  return launch_form<CODEC, LDT, kPieces>(p, stream);
 }
 
 template <int CODEC>
@@ -156,7 +404,7 @@ hipError_t launch_codec(const BlockStoreParams& p, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_block_store(const BlockStoreParams& p, hipStream_t stream) {
-  if (p.owner == nullptr && p.num_tokens > kStoreScanTokens) return hipErrorInvalidValue;
+  if (p.owner == nullptr && (p.num_tokens > kStoreScanTokens || p.block_size > kStoreScanColumns)) return hipErrorInvalidValue;
   return p.codec == kE4M3 ? launch_codec<kE4M3>(p, stream)
          : p.codec == kE5M2 ? launch_codec<kE5M2>(p, stream) : hipErrorInvalidValue;
 }

@@ -29,8 +29,10 @@ struct BlockStoreParams {
   CallCheck check;
 };
 
-// Tokens of a store that finds its blocks' columns by reading all slots in the kernel (one launch).
+// Tokens of a store that finds its blocks' columns by reading all slots in the kernel (one launch, a thread per
+// slot), and columns of a block that it has place for.
 constexpr int64_t kStoreScanTokens = 256;
+constexpr int64_t kStoreScanColumns = 1024;
 
 hipError_t launch_block_store(const BlockStoreParams& p, hipStream_t stream);
 // Zeroes the tags of every column of the blocks that the tokens write (calls captured into graphs).

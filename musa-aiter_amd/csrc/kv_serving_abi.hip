@@ -45,7 +45,7 @@ int block_store(const musa_aiter_hip_block_store_call& c, hipStream_t stream) {
   p.lin_layer_stride = c.lin_layer_stride;
   p.check.stamp = c.stamp;
   bool refused = false;
-  if (c.num_tokens <= kvhip::kStoreScanTokens) {
+  if (c.num_tokens <= kvhip::kStoreScanTokens && c.block_size <= kvhip::kStoreScanColumns) {
     // Every workgroup reads all slots, finds its block's columns among them and refuses the call by itself.
     p.check.report = c.report;
     hipError_t err = kvhip::launch_block_store(p, stream);

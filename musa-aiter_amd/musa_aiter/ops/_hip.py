@@ -861,7 +861,7 @@ def cachegen_decode(*, op: str, codes: torch.Tensor, table: torch.Tensor, out: t
 # musa_aiter_hip_block_store_call: linear, cache and scale pairs, slots, claims, report, guard, stamp, report words,
 # six sizes, linear strides, block and layer strides, codec and type.
 _BLOCK_STORE_CALL = struct.Struct("<6Q4Q2q6q2q4q2i")
-_BLOCK_STORE_SCAN = 256  # tokens up to which the kernel needs no claim tags
+_BLOCK_STORE_SCAN = (256, 1024)  # tokens and block size up to which the kernel needs no claim tags
 
 
 def block_store(*, op: str, device: torch.device, linear, caches, scales, slots: torch.Tensor, sizes, strides,
@@ -874,7 +874,7 @@ def block_store(*, op: str, device: torch.device, linear, caches, scales, slots:
         capturing = torch.cuda.is_current_stream_capturing()
         with stream_lock(key):
             claims, keep = 0, None
-            if sizes[1] > _BLOCK_STORE_SCAN:
+            if sizes[1] > _BLOCK_STORE_SCAN[0] or sizes[5] > _BLOCK_STORE_SCAN[1]:
                 claims, keep = claims_for(device, key, sizes[2] * sizes[5])
             report = guard = stamp = 0
             if not capturing:
