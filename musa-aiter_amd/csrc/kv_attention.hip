@@ -100,8 +100,10 @@ __device__ __forceinline__ float* part_acc(const AttnCall& c, int64_t s, int64_t
   return static_cast<float*>(c.workspace) + 2 * c.splits * c.rows * c.heads + (s * c.rows * c.heads + rh) * c.head_dim;
 }
 
-// Tokens of a part start at multiples of this.
+// A part begins at a multiple of a wave's 64 tokens and, but for the last one, holds whole turns of a workgroup's
+// four waves.
 constexpr int64_t kPartTokens = 64;
+constexpr int64_t kTurnTokens = kPartTokens * kWavesPerBlock;
 
 struct Span {
   int64_t lo, hi;
@@ -111,8 +113,8 @@ struct Span {
 __device__ __forceinline__ Span part_span(int64_t lo, int64_t hi, int64_t s, int64_t splits) {
   lo = lo / kPartTokens * kPartTokens;
   if (hi <= lo) return {lo, lo};
-  const int64_t tiles = (hi - lo + kPartTokens - 1) / kPartTokens;
-  const int64_t per = (tiles + splits - 1) / splits * kPartTokens;
+  const int64_t turns = (hi - lo + kTurnTokens - 1) / kTurnTokens;
+  const int64_t per = (turns + splits - 1) / splits * kTurnTokens;
   const int64_t from = lo + s * per;
   const int64_t to = from + per;
   return {from < hi ? from : hi, to < hi ? to : hi};
@@ -211,8 +213,11 @@ __global__ __launch_bounds__(kBlockThreads) void attention_any_kernel(const Attn
   for (int64_t d = threadIdx.x; d < c.head_dim; d += kBlockThreads) {
     float o = 0.0f;
     for (int w = 0; w < kWavesPerBlock; ++w) o += acc_of[w][d] * fade[w];
-    if (c.splits > 1) part_acc(c, split, rh)[d] = o;
-    else store_o<DT>(c.out, rh * c.head_dim + d, sum == 0.0f ? 0.0f : o / sum);
+    if (c.splits > 1) {
+      if (sum != 0.0f) part_acc(c, split, rh)[d] = o;
+      continue;
+    }
+    store_o<DT>(c.out, rh * c.head_dim + d, sum == 0.0f ? 0.0f : o / sum);
   }
   if (threadIdx.x == 0) {
     if (c.splits > 1) {
@@ -396,15 +401,17 @@ __device__ __forceinline__ void fill_loose_rows(const AttnCall& c, int64_t worke
   }
 }
 
-// Query rows as B operands: element j of step s of lane (x, g) is d = 32 s + 4 j + g of row x.
-template <int HDP, bool EXACT, int CODEC, int DT>
-struct QueryTile {
-  u32x4 q[kQueryParts<CODEC, DT>][HDP / 32];
-  float factor;  // scores times this (and the key scale) are in base 2
+// Query rows as B operands, in LDS (in registers they would cost every wave 16 for 128 dims and a third wave per
+// SIMD its place): element j of step s of lane (x, g) is d = 32 s + 4 j + g of row x.
+template <int HDP, int NT, int CODEC, int DT>
+struct QueryTiles {
+  u32x4 q[NT][kQueryParts<CODEC, DT>][HDP / 32][kWave];
+  float factor[NT][16];  // scores times this (and the key scale) are in base 2
 
-  // `row` is readable; without `mine` the row is zeros.
-  __device__ __forceinline__ void load(const RowsArgs& a, const uint16_t* row, bool mine) {
-    const int g = lane_id() >> 4;
+  // Rows of tile n by one wave; `row` is readable, and without `mine` the row is zeros.
+  template <bool EXACT>
+  __device__ __forceinline__ void fill(const RowsArgs& a, int n, const uint16_t* row, bool mine) {
+    const int x = lane_id() & 15, g = lane_id() >> 4;
     float most = 0.0f;
     uint16_t raw[HDP / 4];
 #pragma unroll
@@ -418,17 +425,25 @@ struct QueryTile {
     most = groups_max(most);
     const bool fine = most > 0.0f && most < __builtin_inff();
     const int up = fine ? Mma<CODEC>::kQueryTop - ilogbf(most) : 0;
-    factor = __builtin_ldexpf(static_cast<float>(a.c.softmax_scale) * kLog2e, Mma<CODEC>::kCodeShift - up);
+    if (g == 0)
+      factor[n][x] = __builtin_ldexpf(static_cast<float>(a.c.softmax_scale) * kLog2e, Mma<CODEC>::kCodeShift - up);
 #pragma unroll
-    for (int l = 0; l < HDP / 4; l += 2) {
-      float a = __builtin_ldexpf(query_value<DT>(raw[l]), up), b = __builtin_ldexpf(query_value<DT>(raw[l + 1]), up);
-      for (int part = 0; part < kQueryParts<CODEC, DT>; ++part) {
-        const uint32_t v = Mma<CODEC>::pack(a, b);
-        q[part][l / 8][l % 8 / 2] = v;
-        const f32x2 took = Mma<CODEC>::unpack(v);
-        a -= took[0];
-        b -= took[1];
+    for (int s = 0; s < HDP / 32; ++s) {
+      u32x4 v[kQueryParts<CODEC, DT>];
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        float lo = __builtin_ldexpf(query_value<DT>(raw[8 * s + j]), up);
+        float hi = __builtin_ldexpf(query_value<DT>(raw[8 * s + j + 1]), up);
+#pragma unroll
+        for (int part = 0; part < kQueryParts<CODEC, DT>; ++part) {
+          v[part][j / 2] = Mma<CODEC>::pack(lo, hi);
+          const f32x2 took = Mma<CODEC>::unpack(v[part][j / 2]);
+          lo -= took[0];
+          hi -= took[1];
+        }
       }
+#pragma unroll
+      for (int part = 0; part < kQueryParts<CODEC, DT>; ++part) q[n][part][s][lane_id()] = v[part];
     }
   }
 };
@@ -465,6 +480,12 @@ __device__ __forceinline__ uint32_t load4(const uint8_t* p) {
 // every tile: held over the loop, the rows' offsets take a register per load, and the registers ran out.
 __device__ __forceinline__ int not_hoisted(int v) {
   asm volatile("" : "+s"(v));
+  return v;
+}
+
+// The same for a value of the lanes: reads at places that follow from it stay where they are written.
+__device__ __forceinline__ int reread(int v) {
+  asm volatile("" : "+v"(v));
   return v;
 }
 
@@ -537,14 +558,20 @@ struct Sight {
 
 // Adds DIMS dims' part, from step FIRST on, of the scores of 16 * NT rows with 64 tokens, before scaling: element r
 // of product i is token 16 g + 4 r + i.
-template <int FIRST, int DIMS, int HDP, bool EXACT, int NT, int CODEC, int DT>
+template <int FIRST, int DIMS, int HDP, int NT, int CODEC, int DT>
 __device__ __forceinline__ void key_products(const Mma<CODEC>& mma, const uint32_t* k,
-                                             const QueryTile<HDP, EXACT, CODEC, DT>* q, f32x4 (*score)[4]) {
+                                             const QueryTiles<HDP, NT, CODEC, DT>& queries, f32x4 (*score)[4]) {
+  const int lane = reread(lane_id());
 #pragma unroll
   for (int step = 0; step < DIMS / 32; ++step) {
     uint32_t w[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) w[j] = mma.prepare(k[8 * step + j]);
+    u32x4 q[NT][kQueryParts<CODEC, DT>];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int part = 0; part < kQueryParts<CODEC, DT>; ++part) q[n][part] = queries.q[n][part][FIRST + step][lane];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       u32x4 a;
@@ -556,7 +583,7 @@ __device__ __forceinline__ void key_products(const Mma<CODEC>& mma, const uint32
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int part = 0; part < kQueryParts<CODEC, DT>; ++part)
-          score[n][i] = Mma<CODEC>::mma(a, q[n].q[part][FIRST + step], score[n][i]);
+          score[n][i] = Mma<CODEC>::mma(a, q[n][part], score[n][i]);
     }
   }
 }
@@ -652,10 +679,16 @@ __device__ __forceinline__ void value_products(const Mma<CODEC>& mma, const u32x
 // what they have in LDS, 128 dims at a time.  A wave loads the next tile's keys once this tile's are used up and
 // its values behind this tile's, so either the one or the other is on its way all the time.
 constexpr int kJoinDims = 128;
+
+// Waves per SIMD that the registers of a variant leave room for (without spills; looked up in the compiler's report).
+constexpr int rows_occupancy(int hdp, bool exact, int tiles, int codec) {
+  if (hdp * tiles > 128) return 1;
+  return tiles > 1 || (hdp == 128 && (!exact || codec == kE5M2)) ? 2 : 3;
+}
 constexpr int kJoinStride = kJoinDims + 4;
 
 template <int HDP, bool EXACT, int NT, int CODEC, int DT>
-__global__ __launch_bounds__(kBlockThreads, HDP * NT <= 128 ? 2 : 1)
+__global__ __launch_bounds__(kBlockThreads, rows_occupancy(HDP, EXACT, NT, CODEC))
 void attention_rows_kernel(const RowsArgs a) {
   const AttnCall& c = a.c;
   constexpr int kRows = 16 * NT;
@@ -668,10 +701,46 @@ void attention_rows_kernel(const RowsArgs a) {
   const int32_t len = said < 0 ? 0 : said < kMostLen ? static_cast<int32_t>(said) : kMostLen;
   const int32_t group = a.group, in_seq = tile.count * group;
   const int32_t before = len - tile.count;  // position of the sequence's first row
-  const Mma<CODEC> mma;
+  const int32_t pos_lo = before + tile.base / group, pos_hi = before + (min(tile.base + kRows, in_seq) - 1) / group;
+  const int32_t end = min(pos_hi + 1, a.room);
+  const int32_t begin = a.window > 0 ? max(pos_lo - a.window + 1, 0) : 0;
+  // Tiles inside [all_lo, all_hi) are seen whole by every row.
+  const int32_t all_lo = a.window > 0 ? max(pos_hi - a.window + 1, 0) : 0;
+  const Span span = part_span(begin, end, split, a.splits);
+  const int32_t last = static_cast<int32_t>(span.hi), all_hi = min(pos_lo + 1, last);
+  if (a.splits > 1 && span.lo >= span.hi) {  // nothing to do: the rows' parts say so
+    for (int n = threadIdx.x; n < kRows; n += kBlockThreads) {
+      const int32_t r = tile.base + n;
+      if (r >= in_seq) break;
+      float* ml = part_ml(c, split, static_cast<int64_t>(tile.first + r / group) * a.heads + head * group + r % group);
+      ml[0] = -__builtin_inff();
+      ml[1] = 0.0f;
+    }
+    return;
+  }
+  const int64_t head_off = static_cast<int64_t>(head) * a.hd * a.bs;
+  const uint8_t* row = static_cast<const uint8_t*>(c.tables) +
+                       tile.seq * c.table_stride * (c.wide_tables ? 8 : 4);
 
-  // Rows and what they see.
-  QueryTile<HDP, EXACT, CODEC, DT> q[NT];
+  constexpr int32_t kStep = kWavesPerBlock * kWaveTokens;
+  // 256 dims go in two halves through the same registers.
+  constexpr int kDims = HDP <= 128 ? HDP : HDP / 2;
+  int32_t token = static_cast<int32_t>(span.lo) + wave * kWaveTokens;
+  uint32_t k[kDims / 4];
+  u32x4 v[kDims / 16];
+  GroupIds ids, next_ids;
+  GroupScales scales;
+  if (token < last) {  // on their way while the queries are read
+    ids = tile_ids(a, row, token, last);
+    next_ids = tile_ids(a, row, token + kStep, last);
+    scales = load_scales(c, head, ids);
+    load_keys<kDims, EXACT>(a, head_off, ids, 0, k);
+    load_values<kDims, EXACT>(a, head_off, ids, 0, v);
+  }
+
+  const Mma<CODEC> mma;
+  // Rows and what they see; the waves share the queries.
+  __shared__ QueryTiles<HDP, NT, CODEC, DT> queries;
   RowState<HDP> state[NT];
   Sight sight[NT];
 #pragma unroll
@@ -680,8 +749,9 @@ void attention_rows_kernel(const RowsArgs a) {
     const bool mine = r < in_seq;
     const int32_t i = mine ? r / group : 0, h = mine ? r - i * group : 0;
     const int32_t pos = before + i;
-    q[n].load(a, static_cast<const uint16_t*>(c.query) + (tile.first + i) * c.query_row_stride +
-                     (head * group + h) * c.query_head_stride, mine);
+    if (wave == n)
+      queries.template fill<EXACT>(a, n, static_cast<const uint16_t*>(c.query) + (tile.first + i) * c.query_row_stride +
+                                             (head * group + h) * c.query_head_stride, mine);
     sight[n].hi = mine ? min(pos + 1, a.room) : 0;
     sight[n].lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
     state[n].m = -__builtin_inff();
@@ -689,43 +759,31 @@ void attention_rows_kernel(const RowsArgs a) {
 #pragma unroll
     for (int l = 0; l < HDP / 16; ++l) state[n].acc[l] = f32x4{0, 0, 0, 0};
   }
-  const int32_t pos_lo = before + tile.base / group, pos_hi = before + (min(tile.base + kRows, in_seq) - 1) / group;
-  const int32_t end = min(pos_hi + 1, a.room);
-  const int32_t begin = a.window > 0 ? max(pos_lo - a.window + 1, 0) : 0;
-  // Tiles inside [all_lo, all_hi) are seen whole by every row.
-  const int32_t all_lo = a.window > 0 ? max(pos_hi - a.window + 1, 0) : 0;
-  const Span span = part_span(begin, end, split, a.splits);
-  const int32_t last = static_cast<int32_t>(span.hi), all_hi = min(pos_lo + 1, last);
-  const int64_t head_off = static_cast<int64_t>(head) * a.hd * a.bs;
-  const uint8_t* row = static_cast<const uint8_t*>(c.tables) +
-                       tile.seq * c.table_stride * (c.wide_tables ? 8 : 4);
+  __syncthreads();
 
-  constexpr int32_t kStep = kWavesPerBlock * kWaveTokens;
-  int32_t token = static_cast<int32_t>(span.lo) + wave * kWaveTokens;
   if (token < last) {
-    // 256 dims go in two halves through the same registers.
-    constexpr int kDims = HDP <= 128 ? HDP : HDP / 2;
-    uint32_t k[kDims / 4];
-    u32x4 v[kDims / 16];
-    GroupIds ids = tile_ids(a, row, token, last);
-    load_keys<kDims, EXACT>(a, head_off, ids, 0, k);
-    load_values<kDims, EXACT>(a, head_off, ids, 0, v);
     for (;;) {
-      const GroupScales scales = load_scales(c, head, ids);
       const int32_t next = token + kStep;
-      const GroupIds next_ids = tile_ids(a, row, next, last);
       f32x4 score[NT][4] = {};
-      key_products<0, kDims, HDP, EXACT, NT, CODEC, DT>(mma, k, q, score);
+      key_products<0, kDims, HDP, NT, CODEC, DT>(mma, k, queries, score);
       if constexpr (HDP > kDims) {
         load_keys<kDims, EXACT>(a, head_off, ids, kDims, k);
-        key_products<kDims / 32, kDims, HDP, EXACT, NT, CODEC, DT>(mma, k, q, score);
+        key_products<kDims / 32, kDims, HDP, NT, CODEC, DT>(mma, k, queries, score);
       }
-      if (next < last) load_keys<kDims, EXACT>(a, head_off, next_ids, 0, k);
+      // Loads return in order: table entries are read two tiles ahead, in front of the keys whose arrival they
+      // would else be waited for with.
+      GroupIds later_ids;
+      GroupScales next_scales;
+      if (next < last) {
+        later_ids = tile_ids(a, row, next + kStep, last);
+        next_scales = load_scales(c, head, next_ids);
+        load_keys<kDims, EXACT>(a, head_off, next_ids, 0, k);
+      }
       const bool masked = token < all_lo || token + kWaveTokens > all_hi || ballot(!scales.seen) != 0;
       u32x4 p[NT][2][kWeightParts<CODEC, DT>];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        soften<HDP, CODEC>(score[n], q[n].factor, scales, masked, token, sight[n], state[n]);
+        soften<HDP, CODEC>(score[n], queries.factor[n][x], scales, masked, token, sight[n], state[n]);
         pack_weights<CODEC, DT>(score[n], 0, p[n][0]);
         pack_weights<CODEC, DT>(score[n], 1, p[n][1]);
       }
@@ -737,6 +795,8 @@ void attention_rows_kernel(const RowsArgs a) {
       if (next >= last) break;
       load_values<kDims, EXACT>(a, head_off, next_ids, 0, v);
       ids = next_ids;
+      next_ids = later_ids;
+      scales = next_scales;
       token = next;
     }
   }
@@ -783,8 +843,11 @@ void attention_rows_kernel(const RowsArgs a) {
         for (int w = 0; w < kWavesPerBlock; ++w) o += joined[w][at][k] * fade[w];
         o *= back;
         if (!EXACT && d0 + k >= a.hd) continue;
-        if (a.splits > 1) part_acc(c, split, rh)[d0 + k] = o;
-        else store_o<DT>(c.out, rh * a.hd + d0 + k, sum == 0.0f ? 0.0f : o / sum);
+        if (a.splits > 1) {
+          if (sum != 0.0f) part_acc(c, split, rh)[d0 + k] = o;
+          continue;
+        }
+        store_o<DT>(c.out, rh * a.hd + d0 + k, sum == 0.0f ? 0.0f : o / sum);
       }
       if (d0 == 0 && (threadIdx.x & 15) == 0) {
         if (a.splits > 1) {
@@ -798,31 +861,57 @@ void attention_rows_kernel(const RowsArgs a) {
   }
 }
 
-// ----- joining the parts: one wave per (row, head) -------------------------------------------------
+// ----- joining the parts: one workgroup per (row, head) ---------------------------------------------
+// Lane s holds part s's maximum and sum; the waves add up the parts' results by turns, and the first one stores
+// their sum.  Parts that saw nothing hold no result and are not read.
+constexpr int kMostSplits = kWave;
+
 template <int DT>
 __global__ __launch_bounds__(kBlockThreads) void attention_join_kernel(const AttnCall c) {
-  const int64_t rh = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave_in_block();
-  if (rh >= c.rows * c.heads) return;
-  const int64_t t = rh / c.heads;
-  if (row_sequence(c, t).seq < 0) return;  // no parts
-  float top = -__builtin_inff();
-  for (int64_t s = 0; s < c.splits; ++s) top = fmaxf(top, part_ml(c, s, rh)[0]);
-  const float ref = top == -__builtin_inff() ? 0.0f : top;
-  float sum = 0.0f;
-  for (int64_t s = 0; s < c.splits; ++s) sum += part_ml(c, s, rh)[1] * __builtin_amdgcn_exp2f(part_ml(c, s, rh)[0] - ref);
-  for (int64_t d = lane_id(); d < c.head_dim; d += kWave) {
-    float o = 0.0f;
-    for (int64_t s = 0; s < c.splits; ++s)
-      o += part_acc(c, s, rh)[d] * __builtin_amdgcn_exp2f(part_ml(c, s, rh)[0] - ref);
-    store_o<DT>(c.out, rh * c.head_dim + d, sum == 0.0f ? 0.0f : o / sum);
+  const int64_t rh = blockIdx.x;
+  const int lane = lane_id(), wave = wave_in_block();
+  const int hd = static_cast<int>(c.head_dim), splits = static_cast<int>(c.splits);
+  __shared__ float sums[kWavesPerBlock - 1][kAnyMaxDim];
+  float m = -__builtin_inff(), l = 0.0f;
+  if (lane < splits) {
+    m = part_ml(c, lane, rh)[0];
+    l = part_ml(c, lane, rh)[1];
   }
-  if (c.lse != nullptr && lane_id() == 0) c.lse[rh] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * kLn2;
+  if (row_sequence(c, rh / c.heads).seq < 0) return;  // no parts: what was read is not looked at
+  const float top = wave_max(m);
+  const float ref = top == -__builtin_inff() ? 0.0f : top;
+  const float fade = __builtin_amdgcn_exp2f(m - ref);
+  const float sum = wave_sum(l * fade);
+  const uint64_t full = ballot(l != 0.0f);
+  float acc[kAnyMaxDim / kWave] = {};
+  for (int s = wave; s < splits; s += kWavesPerBlock) {
+    if ((full >> s & 1) == 0) continue;
+    const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(fade), s));
+    const float* part = part_acc(c, s, rh);
+#pragma unroll
+    for (int i = 0; i < kAnyMaxDim / kWave; ++i)
+      if (lane + i * kWave < hd) acc[i] = __builtin_fmaf(part[lane + i * kWave], f, acc[i]);
+  }
+  if (wave > 0)
+#pragma unroll
+    for (int i = 0; i < kAnyMaxDim / kWave; ++i)
+      if (lane + i * kWave < hd) sums[wave - 1][lane + i * kWave] = acc[i];
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int i = 0; i < kAnyMaxDim / kWave; ++i) {
+    const int d = lane + i * kWave;
+    if (d >= hd) continue;
+    float o = acc[i];
+    for (int w = 0; w < kWavesPerBlock - 1; ++w) o += sums[w][d];
+    store_o<DT>(c.out, rh * hd + d, sum == 0.0f ? 0.0f : o / sum);
+  }
+  if (c.lse != nullptr && lane == 0) c.lse[rh] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * kLn2;
 }
 
 template <int DT>
 hipError_t launch_join(const AttnCall& c, hipStream_t stream) {
-  const int64_t groups = (c.rows * c.heads + kWavesPerBlock - 1) / kWavesPerBlock;
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<DT>), dim3(static_cast<uint32_t>(groups)),
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<DT>), dim3(static_cast<uint32_t>(c.rows * c.heads)),
                      dim3(kBlockThreads), 0, stream, c);
   return hipGetLastError();
 }
@@ -917,7 +1006,7 @@ int64_t attention_splits(const AttnCall& c, int64_t longest) {
   int64_t splits = groups > 0 ? (1024 + groups - 1) / groups : 1;
   const int64_t most = (longest + 255) / 256;
   splits = splits < most ? splits : most;
-  return splits < 1 ? 1 : splits > 64 ? 64 : splits;
+  return splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : splits;
 }
 
 int64_t attention_workspace(const AttnCall& c) {

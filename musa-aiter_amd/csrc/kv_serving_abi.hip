@@ -95,7 +95,7 @@ bool attention_sizes_ok(const musa_aiter_hip_attention_call& c) {
 
 int attention(const musa_aiter_hip_attention_call& c, hipStream_t stream) {
   if (!attention_sizes_ok(c) || c.dtype < 0 || c.dtype > 2 || (c.codec != kvhip::kE4M3 && c.codec != kvhip::kE5M2) ||
-      c.splits < 1 || c.splits > 65535)
+      c.splits < 1 || c.splits > 64)
     return hipErrorInvalidValue;
   if (c.rows == 0) return hipSuccess;
   if (c.query == nullptr || c.out == nullptr || (c.batch > 0 && c.lens == nullptr) ||
