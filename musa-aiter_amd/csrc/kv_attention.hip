@@ -92,12 +92,13 @@ __device__ __forceinline__ void store_o(void* base, int64_t i, float v) {
   else static_cast<uint16_t*>(base)[i] = static_cast<uint16_t>(f32_to_lin<DT>(v));
 }
 
-// Partial results of split s: m and l at [s, row, head], then acc at [s, row, head, dim].
-__device__ __forceinline__ float* part_ml(const AttnCall& c, int64_t s, int64_t rh) {
-  return static_cast<float*>(c.workspace) + 2 * (s * c.rows * c.heads + rh);
+// Partial results in the workspace: (m, l) of `count` parts, then their acc of head_dim values each.  With splits
+// > 1 part s of (row, head) rh is s * rows * heads + rh; with an even cut (splits 0) see FlowCut.
+__device__ __forceinline__ float* part_ml(const AttnCall& c, int64_t part) {
+  return static_cast<float*>(c.workspace) + 2 * part;
 }
-__device__ __forceinline__ float* part_acc(const AttnCall& c, int64_t s, int64_t rh) {
-  return static_cast<float*>(c.workspace) + 2 * c.splits * c.rows * c.heads + (s * c.rows * c.heads + rh) * c.head_dim;
+__device__ __forceinline__ float* part_acc(const AttnCall& c, int64_t count, int64_t part) {
+  return static_cast<float*>(c.workspace) + 2 * count + part * c.head_dim;
 }
 
 // A part begins at a multiple of a wave's 64 tokens and, but for the last one, holds whole turns of a workgroup's
@@ -214,15 +215,15 @@ __global__ __launch_bounds__(kBlockThreads) void attention_any_kernel(const Attn
     float o = 0.0f;
     for (int w = 0; w < kWavesPerBlock; ++w) o += acc_of[w][d] * fade[w];
     if (c.splits > 1) {
-      if (sum != 0.0f) part_acc(c, split, rh)[d] = o;
+      if (sum != 0.0f) part_acc(c, c.splits * c.rows * c.heads, split * c.rows * c.heads + rh)[d] = o;
       continue;
     }
     store_o<DT>(c.out, rh * c.head_dim + d, sum == 0.0f ? 0.0f : o / sum);
   }
   if (threadIdx.x == 0) {
     if (c.splits > 1) {
-      part_ml(c, split, rh)[0] = top;
-      part_ml(c, split, rh)[1] = sum;
+      part_ml(c, split * c.rows * c.heads + rh)[0] = top;
+      part_ml(c, split * c.rows * c.heads + rh)[1] = sum;
     } else if (c.lse != nullptr) {
       c.lse[rh] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * kLn2;
     }
@@ -326,6 +327,18 @@ constexpr int kQueryParts = CODEC == kE5M2 && DT == kLinF16 ? 2 : 1;
 template <int CODEC, int DT>
 constexpr int kWeightParts = CODEC == kE5M2 || DT == kLinF16 ? 2 : 1;
 
+// Values that the compiler takes for new ones, so that what follows from them is computed (or read) again where it
+// is written.  Held over the loops, the offsets of every load and the like take more registers than there are.
+__device__ __forceinline__ int not_hoisted(int v) {  // uniform
+  asm volatile("" : "+s"(v));
+  return v;
+}
+__device__ __forceinline__ int reread(int v) {  // of the lanes
+  asm volatile("" : "+v"(v));
+  return v;
+}
+__device__ __forceinline__ int lane_now() { return reread(lane_id()); }
+
 // Maximum and sum over the four lane groups of 16.
 __device__ __forceinline__ float groups_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16));
@@ -411,7 +424,7 @@ struct QueryTiles {
   // Rows of tile n by one wave; `row` is readable, and without `mine` the row is zeros.
   template <bool EXACT>
   __device__ __forceinline__ void fill(const RowsArgs& a, int n, const uint16_t* row, bool mine) {
-    const int x = lane_id() & 15, g = lane_id() >> 4;
+    const int lane = lane_now(), x = lane & 15, g = lane >> 4;
     float most = 0.0f;
     uint16_t raw[HDP / 4];
 #pragma unroll
@@ -443,63 +456,53 @@ struct QueryTiles {
         }
       }
 #pragma unroll
-      for (int part = 0; part < kQueryParts<CODEC, DT>; ++part) q[n][part][s][lane_id()] = v[part];
+      for (int part = 0; part < kQueryParts<CODEC, DT>; ++part) q[n][part][s][lane] = v[part];
     }
   }
 };
 
-// Table entry of the 16-token group that begins at `token` (multiple of 16), or -1; *inside: token in its block.
-__device__ __forceinline__ int32_t group_block(const RowsArgs& a, const uint8_t* row, int32_t token, int32_t end,
-                                               int32_t* inside) {
-  const uint32_t n16 = static_cast<uint32_t>(token) >> 4, b16 = static_cast<uint32_t>(a.bs) >> 4;
-  const uint32_t j = a.block_shift >= 0 ? n16 >> a.block_shift : n16 / b16;
-  *inside = static_cast<int32_t>((n16 - j * b16) << 4);
+// Table column of the 16-token group that begins at `token` (a multiple of 16).
+__device__ __forceinline__ uint32_t group_column(const RowsArgs& a, int32_t token) {
+  const uint32_t n16 = static_cast<uint32_t>(token) >> 4;
+  return a.block_shift >= 0 ? n16 >> a.block_shift : n16 / (static_cast<uint32_t>(a.bs) >> 4);
+}
+
+// Its first token's place in the block.
+__device__ __forceinline__ int32_t group_place(const RowsArgs& a, int32_t token) {
+  return token - static_cast<int32_t>(group_column(a, token)) * a.bs;
+}
+
+// The block of the group, or -1.
+__device__ __forceinline__ int32_t group_block(const RowsArgs& a, const uint8_t* row, int32_t token, int32_t end) {
   if (token >= end) return -1;
-  const int64_t blk = int_at(row, j, a.c.wide_tables);
+  const int64_t blk = int_at(row, group_column(a, token), a.c.wide_tables);
   return blk >= 0 && blk < a.num_blocks ? static_cast<int32_t>(blk) : -1;
 }
 
 struct GroupIds {
-  int32_t k, v;          // blocks of the groups whose keys and values the lane loads
-  int32_t k_in, v_in;
+  int32_t k, v;  // blocks of the groups whose keys and values the lane loads
 };
 
 __device__ __forceinline__ GroupIds tile_ids(const RowsArgs& a, const uint8_t* row, int32_t token, int32_t end) {
-  const int x = lane_id() & 15, g = lane_id() >> 4;
-  GroupIds ids;
-  ids.k = group_block(a, row, token + 16 * (x >> 2), end, &ids.k_in);
-  ids.v = group_block(a, row, token + 16 * g, end, &ids.v_in);
-  return ids;
+  const int lane = lane_now(), x = lane & 15, g = lane >> 4;
+  return {group_block(a, row, token + 16 * (x >> 2), end), group_block(a, row, token + 16 * g, end)};
 }
 
 __device__ __forceinline__ uint32_t load4(const uint8_t* p) {
   return *reinterpret_cast<const KVHIP_GLOBAL uint32_t*>(reinterpret_cast<uint64_t>(p));
 }
 
-// A uniform value that the compiler takes for a new one, so that what follows from it is computed again for
-// every tile: held over the loop, the rows' offsets take a register per load, and the registers ran out.
-__device__ __forceinline__ int not_hoisted(int v) {
-  asm volatile("" : "+s"(v));
-  return v;
-}
-
-// The same for a value of the lanes: reads at places that follow from it stay where they are written.
-__device__ __forceinline__ int reread(int v) {
-  asm volatile("" : "+v"(v));
-  return v;
-}
-
 // DIMS rows of the keys of 64 tokens: dword l is row d = first + 4 l + g of the lane's 4 tokens.  A group without a block reads block
 // 0, which every cache has; its scores are masked.  Without EXACT rows past head_dim read the last one: the
 // query is zero there.
 template <int DIMS, bool EXACT>
-__device__ __forceinline__ void load_keys(const RowsArgs& a, int64_t head_off, const GroupIds& ids, int first,
-                                          uint32_t* k) {
+__device__ __forceinline__ void load_keys(const RowsArgs& a, int64_t head_off, int32_t token, const GroupIds& ids,
+                                          int first, uint32_t* k) {
   const AttnCall& c = a.c;
-  const int x = lane_id() & 15, g = lane_id() >> 4;
+  const int lane = lane_now(), x = lane & 15, g = lane >> 4;
   const int32_t bs = a.bs;
   const uint8_t* p = static_cast<const uint8_t*>(c.cache[0]) + static_cast<int64_t>(ids.k < 0 ? 0 : ids.k) *
-                     c.cache_block_stride[0] + head_off + ids.k_in + 4 * (x & 3);
+                     c.cache_block_stride[0] + head_off + group_place(a, token + 16 * (x >> 2)) + 4 * (x & 3);
   if constexpr (EXACT) {
     p += (first + g) * bs;
 #pragma unroll
@@ -526,13 +529,14 @@ __device__ __forceinline__ GroupScales load_scales(const AttnCall& c, int32_t he
 // DIMS rows of the values of 64 tokens: piece l is row d = first + 16 l + x of the 16 tokens of group g (rows past
 // head_dim as above: outputs past it are not stored).
 template <int DIMS, bool EXACT>
-__device__ __forceinline__ void load_values(const RowsArgs& a, int64_t head_off, const GroupIds& ids, int first,
-                                            u32x4* v) {
+__device__ __forceinline__ void load_values(const RowsArgs& a, int64_t head_off, int32_t token, const GroupIds& ids,
+                                            int first, u32x4* v) {
   const AttnCall& c = a.c;
-  const int x = lane_id() & 15;
+  const int lane = lane_now(), x = lane & 15;
   const int32_t bs = a.bs;
   const int64_t blk = ids.v < 0 ? 0 : ids.v;
-  const uint8_t* p = static_cast<const uint8_t*>(c.cache[1]) + blk * c.cache_block_stride[1] + head_off + ids.v_in;
+  const uint8_t* p = static_cast<const uint8_t*>(c.cache[1]) + blk * c.cache_block_stride[1] + head_off +
+                     group_place(a, token + 16 * (lane >> 4));
   if constexpr (EXACT) {
     p += (first + x) * bs;
 #pragma unroll
@@ -561,7 +565,7 @@ struct Sight {
 template <int FIRST, int DIMS, int HDP, int NT, int CODEC, int DT>
 __device__ __forceinline__ void key_products(const Mma<CODEC>& mma, const uint32_t* k,
                                              const QueryTiles<HDP, NT, CODEC, DT>& queries, f32x4 (*score)[4]) {
-  const int lane = reread(lane_id());
+  const int lane = lane_now();
 #pragma unroll
   for (int step = 0; step < DIMS / 32; ++step) {
     uint32_t w[8];
@@ -598,7 +602,7 @@ __device__ __forceinline__ void soften(f32x4* score, float factor, const GroupSc
 #pragma unroll
   for (int i = 0; i < 4; ++i) score[i] *= f;
   if (masked) {
-    const int first = token + 16 * (lane_id() >> 4);
+    const int first = token + 16 * (lane_now() >> 4);
     const int lo = sight.lo - first, hi = seen ? sight.hi - first : 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -687,37 +691,51 @@ constexpr int rows_occupancy(int hdp, bool exact, int tiles, int codec) {
 }
 constexpr int kJoinStride = kJoinDims + 4;
 
-template <int HDP, bool EXACT, int NT, int CODEC, int DT>
-__global__ __launch_bounds__(kBlockThreads, rows_occupancy(HDP, EXACT, NT, CODEC))
-void attention_rows_kernel(const RowsArgs a) {
-  const AttnCall& c = a.c;
-  constexpr int kRows = 16 * NT;
-  const int32_t head = blockIdx.y, split = blockIdx.z;
-  const RowTile tile = find_tile(a, blockIdx.x, kRows);
-  if (c.starts != nullptr && c.fill_rows && head == 0 && split == 0) fill_loose_rows<DT>(c, blockIdx.x, gridDim.x);
-  if (tile.seq < 0) return;
-  const int x = lane_id() & 15, wave = wave_in_block();
-  const int64_t said = seq_len(c, tile.seq);
+// A row tile's work on cached tokens [lo, hi), and where its result goes: the output (parts 0), or the `parts` of
+// the workspace, row r of the tile to part first_part + r or, with by_row, first_part + its (row, head) number.
+struct Segment {
+  RowTile tile;
+  int32_t head, lo, hi;
+  int64_t parts, first_part;
+  bool by_row;
+};
+
+// Positions that the rows of a tile see between them.
+struct Reach {
+  int32_t before;           // position of the sequence's first row
+  int32_t pos_lo, pos_hi;   // of the tile's first and last row
+  int32_t begin, end;       // seen by any row
+};
+
+__device__ __forceinline__ Reach tile_reach(const RowsArgs& a, const RowTile& tile, int rows) {
+  const int64_t said = seq_len(a.c, tile.seq);
   const int32_t len = said < 0 ? 0 : said < kMostLen ? static_cast<int32_t>(said) : kMostLen;
-  const int32_t group = a.group, in_seq = tile.count * group;
-  const int32_t before = len - tile.count;  // position of the sequence's first row
-  const int32_t pos_lo = before + tile.base / group, pos_hi = before + (min(tile.base + kRows, in_seq) - 1) / group;
-  const int32_t end = min(pos_hi + 1, a.room);
-  const int32_t begin = a.window > 0 ? max(pos_lo - a.window + 1, 0) : 0;
-  // Tiles inside [all_lo, all_hi) are seen whole by every row.
-  const int32_t all_lo = a.window > 0 ? max(pos_hi - a.window + 1, 0) : 0;
-  const Span span = part_span(begin, end, split, a.splits);
-  const int32_t last = static_cast<int32_t>(span.hi), all_hi = min(pos_lo + 1, last);
-  if (a.splits > 1 && span.lo >= span.hi) {  // nothing to do: the rows' parts say so
-    for (int n = threadIdx.x; n < kRows; n += kBlockThreads) {
-      const int32_t r = tile.base + n;
-      if (r >= in_seq) break;
-      float* ml = part_ml(c, split, static_cast<int64_t>(tile.first + r / group) * a.heads + head * group + r % group);
-      ml[0] = -__builtin_inff();
-      ml[1] = 0.0f;
-    }
-    return;
-  }
+  Reach r;
+  r.before = len - tile.count;
+  r.pos_lo = r.before + tile.base / a.group;
+  r.pos_hi = r.before + (min(tile.base + rows, tile.count * a.group) - 1) / a.group;
+  r.end = min(r.pos_hi + 1, a.room);
+  r.begin = a.window > 0 ? max(r.pos_lo - a.window + 1, 0) : 0;
+  return r;
+}
+
+template <int HDP, int NT, int CODEC, int DT>
+struct RowsShared {
+  QueryTiles<HDP, NT, CODEC, DT> queries;
+  float joined[kWavesPerBlock][16][kJoinStride];
+  float ml[kWavesPerBlock][16][2];
+};
+
+template <int HDP, bool EXACT, int NT, int CODEC, int DT>
+__device__ __forceinline__ void run_segment(const RowsArgs& a, const Segment& seg, const Reach& reach,
+                                            RowsShared<HDP, NT, CODEC, DT>& shared) {
+  const AttnCall& c = a.c;
+  const RowTile& tile = seg.tile;
+  const int32_t head = seg.head, group = a.group, in_seq = tile.count * group, before = reach.before;
+  const int lane = lane_now(), x = lane & 15, wave = wave_in_block();
+  // Tiles of tokens inside [all_lo, all_hi) are seen whole by every row.
+  const int32_t all_lo = a.window > 0 ? max(reach.pos_hi - a.window + 1, 0) : 0;
+  const int32_t last = seg.hi, all_hi = min(reach.pos_lo + 1, last);
   const int64_t head_off = static_cast<int64_t>(head) * a.hd * a.bs;
   const uint8_t* row = static_cast<const uint8_t*>(c.tables) +
                        tile.seq * c.table_stride * (c.wide_tables ? 8 : 4);
@@ -725,7 +743,7 @@ void attention_rows_kernel(const RowsArgs a) {
   constexpr int32_t kStep = kWavesPerBlock * kWaveTokens;
   // 256 dims go in two halves through the same registers.
   constexpr int kDims = HDP <= 128 ? HDP : HDP / 2;
-  int32_t token = static_cast<int32_t>(span.lo) + wave * kWaveTokens;
+  int32_t token = seg.lo + wave * kWaveTokens;
   uint32_t k[kDims / 4];
   u32x4 v[kDims / 16];
   GroupIds ids, next_ids;
@@ -734,13 +752,13 @@ void attention_rows_kernel(const RowsArgs a) {
     ids = tile_ids(a, row, token, last);
     next_ids = tile_ids(a, row, token + kStep, last);
     scales = load_scales(c, head, ids);
-    load_keys<kDims, EXACT>(a, head_off, ids, 0, k);
-    load_values<kDims, EXACT>(a, head_off, ids, 0, v);
+    load_keys<kDims, EXACT>(a, head_off, token, ids, 0, k);
+    load_values<kDims, EXACT>(a, head_off, token, ids, 0, v);
   }
 
   const Mma<CODEC> mma;
   // Rows and what they see; the waves share the queries.
-  __shared__ QueryTiles<HDP, NT, CODEC, DT> queries;
+  QueryTiles<HDP, NT, CODEC, DT>& queries = shared.queries;
   RowState<HDP> state[NT];
   Sight sight[NT];
 #pragma unroll
@@ -767,7 +785,7 @@ void attention_rows_kernel(const RowsArgs a) {
       f32x4 score[NT][4] = {};
       key_products<0, kDims, HDP, NT, CODEC, DT>(mma, k, queries, score);
       if constexpr (HDP > kDims) {
-        load_keys<kDims, EXACT>(a, head_off, ids, kDims, k);
+        load_keys<kDims, EXACT>(a, head_off, token, ids, kDims, k);
         key_products<kDims / 32, kDims, HDP, NT, CODEC, DT>(mma, k, queries, score);
       }
       // Loads return in order: table entries are read two tiles ahead, in front of the keys whose arrival they
@@ -777,7 +795,7 @@ void attention_rows_kernel(const RowsArgs a) {
       if (next < last) {
         later_ids = tile_ids(a, row, next + kStep, last);
         next_scales = load_scales(c, head, next_ids);
-        load_keys<kDims, EXACT>(a, head_off, next_ids, 0, k);
+        load_keys<kDims, EXACT>(a, head_off, next, next_ids, 0, k);
       }
       const bool masked = token < all_lo || token + kWaveTokens > all_hi || ballot(!scales.seen) != 0;
       u32x4 p[NT][2][kWeightParts<CODEC, DT>];
@@ -789,11 +807,11 @@ void attention_rows_kernel(const RowsArgs a) {
       }
       value_products<0, kDims, HDP, NT, CODEC, DT>(mma, v, p, state);
       if constexpr (HDP > kDims) {
-        load_values<kDims, EXACT>(a, head_off, ids, kDims, v);
+        load_values<kDims, EXACT>(a, head_off, token, ids, kDims, v);
         value_products<kDims / 16, kDims, HDP, NT, CODEC, DT>(mma, v, p, state);
       }
       if (next >= last) break;
-      load_values<kDims, EXACT>(a, head_off, next_ids, 0, v);
+      load_values<kDims, EXACT>(a, head_off, next, next_ids, 0, v);
       ids = next_ids;
       next_ids = later_ids;
       scales = next_scales;
@@ -804,8 +822,8 @@ void attention_rows_kernel(const RowsArgs a) {
   mma.done();
 
   // The four waves' results of a row are joined by the thread that stores them.
-  __shared__ float joined[kWavesPerBlock][16][kJoinStride];
-  __shared__ float ml[kWavesPerBlock][16][2];
+  auto& joined = shared.joined;
+  auto& ml = shared.ml;
   constexpr int kChunk = HDP < kJoinDims ? HDP : kJoinDims;
   const float back = __builtin_ldexpf(1.0f, Mma<CODEC>::kCodeShift - Mma<CODEC>::kWeightTop);
 #pragma unroll
@@ -814,19 +832,20 @@ void attention_rows_kernel(const RowsArgs a) {
 #pragma unroll
     for (int d0 = 0; d0 < HDP; d0 += kChunk) {
       __syncthreads();
-      if (lane_id() < 16) {
+      if (lane < 16) {
         ml[wave][x][0] = state[n].m;
         ml[wave][x][1] = l;
       }
 #pragma unroll
       for (int k = 0; k < kChunk / 16; ++k)
-        *reinterpret_cast<f32x4*>(&joined[wave][x][16 * k + 4 * (lane_id() >> 4)]) = state[n].acc[d0 / 16 + k];
+        *reinterpret_cast<f32x4*>(&joined[wave][x][16 * k + 4 * (lane >> 4)]) = state[n].acc[d0 / 16 + k];
       __syncthreads();
       const int at = threadIdx.x >> 4;
       const int32_t r = tile.base + 16 * n + at;
       if (r >= in_seq) continue;
       const int32_t i = r / group;
       const int64_t rh = static_cast<int64_t>(tile.first + i) * a.heads + head * group + (r - i * group);
+      const int64_t part = seg.first_part + (seg.by_row ? rh : 16 * n + at);
       float top = ml[0][at][0];
 #pragma unroll
       for (int w = 1; w < kWavesPerBlock; ++w) top = fmaxf(top, ml[w][at][0]);
@@ -843,16 +862,16 @@ void attention_rows_kernel(const RowsArgs a) {
         for (int w = 0; w < kWavesPerBlock; ++w) o += joined[w][at][k] * fade[w];
         o *= back;
         if (!EXACT && d0 + k >= a.hd) continue;
-        if (a.splits > 1) {
-          if (sum != 0.0f) part_acc(c, split, rh)[d0 + k] = o;
+        if (seg.parts > 0) {
+          if (sum != 0.0f) part_acc(c, seg.parts, part)[d0 + k] = o;
           continue;
         }
         store_o<DT>(c.out, rh * a.hd + d0 + k, sum == 0.0f ? 0.0f : o / sum);
       }
       if (d0 == 0 && (threadIdx.x & 15) == 0) {
-        if (a.splits > 1) {
-          part_ml(c, split, rh)[0] = top;
-          part_ml(c, split, rh)[1] = sum;
+        if (seg.parts > 0) {
+          part_ml(c, part)[0] = top;
+          part_ml(c, part)[1] = sum;
         } else if (c.lse != nullptr) {
           c.lse[rh] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * kLn2;
         }
@@ -861,36 +880,200 @@ void attention_rows_kernel(const RowsArgs a) {
   }
 }
 
+// One workgroup per (row tile, kv head, part).
+template <int HDP, bool EXACT, int NT, int CODEC, int DT>
+__global__ __launch_bounds__(kBlockThreads, rows_occupancy(HDP, EXACT, NT, CODEC))
+void attention_rows_kernel(const RowsArgs a) {
+  const AttnCall& c = a.c;
+  __shared__ RowsShared<HDP, NT, CODEC, DT> shared;
+  const int32_t head = blockIdx.y, split = blockIdx.z;
+  const RowTile tile = find_tile(a, blockIdx.x, 16 * NT);
+  if (c.starts != nullptr && c.fill_rows && head == 0 && split == 0) fill_loose_rows<DT>(c, blockIdx.x, gridDim.x);
+  if (tile.seq < 0) return;
+  const Reach reach = tile_reach(a, tile, 16 * NT);
+  const Span span = part_span(reach.begin, reach.end, split, a.splits);
+  const int64_t per_part = c.rows * c.heads;
+  if (a.splits > 1 && span.lo >= span.hi) {  // nothing to do: the rows' parts say so
+    const int32_t group = a.group, in_seq = tile.count * group;
+    const int32_t r = tile.base + threadIdx.x;
+    if (threadIdx.x >= 16 * NT || r >= in_seq) return;
+    const int64_t rh = static_cast<int64_t>(tile.first + r / group) * a.heads + head * group + r % group;
+    part_ml(c, split * per_part + rh)[0] = -__builtin_inff();
+    part_ml(c, split * per_part + rh)[1] = 0.0f;
+    return;
+  }
+  const Segment seg{tile, head, static_cast<int32_t>(span.lo), static_cast<int32_t>(span.hi),
+                    a.splits > 1 ? a.splits * per_part : 0, split * per_part, true};
+  run_segment<HDP, EXACT, NT, CODEC, DT>(a, seg, reach, shared);
+}
+
+// The even cut of a decode step.  Sequences differ in length, so equal parts of each leave most of the chip waiting
+// for the longest (64 sequences of 256 to 8192 tokens: 3.8 TB/s, against 5.1 TB/s where all are equally long).
+// Here a unit is 256 tokens (a turn of a workgroup) of a line, one (sequence, row tile, kv head); the lines of all
+// sequences stand one behind another, and workgroup i of n takes units [i * all / n, (i + 1) * all / n).  Only its
+// first line may have begun, and only its last one may go on, in another workgroup: their parts are 2 i and
+// 2 i + 1 (times the tile's rows); lines in between, or all its own, go to the output at once.
+struct FlowCut {
+  uint32_t all, n;
+  __device__ __forceinline__ uint32_t start(uint32_t i) const {
+    return static_cast<uint32_t>(static_cast<uint64_t>(i) * all / n);
+  }
+  __device__ __forceinline__ uint32_t owner(uint32_t unit) const {
+    return static_cast<uint32_t>((static_cast<uint64_t>(unit + 1) * n - 1) / all);
+  }
+};
+
+constexpr int32_t kUnitTokens = 256;
+
+__device__ __forceinline__ int32_t reach_turns(const Reach& r) {  // at least one, for the row's zeros
+  const int32_t n = r.end - r.begin / kWaveTokens * kWaveTokens;
+  return r.end > r.begin ? (n + kUnitTokens - 1) / kUnitTokens : 1;
+}
+
+__device__ __forceinline__ int32_t seq_turns(const RowsArgs& a, int32_t b) {
+  return reach_turns(tile_reach(a, RowTile{b, b, 1, 0}, 1));
+}
+
+// A line's sequence, its number within the sequence, the sequence's turns and the line's first unit.  (All units
+// together are fewer than 2^31: attention_flows.)
+struct FlowLine {
+  int32_t seq, line, turns;
+  uint32_t first;
+};
+
+// Finds the line that holds `unit`, or with seq >= 0 the first line of that sequence; *all receives the sum.
+__device__ __forceinline__ FlowLine find_line(const RowsArgs& a, uint32_t lines, uint32_t unit, int32_t seq,
+                                              uint32_t* all) {
+  FlowLine found{-1, 0, 1, 0};
+  uint32_t before = 0;
+  for (int32_t b0 = 0; b0 < a.batch; b0 += kWave) {
+    const int32_t b = b0 + lane_id();
+    const uint32_t turns = b < a.batch ? seq_turns(a, b) : 0;
+    uint32_t end = turns * lines;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const uint32_t y = __shfl_up(end, o);
+      if (lane_id() >= o) end += y;
+    }
+    end += before;
+    const uint64_t hit = ballot(b < a.batch && (seq >= 0 ? b == seq : end > unit));
+    if (found.seq < 0 && hit != 0) {
+      const int src = __builtin_ctzll(hit);
+      found.seq = b0 + src;
+      found.turns = __builtin_amdgcn_readlane(turns, src);
+      const uint32_t base = __builtin_amdgcn_readlane(end, src) - found.turns * lines;
+      found.line = seq >= 0 ? 0 : static_cast<int32_t>((unit - base) / static_cast<uint32_t>(found.turns));
+      found.first = base + static_cast<uint32_t>(found.line) * found.turns;
+      if (all == nullptr) return found;
+    }
+    before = __builtin_amdgcn_readlane(end, kWave - 1);
+  }
+  if (all != nullptr) *all = before;
+  return found;
+}
+
+__device__ __forceinline__ FlowCut flow_cut(uint32_t all, uint32_t groups) { return {all, all < groups ? all : groups}; }
+
+template <int HDP, bool EXACT, int NT, int CODEC, int DT>
+__global__ __launch_bounds__(kBlockThreads, rows_occupancy(HDP, EXACT, NT, CODEC))
+void attention_flow_kernel(const RowsArgs a) {
+  __shared__ RowsShared<HDP, NT, CODEC, DT> shared;
+  const uint32_t lines = static_cast<uint32_t>(a.heads / a.group) * a.seq_tiles;
+  // This workgroup's units to come and the line that they begin in (in registers they would be held over a segment).
+  __shared__ struct {
+    uint32_t unit, end, first;
+    int32_t seq, line;
+  } share;
+  {
+    uint32_t all = 0;
+    find_line(a, lines, 0xFFFFFFFFu, -1, &all);
+    const FlowCut cut = flow_cut(all, gridDim.x);
+    if (blockIdx.x >= cut.n) return;
+    const uint32_t unit = cut.start(blockIdx.x);
+    const FlowLine line = find_line(a, lines, unit, -1, nullptr);
+    if (threadIdx.x == 0) share = {unit, cut.start(blockIdx.x + 1), line.first, line.seq, line.line};
+  }
+  for (;;) {
+    __syncthreads();
+    const uint32_t unit = __builtin_amdgcn_readfirstlane(share.unit), end = __builtin_amdgcn_readfirstlane(share.end);
+    const uint32_t first = __builtin_amdgcn_readfirstlane(share.first);
+    const int32_t seq = __builtin_amdgcn_readfirstlane(share.seq), line = __builtin_amdgcn_readfirstlane(share.line);
+    if (unit >= end) return;
+    const int32_t head = line / a.seq_tiles, tile_no = line - head * a.seq_tiles;
+    const RowTile tile{seq, seq, 1, tile_no * 16 * NT};
+    const Reach reach = tile_reach(a, tile, 16 * NT);
+    const int32_t turns = reach_turns(reach), turn = static_cast<int32_t>(unit - first);
+    const int32_t take = min(static_cast<int32_t>(end - unit), turns - turn);
+    const int32_t lo = reach.begin / kWaveTokens * kWaveTokens + turn * kUnitTokens;
+    const bool whole = take == turns;
+    const Segment seg{tile, head, lo, min(reach.end, lo + take * kUnitTokens),
+                      whole ? 0 : int64_t{2} * gridDim.x * 16 * NT,
+                      (int64_t{2} * blockIdx.x + (turn == 0)) * 16 * NT, false};
+    __syncthreads();  // every wave has read its share
+    if (threadIdx.x == 0) {
+      const bool same = line + 1 < static_cast<int32_t>(lines);
+      share.unit = unit + take;
+      share.first = first + turns;
+      share.seq = same ? seq : seq + 1;
+      share.line = same ? line + 1 : 0;
+    }
+    run_segment<HDP, EXACT, NT, CODEC, DT>(a, seg, reach, shared);
+  }
+}
+
 // ----- joining the parts: one workgroup per (row, head) ---------------------------------------------
-// Lane s holds part s's maximum and sum; the waves add up the parts' results by turns, and the first one stores
-// their sum.  Parts that saw nothing hold no result and are not read.
-constexpr int kMostSplits = kWave;
+// Lane j holds the maximum and sum of part j of a round of 64; the waves add up the parts' results by turns, and the
+// first one stores their sum.  Parts that saw nothing hold no result: what is read in its place is not used.
+constexpr int kMostSplits = 64;
+
+// The parts of a (row, head): part j is first + j * step, but part 0 of an even cut is its own.
+struct PartList {
+  int64_t count, total, zeroth, first, step;
+  __device__ __forceinline__ int64_t at(int64_t j) const { return j == 0 ? zeroth : first + j * step; }
+};
 
 template <int DT>
-__global__ __launch_bounds__(kBlockThreads) void attention_join_kernel(const AttnCall c) {
-  const int64_t rh = blockIdx.x;
+__device__ __forceinline__ void join_parts(const AttnCall& c, int64_t rh, const PartList& parts) {
   const int lane = lane_id(), wave = wave_in_block();
-  const int hd = static_cast<int>(c.head_dim), splits = static_cast<int>(c.splits);
+  const int hd = static_cast<int>(c.head_dim);
   __shared__ float sums[kWavesPerBlock - 1][kAnyMaxDim];
-  float m = -__builtin_inff(), l = 0.0f;
-  if (lane < splits) {
-    m = part_ml(c, lane, rh)[0];
-    l = part_ml(c, lane, rh)[1];
-  }
-  if (row_sequence(c, rh / c.heads).seq < 0) return;  // no parts: what was read is not looked at
-  const float top = wave_max(m);
+  float top = -__builtin_inff();
+  for (int64_t j = lane; j < parts.count; j += kWave) top = fmaxf(top, part_ml(c, parts.at(j))[0]);
+  top = wave_max(top);
   const float ref = top == -__builtin_inff() ? 0.0f : top;
-  const float fade = __builtin_amdgcn_exp2f(m - ref);
-  const float sum = wave_sum(l * fade);
-  const uint64_t full = ballot(l != 0.0f);
+  float sum = 0.0f;
   float acc[kAnyMaxDim / kWave] = {};
-  for (int s = wave; s < splits; s += kWavesPerBlock) {
-    if ((full >> s & 1) == 0) continue;
-    const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(fade), s));
-    const float* part = part_acc(c, s, rh);
+  for (int64_t j0 = 0; j0 < parts.count; j0 += kWave) {
+    float m = -__builtin_inff(), l = 0.0f;
+    if (j0 + lane < parts.count) {
+      m = part_ml(c, parts.at(j0 + lane))[0];
+      l = part_ml(c, parts.at(j0 + lane))[1];
+    }
+    const float fade = __builtin_amdgcn_exp2f(m - ref);
+    sum += wave_sum(l * fade);
+    const int64_t left = parts.count - j0;
+    const int round = left < kWave ? static_cast<int>(left) : kWave;
+    for (int s0 = wave; s0 < round; s0 += 4 * kWavesPerBlock) {
+      float f[4], part[4][kAnyMaxDim / kWave];
 #pragma unroll
-    for (int i = 0; i < kAnyMaxDim / kWave; ++i)
-      if (lane + i * kWave < hd) acc[i] = __builtin_fmaf(part[lane + i * kWave], f, acc[i]);
+      for (int u = 0; u < 4; ++u) {  // four parts on their way at a time
+        const int s = s0 + u * kWavesPerBlock < round ? s0 + u * kWavesPerBlock : s0;
+        const bool used = s0 + u * kWavesPerBlock < round &&
+                          __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l), s)) != 0.0f;
+        f[u] = used ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(fade), s)) : 0.0f;
+        const float* p = part_acc(c, parts.total, parts.at(j0 + s));
+#pragma unroll
+        for (int i = 0; i < kAnyMaxDim / kWave; ++i) {
+          part[u][i] = 0.0f;
+          if (i * kWave < hd && lane + i * kWave < hd) part[u][i] = p[lane + i * kWave];
+          if (!used) part[u][i] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < kAnyMaxDim / kWave; ++i) acc[i] = __builtin_fmaf(part[u][i], f[u], acc[i]);
+    }
   }
   if (wave > 0)
 #pragma unroll
@@ -907,6 +1090,32 @@ __global__ __launch_bounds__(kBlockThreads) void attention_join_kernel(const Att
     store_o<DT>(c.out, rh * hd + d, sum == 0.0f ? 0.0f : o / sum);
   }
   if (c.lse != nullptr && lane == 0) c.lse[rh] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * kLn2;
+}
+
+template <int DT>
+__global__ __launch_bounds__(kBlockThreads) void attention_join_kernel(const AttnCall c) {
+  const int64_t rh = blockIdx.x, per_part = c.rows * c.heads;
+  if (row_sequence(c, rh / c.heads).seq < 0) return;  // no parts
+  join_parts<DT>(c, rh, {c.splits, c.splits * per_part, rh, rh, per_part});
+}
+
+// Lines that lie in one workgroup's share are done.
+template <int DT>
+__global__ __launch_bounds__(kBlockThreads) void attention_flow_join_kernel(const RowsArgs a, uint32_t groups,
+                                                                           int32_t tile_rows) {
+  const int32_t seq = blockIdx.x / a.heads, hq = blockIdx.x - seq * a.heads;
+  const int32_t head = hq / a.group, r = hq - head * a.group, tile = r / tile_rows;
+  uint32_t all = 0;
+  const FlowLine of = find_line(a, static_cast<uint32_t>(a.heads / a.group) * a.seq_tiles, 0, seq, &all);
+  const FlowCut cut = flow_cut(all, groups);
+  const uint32_t first = of.first + static_cast<uint32_t>(head * a.seq_tiles + tile) * of.turns;
+  const uint32_t from = cut.owner(first), to = cut.owner(first + of.turns - 1);
+  if (from == to) return;
+  const int64_t in_tile = r - tile * tile_rows;
+  join_parts<DT>(a.c, blockIdx.x,
+                 {static_cast<int64_t>(to - from + 1), int64_t{2} * groups * tile_rows,
+                  (2 * static_cast<int64_t>(from) + 1) * tile_rows + in_tile,
+                  2 * static_cast<int64_t>(from) * tile_rows + in_tile, int64_t{2} * tile_rows});
 }
 
 template <int DT>
@@ -948,8 +1157,20 @@ int64_t tiles_bound(const AttnCall& c, int size) {
   return c.rows * group / size + c.batch;
 }
 
-template <int HDP, bool EXACT, int NT, int CODEC, int DT>
-hipError_t launch_rows_as(const AttnCall& c, hipStream_t stream) {
+// Workgroups of an even cut: what the chip holds at once, or one for each 256 tokens of `longest`-token sequences.
+constexpr int64_t kComputeUnits = 256;
+
+int64_t flow_groups(const AttnCall& c) {
+  const int size = 16 * row_tiles(c);
+  const bool exact = c.head_dim == 64 || c.head_dim == 96 || c.head_dim == 128 || c.head_dim == 256;
+  const int hdp = c.head_dim <= 64 ? 64 : exact && c.head_dim == 96 ? 96 : c.head_dim <= 128 ? 128 : 256;
+  int64_t n = kComputeUnits * rows_occupancy(hdp, exact, size / 16, c.codec);
+  const int64_t turns = (c.max_blocks * c.block_size + 255) / 256;
+  const int64_t most = tiles_bound(c, size) * c.kv_heads * (turns > 0 ? turns : 1);
+  return most < n ? most : n;
+}
+
+RowsArgs rows_args(const AttnCall& c, int tiles) {
   RowsArgs a{};
   a.c = c;
   a.batch = static_cast<int32_t>(c.batch);
@@ -963,7 +1184,23 @@ hipError_t launch_rows_as(const AttnCall& c, hipStream_t stream) {
   a.group = static_cast<int32_t>(c.heads / c.kv_heads);
   const int64_t b16 = c.block_size / 16;
   a.block_shift = (b16 & (b16 - 1)) == 0 ? __builtin_ctzll(b16) : -1;
-  a.seq_tiles = (a.group + 16 * NT - 1) / (16 * NT);
+  a.seq_tiles = (a.group + 16 * tiles - 1) / (16 * tiles);
+  return a;
+}
+
+template <int HDP, bool EXACT, int NT, int CODEC, int DT>
+hipError_t launch_rows_as(const AttnCall& c, hipStream_t stream) {
+  const RowsArgs a = rows_args(c, NT);
+  if (c.splits == 0) {
+    const uint32_t groups = static_cast<uint32_t>(flow_groups(c));
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_flow_kernel<HDP, EXACT, NT, CODEC, DT>), dim3(groups),
+                       dim3(kBlockThreads), 0, stream, a);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_flow_join_kernel<DT>), dim3(static_cast<uint32_t>(c.rows * c.heads)),
+                       dim3(kBlockThreads), 0, stream, a, groups, 16 * NT);
+    return hipGetLastError();
+  }
   int64_t tiles = tiles_bound(c, 16 * NT);
   if (tiles < 1) tiles = 1;  // rows of no sequence are still to be filled
   const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>(c.kv_heads), static_cast<uint32_t>(c.splits));
@@ -994,23 +1231,33 @@ hipError_t launch_typed(const AttnCall& c, hipStream_t stream) {
 template <int DT>
 hipError_t launch_dtype(const AttnCall& c, hipStream_t stream) {
   const hipError_t err = c.codec == kE4M3 ? launch_typed<DT, kE4M3>(c, stream) : launch_typed<DT, kE5M2>(c, stream);
-  if (err != hipSuccess || c.splits == 1) return err;
+  if (err != hipSuccess || c.splits <= 1) return err;
   return launch_join<DT>(c, stream);
 }
 
 }  // namespace
 
-// Parts: enough workgroups for two per CU and then some, none below 256 tokens (a workgroup's four waves).
+bool attention_flows(const AttnCall& c) {
+  const int64_t turns = (c.max_blocks * c.block_size + 255) / 256 + 1;
+  return c.starts == nullptr && c.batch > 0 && takes_rows(c) &&
+         c.batch < (int64_t{1} << 31) / turns / (c.kv_heads + c.heads);
+}
+
+// How a call is cut.  Decode steps of more than 512 tokens: evenly (0).  Others: enough parts for four workgroups
+// per CU, none below 256 tokens (a turn of a workgroup's four waves).
 int64_t attention_splits(const AttnCall& c, int64_t longest) {
+  if (attention_flows(c) && longest > 512) return 0;
   const int64_t groups = takes_rows(c) ? tiles_bound(c, 16 * row_tiles(c)) * c.kv_heads : c.rows * c.heads;
   int64_t splits = groups > 0 ? (1024 + groups - 1) / groups : 1;
-  const int64_t most = (longest + 255) / 256;
+  const int64_t most = longest / 256;
   splits = splits < most ? splits : most;
   return splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : splits;
 }
 
 int64_t attention_workspace(const AttnCall& c) {
-  return c.splits <= 1 ? 0 : 4 * c.splits * c.rows * c.heads * (c.head_dim + 2);
+  if (c.splits == 1) return 0;
+  const int64_t parts = c.splits == 0 ? 2 * flow_groups(c) * 16 * row_tiles(c) : c.splits * c.rows * c.heads;
+  return 4 * parts * (c.head_dim + 2);
 }
 
 hipError_t launch_attention(const AttnCall& c, hipStream_t stream) {

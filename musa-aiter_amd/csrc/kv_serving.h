@@ -40,6 +40,8 @@ hipError_t launch_block_tag_reset(const int64_t* slots, int64_t n, int64_t num_b
                                   uint64_t* owner, hipStream_t stream);
 
 hipError_t launch_attention(const musa_aiter_hip_attention_call& c, hipStream_t stream);
+// Whether the call can be cut evenly (splits 0).
+bool attention_flows(const musa_aiter_hip_attention_call& c);
 int64_t attention_splits(const musa_aiter_hip_attention_call& c, int64_t longest);
 int64_t attention_workspace(const musa_aiter_hip_attention_call& c);
 

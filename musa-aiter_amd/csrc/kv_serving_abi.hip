@@ -95,7 +95,7 @@ bool attention_sizes_ok(const musa_aiter_hip_attention_call& c) {
 
 int attention(const musa_aiter_hip_attention_call& c, hipStream_t stream) {
   if (!attention_sizes_ok(c) || c.dtype < 0 || c.dtype > 2 || (c.codec != kvhip::kE4M3 && c.codec != kvhip::kE5M2) ||
-      c.splits < 1 || c.splits > 64)
+      c.splits < 0 || c.splits > 64)
     return hipErrorInvalidValue;
   if (c.rows == 0) return hipSuccess;
   if (c.query == nullptr || c.out == nullptr || (c.batch > 0 && c.lens == nullptr) ||
@@ -104,7 +104,8 @@ int attention(const musa_aiter_hip_attention_call& c, hipStream_t stream) {
   if (c.starts == nullptr && c.rows != c.batch) return hipErrorInvalidValue;
   for (int kv = 0; kv < 2; ++kv)
     if (c.cache[kv] == nullptr || c.scale[kv] == nullptr) return hipErrorInvalidValue;
-  if (c.workspace_bytes < kvhip::attention_workspace(c) || (c.splits > 1 && c.workspace == nullptr))
+  if (c.splits == 0 && !kvhip::attention_flows(c)) return hipErrorInvalidValue;
+  if (c.workspace_bytes < kvhip::attention_workspace(c) || (c.splits != 1 && c.workspace == nullptr))
     return hipErrorInvalidValue;
   return kvhip::launch_attention(c, stream);
 }

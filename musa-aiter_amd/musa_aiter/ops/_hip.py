@@ -918,7 +918,7 @@ def attention(*, op: str, query: torch.Tensor, out: torch.Tensor, lse: torch.Ten
     with on_device(device):
         workspace = None
         splits = fn("musa_aiter_hip_attention_splits")(bytes(call), longest)
-        if splits > 1:
+        if splits != 1:
             struct.pack_into("<q", call, _ATTENTION_SPLITS_AT, splits)
             size = fn("musa_aiter_hip_attention_workspace")(bytes(call))
             workspace = torch.empty(size, dtype=torch.uint8, device=device)
