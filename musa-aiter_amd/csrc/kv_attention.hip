@@ -100,6 +100,10 @@ __device__ __forceinline__ float* part_ml(const AttnCall& c, int64_t part) {
 __device__ __forceinline__ float* part_acc(const AttnCall& c, int64_t count, int64_t part) {
   return static_cast<float*>(c.workspace) + 2 * count + part * c.head_dim;
 }
+// Behind them, for an even cut: the first and last workgroup of every line.
+__device__ __forceinline__ uint32_t* line_owners(const AttnCall& c, int64_t count, int64_t line) {
+  return static_cast<uint32_t*>(c.workspace) + (2 + c.head_dim) * count + 2 * line;
+}
 
 // A part begins at a multiple of a wave's 64 tokens and, but for the last one, holds whole turns of a workgroup's
 // four waves.
@@ -358,6 +362,7 @@ struct RowsArgs {
   int32_t block_shift;  // log2(block_size / 16), or -1
   int32_t seq_tiles;    // row tiles of every sequence (no row table)
   int32_t window, splits;
+  int32_t slot_rows;  // even cut: rows of a part
 };
 
 constexpr int32_t kMostRoom = 1 << 29;
@@ -821,11 +826,9 @@ __device__ __forceinline__ void run_segment(const RowsArgs& a, const Segment& se
 
   mma.done();
 
-  // The four waves' results of a row are joined by the thread that stores them.
-  auto& joined = shared.joined;
-  auto& ml = shared.ml;
-  constexpr int kChunk = HDP < kJoinDims ? HDP : kJoinDims;
   const float back = __builtin_ldexpf(1.0f, Mma<CODEC>::kCodeShift - Mma<CODEC>::kWeightTop);
+  // The four waves' results of a row are joined by the thread that stores them.
+  constexpr int kChunk = HDP < kJoinDims ? HDP : kJoinDims;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const float l = groups_sum(state[n].l);
@@ -833,12 +836,12 @@ __device__ __forceinline__ void run_segment(const RowsArgs& a, const Segment& se
     for (int d0 = 0; d0 < HDP; d0 += kChunk) {
       __syncthreads();
       if (lane < 16) {
-        ml[wave][x][0] = state[n].m;
-        ml[wave][x][1] = l;
+        shared.ml[wave][x][0] = state[n].m;
+        shared.ml[wave][x][1] = l;
       }
 #pragma unroll
       for (int k = 0; k < kChunk / 16; ++k)
-        *reinterpret_cast<f32x4*>(&joined[wave][x][16 * k + 4 * (lane >> 4)]) = state[n].acc[d0 / 16 + k];
+        *reinterpret_cast<f32x4*>(&shared.joined[wave][x][16 * k + 4 * (lane >> 4)]) = state[n].acc[d0 / 16 + k];
       __syncthreads();
       const int at = threadIdx.x >> 4;
       const int32_t r = tile.base + 16 * n + at;
@@ -846,20 +849,20 @@ __device__ __forceinline__ void run_segment(const RowsArgs& a, const Segment& se
       const int32_t i = r / group;
       const int64_t rh = static_cast<int64_t>(tile.first + i) * a.heads + head * group + (r - i * group);
       const int64_t part = seg.first_part + (seg.by_row ? rh : 16 * n + at);
-      float top = ml[0][at][0];
+      float top = shared.ml[0][at][0];
 #pragma unroll
-      for (int w = 1; w < kWavesPerBlock; ++w) top = fmaxf(top, ml[w][at][0]);
+      for (int w = 1; w < kWavesPerBlock; ++w) top = fmaxf(top, shared.ml[w][at][0]);
       const float ref = top == -__builtin_inff() ? 0.0f : top;
       float fade[kWavesPerBlock], sum = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWavesPerBlock; ++w) {
-        fade[w] = __builtin_amdgcn_exp2f(ml[w][at][0] - ref);
-        sum += ml[w][at][1] * fade[w];
+        fade[w] = __builtin_amdgcn_exp2f(shared.ml[w][at][0] - ref);
+        sum += shared.ml[w][at][1] * fade[w];
       }
       for (int k = threadIdx.x & 15; k < kChunk; k += 16) {
         float o = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWavesPerBlock; ++w) o += joined[w][at][k] * fade[w];
+        for (int w = 0; w < kWavesPerBlock; ++w) o += shared.joined[w][at][k] * fade[w];
         o *= back;
         if (!EXACT && d0 + k >= a.hd) continue;
         if (seg.parts > 0) {
@@ -909,10 +912,11 @@ void attention_rows_kernel(const RowsArgs a) {
 
 // The even cut of a decode step.  Sequences differ in length, so equal parts of each leave most of the chip waiting
 // for the longest (64 sequences of 256 to 8192 tokens: 3.8 TB/s, against 5.1 TB/s where all are equally long).
-// Here a unit is 256 tokens (a turn of a workgroup) of a line, one (sequence, row tile, kv head); the lines of all
-// sequences stand one behind another, and workgroup i of n takes units [i * all / n, (i + 1) * all / n).  Only its
-// first line may have begun, and only its last one may go on, in another workgroup: their parts are 2 i and
-// 2 i + 1 (times the tile's rows); lines in between, or all its own, go to the output at once.
+// Here a unit is 256 tokens (a turn of a workgroup's four waves) of a line, one (sequence, row tile, kv head); the lines
+// of all sequences stand one behind another, and workgroup i of n takes units [i * all / n, (i + 1) * all / n).
+// Only its first line may have begun, and only its last one may go on, in another workgroup: their parts are 2 i
+// and 2 i + 1 (times slot_rows); lines in between, or all its own, go to the output at once.
+// (Workgroups of one wave, which begin fewer lines each, were no faster at 512 and 2048 lines and slower at 16.)
 struct FlowCut {
   uint32_t all, n;
   __device__ __forceinline__ uint32_t start(uint32_t i) const {
@@ -923,9 +927,9 @@ struct FlowCut {
   }
 };
 
-constexpr int32_t kUnitTokens = 256;
+constexpr int32_t kUnitTokens = kWavesPerBlock * kWaveTokens;
 
-__device__ __forceinline__ int32_t reach_turns(const Reach& r) {  // at least one, for the row's zeros
+__device__ __forceinline__ int32_t reach_turns(const Reach& r) {  // at least one: the row's zeros
   const int32_t n = r.end - r.begin / kWaveTokens * kWaveTokens;
   return r.end > r.begin ? (n + kUnitTokens - 1) / kUnitTokens : 1;
 }
@@ -941,10 +945,8 @@ struct FlowLine {
   uint32_t first;
 };
 
-// Finds the line that holds `unit`, or with seq >= 0 the first line of that sequence; *all receives the sum.
-__device__ __forceinline__ FlowLine find_line(const RowsArgs& a, uint32_t lines, uint32_t unit, int32_t seq,
-                                              uint32_t* all) {
-  FlowLine found{-1, 0, 1, 0};
+// Finds the line that holds `unit`; with `all`, the sum of all units is left there instead.
+__device__ __forceinline__ FlowLine find_line(const RowsArgs& a, uint32_t lines, uint32_t unit, uint32_t* all) {
   uint32_t before = 0;
   for (int32_t b0 = 0; b0 < a.batch; b0 += kWave) {
     const int32_t b = b0 + lane_id();
@@ -956,20 +958,21 @@ __device__ __forceinline__ FlowLine find_line(const RowsArgs& a, uint32_t lines,
       if (lane_id() >= o) end += y;
     }
     end += before;
-    const uint64_t hit = ballot(b < a.batch && (seq >= 0 ? b == seq : end > unit));
-    if (found.seq < 0 && hit != 0) {
+    const uint64_t hit = ballot(b < a.batch && end > unit);
+    if (all == nullptr && hit != 0) {
       const int src = __builtin_ctzll(hit);
+      FlowLine found;
       found.seq = b0 + src;
       found.turns = __builtin_amdgcn_readlane(turns, src);
       const uint32_t base = __builtin_amdgcn_readlane(end, src) - found.turns * lines;
-      found.line = seq >= 0 ? 0 : static_cast<int32_t>((unit - base) / static_cast<uint32_t>(found.turns));
+      found.line = static_cast<int32_t>((unit - base) / static_cast<uint32_t>(found.turns));
       found.first = base + static_cast<uint32_t>(found.line) * found.turns;
-      if (all == nullptr) return found;
+      return found;
     }
     before = __builtin_amdgcn_readlane(end, kWave - 1);
   }
   if (all != nullptr) *all = before;
-  return found;
+  return {-1, 0, 1, 0};
 }
 
 __device__ __forceinline__ FlowCut flow_cut(uint32_t all, uint32_t groups) { return {all, all < groups ? all : groups}; }
@@ -981,17 +984,17 @@ void attention_flow_kernel(const RowsArgs a) {
   const uint32_t lines = static_cast<uint32_t>(a.heads / a.group) * a.seq_tiles;
   // This workgroup's units to come and the line that they begin in (in registers they would be held over a segment).
   __shared__ struct {
-    uint32_t unit, end, first;
+    uint32_t unit, end, first, all;
     int32_t seq, line;
   } share;
   {
     uint32_t all = 0;
-    find_line(a, lines, 0xFFFFFFFFu, -1, &all);
+    find_line(a, lines, 0, &all);
     const FlowCut cut = flow_cut(all, gridDim.x);
     if (blockIdx.x >= cut.n) return;
     const uint32_t unit = cut.start(blockIdx.x);
-    const FlowLine line = find_line(a, lines, unit, -1, nullptr);
-    if (threadIdx.x == 0) share = {unit, cut.start(blockIdx.x + 1), line.first, line.seq, line.line};
+    const FlowLine line = find_line(a, lines, unit, nullptr);
+    if (threadIdx.x == 0) share = {unit, cut.start(blockIdx.x + 1), line.first, all, line.seq, line.line};
   }
   for (;;) {
     __syncthreads();
@@ -1007,8 +1010,8 @@ void attention_flow_kernel(const RowsArgs a) {
     const int32_t lo = reach.begin / kWaveTokens * kWaveTokens + turn * kUnitTokens;
     const bool whole = take == turns;
     const Segment seg{tile, head, lo, min(reach.end, lo + take * kUnitTokens),
-                      whole ? 0 : int64_t{2} * gridDim.x * 16 * NT,
-                      (int64_t{2} * blockIdx.x + (turn == 0)) * 16 * NT, false};
+                      whole ? 0 : int64_t{2} * gridDim.x * a.slot_rows,
+                      (int64_t{2} * blockIdx.x + (turn == 0)) * a.slot_rows, false};
     __syncthreads();  // every wave has read its share
     if (threadIdx.x == 0) {
       const bool same = line + 1 < static_cast<int32_t>(lines);
@@ -1016,6 +1019,11 @@ void attention_flow_kernel(const RowsArgs a) {
       share.first = first + turns;
       share.seq = same ? seq : seq + 1;
       share.line = same ? line + 1 : 0;
+      if (turn == 0) {
+        uint32_t* owners = line_owners(a.c, int64_t{2} * gridDim.x * a.slot_rows, static_cast<int64_t>(seq) * lines + line);
+        owners[0] = blockIdx.x;
+        owners[1] = whole ? blockIdx.x : flow_cut(share.all, gridDim.x).owner(first + turns - 1);
+      }
     }
     run_segment<HDP, EXACT, NT, CODEC, DT>(a, seg, reach, shared);
   }
@@ -1032,11 +1040,11 @@ struct PartList {
   __device__ __forceinline__ int64_t at(int64_t j) const { return j == 0 ? zeroth : first + j * step; }
 };
 
-template <int DT>
+// WAVES of the workgroup add up one (row, head) together.
+template <int DT, int WAVES>
 __device__ __forceinline__ void join_parts(const AttnCall& c, int64_t rh, const PartList& parts) {
-  const int lane = lane_id(), wave = wave_in_block();
+  const int lane = lane_id(), wave = WAVES > 1 ? wave_in_block() : 0;
   const int hd = static_cast<int>(c.head_dim);
-  __shared__ float sums[kWavesPerBlock - 1][kAnyMaxDim];
   float top = -__builtin_inff();
   for (int64_t j = lane; j < parts.count; j += kWave) top = fmaxf(top, part_ml(c, parts.at(j))[0]);
   top = wave_max(top);
@@ -1053,12 +1061,12 @@ __device__ __forceinline__ void join_parts(const AttnCall& c, int64_t rh, const 
     sum += wave_sum(l * fade);
     const int64_t left = parts.count - j0;
     const int round = left < kWave ? static_cast<int>(left) : kWave;
-    for (int s0 = wave; s0 < round; s0 += 4 * kWavesPerBlock) {
+    for (int s0 = wave; s0 < round; s0 += 4 * WAVES) {
       float f[4], part[4][kAnyMaxDim / kWave];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {  // four parts on their way at a time
-        const int s = s0 + u * kWavesPerBlock < round ? s0 + u * kWavesPerBlock : s0;
-        const bool used = s0 + u * kWavesPerBlock < round &&
+        const int s = s0 + u * WAVES < round ? s0 + u * WAVES : s0;
+        const bool used = s0 + u * WAVES < round &&
                           __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l), s)) != 0.0f;
         f[u] = used ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(fade), s)) : 0.0f;
         const float* p = part_acc(c, parts.total, parts.at(j0 + s));
@@ -1075,53 +1083,62 @@ __device__ __forceinline__ void join_parts(const AttnCall& c, int64_t rh, const 
         for (int i = 0; i < kAnyMaxDim / kWave; ++i) acc[i] = __builtin_fmaf(part[u][i], f[u], acc[i]);
     }
   }
-  if (wave > 0)
+  if constexpr (WAVES > 1) {
+    __shared__ float sums[WAVES - 1][kAnyMaxDim];
+    if (wave > 0)
+#pragma unroll
+      for (int i = 0; i < kAnyMaxDim / kWave; ++i)
+        if (lane + i * kWave < hd) sums[wave - 1][lane + i * kWave] = acc[i];
+    __syncthreads();
+    if (wave > 0) return;
 #pragma unroll
     for (int i = 0; i < kAnyMaxDim / kWave; ++i)
-      if (lane + i * kWave < hd) sums[wave - 1][lane + i * kWave] = acc[i];
-  __syncthreads();
-  if (wave > 0) return;
-#pragma unroll
-  for (int i = 0; i < kAnyMaxDim / kWave; ++i) {
-    const int d = lane + i * kWave;
-    if (d >= hd) continue;
-    float o = acc[i];
-    for (int w = 0; w < kWavesPerBlock - 1; ++w) o += sums[w][d];
-    store_o<DT>(c.out, rh * hd + d, sum == 0.0f ? 0.0f : o / sum);
+      if (lane + i * kWave < hd)
+        for (int w = 0; w < WAVES - 1; ++w) acc[i] += sums[w][lane + i * kWave];
   }
+#pragma unroll
+  for (int i = 0; i < kAnyMaxDim / kWave; ++i)
+    if (lane + i * kWave < hd) store_o<DT>(c.out, rh * hd + lane + i * kWave, sum == 0.0f ? 0.0f : acc[i] / sum);
   if (c.lse != nullptr && lane == 0) c.lse[rh] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * kLn2;
 }
 
-template <int DT>
+// A workgroup per (row, head), or with WAVES 1 a wave (many rows, few parts of each).
+constexpr int64_t kWaveJoinRows = 512;
+
+template <int DT, int WAVES>
 __global__ __launch_bounds__(kBlockThreads) void attention_join_kernel(const AttnCall c) {
-  const int64_t rh = blockIdx.x, per_part = c.rows * c.heads;
-  if (row_sequence(c, rh / c.heads).seq < 0) return;  // no parts
-  join_parts<DT>(c, rh, {c.splits, c.splits * per_part, rh, rh, per_part});
+  const int64_t rh = WAVES > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave_in_block();
+  const int64_t per_part = c.rows * c.heads;
+  if (rh >= per_part || row_sequence(c, rh / c.heads).seq < 0) return;  // no parts
+  join_parts<DT, WAVES>(c, rh, {c.splits, c.splits * per_part, rh, rh, per_part});
 }
 
 // Lines that lie in one workgroup's share are done.
-template <int DT>
+template <int DT, int WAVES>
 __global__ __launch_bounds__(kBlockThreads) void attention_flow_join_kernel(const RowsArgs a, uint32_t groups,
                                                                            int32_t tile_rows) {
-  const int32_t seq = blockIdx.x / a.heads, hq = blockIdx.x - seq * a.heads;
+  const uint32_t rh = WAVES > 1 ? blockIdx.x : blockIdx.x * kWavesPerBlock + wave_in_block();
+  if (rh >= static_cast<uint32_t>(a.batch) * a.heads) return;
+  const int32_t seq = rh / a.heads, hq = rh - seq * a.heads;
   const int32_t head = hq / a.group, r = hq - head * a.group, tile = r / tile_rows;
-  uint32_t all = 0;
-  const FlowLine of = find_line(a, static_cast<uint32_t>(a.heads / a.group) * a.seq_tiles, 0, seq, &all);
-  const FlowCut cut = flow_cut(all, groups);
-  const uint32_t first = of.first + static_cast<uint32_t>(head * a.seq_tiles + tile) * of.turns;
-  const uint32_t from = cut.owner(first), to = cut.owner(first + of.turns - 1);
+  const int64_t rows = a.slot_rows, total = 2 * groups * rows, in_tile = r - tile * tile_rows;
+  const int64_t line = (static_cast<int64_t>(seq) * (a.heads / a.group) + head) * a.seq_tiles + tile;
+  const uint32_t* owners = line_owners(a.c, total, line);
+  const int64_t from = __builtin_amdgcn_readfirstlane(owners[0]), to = __builtin_amdgcn_readfirstlane(owners[1]);
   if (from == to) return;
-  const int64_t in_tile = r - tile * tile_rows;
-  join_parts<DT>(a.c, blockIdx.x,
-                 {static_cast<int64_t>(to - from + 1), int64_t{2} * groups * tile_rows,
-                  (2 * static_cast<int64_t>(from) + 1) * tile_rows + in_tile,
-                  2 * static_cast<int64_t>(from) * tile_rows + in_tile, int64_t{2} * tile_rows});
+  join_parts<DT, WAVES>(a.c, rh, {to - from + 1, total, (2 * from + 1) * rows + in_tile, 2 * from * rows + in_tile, 2 * rows});
 }
 
 template <int DT>
 hipError_t launch_join(const AttnCall& c, hipStream_t stream) {
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<DT>), dim3(static_cast<uint32_t>(c.rows * c.heads)),
-                     dim3(kBlockThreads), 0, stream, c);
+  const int64_t rh = c.rows * c.heads;
+  if (rh < kWaveJoinRows)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<DT, kWavesPerBlock>), dim3(static_cast<uint32_t>(rh)),
+                       dim3(kBlockThreads), 0, stream, c);
+  else
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<DT, 1>),
+                       dim3(static_cast<uint32_t>((rh + kWavesPerBlock - 1) / kWavesPerBlock)), dim3(kBlockThreads), 0,
+                       stream, c);
   return hipGetLastError();
 }
 
@@ -1157,17 +1174,23 @@ int64_t tiles_bound(const AttnCall& c, int size) {
   return c.rows * group / size + c.batch;
 }
 
-// Workgroups of an even cut: what the chip holds at once, or one for each 256 tokens of `longest`-token sequences.
+// How an even cut is made: workgroups (what the chip holds at once, or one for each unit that the tables have room
+// for) and rows of a part.
 constexpr int64_t kComputeUnits = 256;
 
-int64_t flow_groups(const AttnCall& c) {
-  const int size = 16 * row_tiles(c);
+struct FlowPlan {
+  int64_t groups, slot_rows;
+};
+
+FlowPlan flow_plan(const AttnCall& c) {
+  const int tiles = row_tiles(c), size = 16 * tiles;
   const bool exact = c.head_dim == 64 || c.head_dim == 96 || c.head_dim == 128 || c.head_dim == 256;
   const int hdp = c.head_dim <= 64 ? 64 : exact && c.head_dim == 96 ? 96 : c.head_dim <= 128 ? 128 : 256;
-  int64_t n = kComputeUnits * rows_occupancy(hdp, exact, size / 16, c.codec);
-  const int64_t turns = (c.max_blocks * c.block_size + 255) / 256;
-  const int64_t most = tiles_bound(c, size) * c.kv_heads * (turns > 0 ? turns : 1);
-  return most < n ? most : n;
+  const int64_t lines = tiles_bound(c, size) * c.kv_heads, group = c.heads / c.kv_heads;
+  const int64_t turns = (c.max_blocks * c.block_size + kUnitTokens - 1) / kUnitTokens;
+  const int64_t most = lines * (turns > 0 ? turns : 1);
+  const int64_t held = kComputeUnits * rows_occupancy(hdp, exact, tiles, c.codec);
+  return {most < held ? most : held, group < size ? group : size};
 }
 
 RowsArgs rows_args(const AttnCall& c, int tiles) {
@@ -1190,15 +1213,23 @@ RowsArgs rows_args(const AttnCall& c, int tiles) {
 
 template <int HDP, bool EXACT, int NT, int CODEC, int DT>
 hipError_t launch_rows_as(const AttnCall& c, hipStream_t stream) {
-  const RowsArgs a = rows_args(c, NT);
+  RowsArgs a = rows_args(c, NT);
   if (c.splits == 0) {
-    const uint32_t groups = static_cast<uint32_t>(flow_groups(c));
+    const FlowPlan plan = flow_plan(c);
+    const uint32_t groups = static_cast<uint32_t>(plan.groups);
+    a.slot_rows = static_cast<int32_t>(plan.slot_rows);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_flow_kernel<HDP, EXACT, NT, CODEC, DT>), dim3(groups),
                        dim3(kBlockThreads), 0, stream, a);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_flow_join_kernel<DT>), dim3(static_cast<uint32_t>(c.rows * c.heads)),
-                       dim3(kBlockThreads), 0, stream, a, groups, 16 * NT);
+    const int64_t rh = c.rows * c.heads;
+    if (rh < kWaveJoinRows)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_flow_join_kernel<DT, kWavesPerBlock>),
+                         dim3(static_cast<uint32_t>(rh)), dim3(kBlockThreads), 0, stream, a, groups, 16 * NT);
+    else
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_flow_join_kernel<DT, 1>),
+                         dim3(static_cast<uint32_t>((rh + kWavesPerBlock - 1) / kWavesPerBlock)), dim3(kBlockThreads),
+                         0, stream, a, groups, 16 * NT);
     return hipGetLastError();
   }
   int64_t tiles = tiles_bound(c, 16 * NT);
@@ -1238,7 +1269,7 @@ hipError_t launch_dtype(const AttnCall& c, hipStream_t stream) {
 }  // namespace
 
 bool attention_flows(const AttnCall& c) {
-  const int64_t turns = (c.max_blocks * c.block_size + 255) / 256 + 1;
+  const int64_t turns = c.max_blocks * c.block_size / kWaveTokens + 2;
   return c.starts == nullptr && c.batch > 0 && takes_rows(c) &&
          c.batch < (int64_t{1} << 31) / turns / (c.kv_heads + c.heads);
 }
@@ -1256,7 +1287,12 @@ int64_t attention_splits(const AttnCall& c, int64_t longest) {
 
 int64_t attention_workspace(const AttnCall& c) {
   if (c.splits == 1) return 0;
-  const int64_t parts = c.splits == 0 ? 2 * flow_groups(c) * 16 * row_tiles(c) : c.splits * c.rows * c.heads;
+  int64_t parts = c.splits * c.rows * c.heads;
+  if (c.splits == 0) {
+    const FlowPlan plan = flow_plan(c);
+    parts = 2 * plan.groups * plan.slot_rows;
+    return 4 * parts * (c.head_dim + 2) + 8 * tiles_bound(c, 16 * row_tiles(c)) * c.kv_heads;
+  }
   return 4 * parts * (c.head_dim + 2);
 }
 
