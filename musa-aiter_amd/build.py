@@ -67,12 +67,18 @@ def _compile(src: Path, obj: Path) -> None:
         sys.stderr.write("\n".join(noise) + "\n")
 
 
-HOST_SOURCE = "kv_host.cpp"
+HOST_SOURCES = ("kv_host.cpp", "kv_host_serving.cpp")
 HOST_MODULE = "_kv_host"
 
 
 def host_module_path() -> Path:
     return OUT_DIR / (HOST_MODULE + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def _run_host(cmd: list[str]) -> None:
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"host module build failed:\n{' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
 
 
 def _build_host() -> Path:
@@ -84,15 +90,16 @@ def _build_host() -> Path:
     out = host_module_path()
     tmp = out.with_name(out.name + ".tmp")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-shared", "-fPIC", "-std=c++17", "-Wall",
-           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", f"-DTORCH_EXTENSION_NAME={HOST_MODULE}",
-           f"-I{sysconfig.get_paths()['include']}", f"-I{ROOT.parent / 'include'}",
-           *[f"-I{p}" for p in cpp_extension.include_paths()],
-           str(CSRC / HOST_SOURCE), "-o", str(tmp),
-           *[f"-L{p}" for p in cpp_extension.library_paths()], "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"host module build failed:\n{' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
+    compile_cmd = [os.environ.get("CXX", "g++"), "-O2", "-fPIC", "-std=c++17", "-Wall", "-c",
+                   f"-D_GLIBCXX_USE_CXX11_ABI={abi}", f"-DTORCH_EXTENSION_NAME={HOST_MODULE}",
+                   f"-I{sysconfig.get_paths()['include']}", f"-I{ROOT.parent / 'include'}",
+                   *[f"-I{p}" for p in cpp_extension.include_paths()]]
+    objs = [ROOT / "_build" / (Path(s).stem + ".o") for s in HOST_SOURCES]
+    cmds = [[*compile_cmd, str(CSRC / s), "-o", str(o)] for s, o in zip(HOST_SOURCES, objs)]
+    with concurrent.futures.ThreadPoolExecutor(max_workers=len(cmds)) as pool:
+        list(pool.map(_run_host, cmds))
+    _run_host([os.environ.get("CXX", "g++"), "-shared", *map(str, objs), "-o", str(tmp),
+               *[f"-L{p}" for p in cpp_extension.library_paths()], "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python"])
     os.replace(tmp, out)
     return out
 

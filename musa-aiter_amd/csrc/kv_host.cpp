@@ -341,6 +341,8 @@ py::tuple paged_call(const py::handle& key_cache, const py::handle& value_cache,
 
 }  // namespace
 
+void add_serving_calls(py::module_& m);  // kv_host_serving.cpp
+
 PYBIND11_MODULE(_kv_host, m) {
   m.doc() = "Host-side tensor checks and address tables for the MI355X KV path";
   m.def("check_tensors", &check_tensors, py::arg("items"), py::arg("shape"), py::arg("like"));
@@ -349,6 +351,7 @@ PYBIND11_MODULE(_kv_host, m) {
   m.def("object_index", &object_index, py::arg("first"), py::arg("second"));
   m.def("two_x_nl_rows", &two_x_nl_rows);
   m.def("paged_call", &paged_call);
+  add_serving_calls(m);
   m.attr("NOT_TAKEN") = kNotTaken;
   m.attr("OK") = static_cast<int>(kOk);
   m.attr("SHAPE") = static_cast<int>(kShape);

@@ -954,3 +954,84 @@ def pages(kind: str, *, op: str, device: torch.device, tables: torch.Tensor, len
         rc = fn("musa_aiter_hip_pages_" + kind)(bytes(call), stream_ptr(device))
         del workspace
     check(rc, op)
+
+
+# The same calls with the argument checks and the packing in the host module.  Each returns None, with nothing
+# launched, where the arguments are not ones the module takes as they are; the caller then makes its own checks.
+_entry_addresses: dict[str, int] = {}
+
+
+def _entry(name: str) -> int:
+    found = _entry_addresses.get(name)
+    if found is None:
+        found = _entry_addresses[name] = ctypes.cast(fn(name), ctypes.c_void_p).value
+    return found
+
+
+def attention_native(op, query, key_cache, value_cache, tables, lens, k_scales, v_scales, starts, out, longest: int,
+                     softmax_scale: float, window: int, codec: int, with_lse: bool):
+    """(out, lse) of one attention call, or None."""
+    if type(query) is not torch.Tensor or not query.is_cuda:
+        return None
+    index = torch._C._cuda_getDevice()
+    rc, result, lse = (_host or host()).attention_call(
+        query, key_cache, value_cache, tables, lens, k_scales, v_scales, starts, out, longest, softmax_scale, window,
+        codec, with_lse, _entry("musa_aiter_hip_attention"), _entry("musa_aiter_hip_attention_splits"),
+        _entry("musa_aiter_hip_attention_workspace"), torch._C._cuda_getCurrentRawStream(index), index)
+    if rc == _host.NOT_TAKEN:
+        return None
+    check(rc, op)
+    return result, lse
+
+
+def block_store_native(op, key_linear, value_linear, key_cache, value_cache, slots, k_scales, v_scales, codec: int):
+    """One block-scaled store: True, or None where nothing was stored."""
+    if type(key_cache) is not torch.Tensor or not key_cache.is_cuda or torch._C._cuda_isCurrentStreamCapturing():
+        return None
+    index = torch._C._cuda_getDevice()
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    key = (index, stream)
+    lock = _stream_locks.get(key)
+    if lock is None or type(slots) is not torch.Tensor or key_cache.dim() < 4:
+        return None  # the stream's first call makes its lock and check set
+    h = _host or host()
+    entry = _entry("musa_aiter_hip_block_store")
+    with lock:
+        checks = _check_sets.get(key)
+        if checks is None:
+            return None
+        claims, held = 0, None
+        if slots.numel() > _BLOCK_STORE_SCAN[0] or key_cache.shape[-1] > _BLOCK_STORE_SCAN[1]:
+            held = _claim_sets.get(key)
+            if held is None or held[1].epoch == _EPOCH_LAST:
+                return None
+            held[1].epoch += 1
+            claims = held[2]
+        checks.stamp = next(_stamps)
+        rc = h.block_store_call(key_linear, value_linear, key_cache, value_cache, slots, k_scales, v_scales, codec,
+                                entry, claims, checks.report_ptr, checks.guard_ptr, _REPORT_WORDS, checks.stamp, stream,
+                                index)
+        del held
+    if rc == h.NOT_TAKEN or rc == _REFUSED:
+        return None
+    check(rc, op)
+    return True
+
+
+_PAGE_KINDS = {"fork": 0, "extend": 1, "compact": 2, "free": 3}
+
+
+def pages_native(kind: str, op, key_cache, value_cache, tables, lens, refs, rows, k_scales, v_scales, block_size: int,
+                 max_new: int):
+    """(slots, result) of one page operation, each None where it has none; or None."""
+    if type(tables) is not torch.Tensor or not tables.is_cuda:
+        return None
+    index = torch._C._cuda_getDevice()
+    rc, slots, result = (_host or host()).pages_call(
+        key_cache, value_cache, tables, lens, refs, rows, k_scales, v_scales, block_size, max_new, _PAGE_KINDS[kind],
+        _entry("musa_aiter_hip_pages_" + kind), _entry("musa_aiter_hip_pages_workspace"),
+        torch._C._cuda_getCurrentRawStream(index), index)
+    if rc == _host.NOT_TAKEN:
+        return None
+    check(rc, op)
+    return slots, result

@@ -22,6 +22,7 @@ from musa_aiter.ops.kv_transfer import (
     _FP8_CACHE_DTYPES,
     _INDEX_DTYPES,
     _LIN_DTYPE,
+    _NATIVE_FORMATS,
     _LinearPair,
     _codec,
     _emit,
@@ -110,6 +111,11 @@ def kv_linear_to_paged_fp8_block(
     ``ValueError``, with nothing stored; in a call that is being captured it is skipped.
     """
     op = "kv_linear_to_paged_fp8_block"
+    codec = _NATIVE_FORMATS.get(fp8_format)
+    if codec is not None and _hip.block_store_native(op, key_linear, value_linear, key_cache_fp8, value_cache_fp8,
+                                                     slot_mapping, k_scales, v_scales, codec):
+        _emit(op, key_linear, f"gfx950 {fp8_format.upper()} store with block scales")
+        return
     fp8_format = _normalize_fp8_format(fp8_format)
     nl, nb, nh, hd, bs = _check_fp8_caches(op, key_cache_fp8, value_cache_fp8)
     layered = key_cache_fp8.dim() == 5
@@ -203,6 +209,18 @@ def kv_paged_attention_fp8(
     ``return_lse`` also the float32 ``[T, heads]`` logarithms of the rows' softmax sums.
     """
     op = "kv_paged_attention_fp8"
+    native = _NATIVE_FORMATS.get(fp8_format)
+    if native is not None and (window is None or type(window) is int and window > 0) \
+            and (max_seq_len is None or type(max_seq_len) is int and max_seq_len >= 0) \
+            and (softmax_scale is None or type(softmax_scale) is float and math.isfinite(softmax_scale)):
+        got = _hip.attention_native(
+            op, query, key_cache_fp8, value_cache_fp8, block_tables, seq_lens, k_scales, v_scales, query_starts, out,
+            -1 if max_seq_len is None else max_seq_len,
+            query.shape[-1] ** -0.5 if softmax_scale is None and query.dim() and query.shape[-1] else softmax_scale or 0.0,
+            window or 0, native, return_lse)
+        if got is not None:
+            _emit(op, query, f"gfx950 {fp8_format.upper()} paged attention with block scales")
+            return got if return_lse else got[0]
     if query.dim() != 3:
         raise ValueError(f"{op}: query must be [rows, heads, head_dim]")
     if query.dtype not in _LIN_DTYPE:

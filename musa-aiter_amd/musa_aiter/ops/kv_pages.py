@@ -122,6 +122,12 @@ def kv_extend_paged_sequences(
     ``block_tables`` is too short).
     """
     op = "kv_extend_paged_sequences"
+    if type(max_new) is int and max_new >= 0:
+        got = _hip.pages_native("extend", op, key_cache, value_cache, block_tables, seq_lens, ref_counts, new_lens,
+                                k_scales, v_scales, 0, max_new)
+        if got is not None:
+            _emit(op, key_cache, "gfx950 page allocation with copy of shared pages")
+            return got
     batch = _check_state(op, block_tables, seq_lens, ref_counts)
     block_size, pool = _check_pool(op, key_cache, value_cache, k_scales, v_scales, ref_counts)
     device = block_tables.device
@@ -152,6 +158,10 @@ def kv_fork_paged_sequences(
     row whose parent is not in [0, batch) becomes empty.
     """
     op = "kv_fork_paged_sequences"
+    if type(block_size) is int and block_size > 0 and _hip.pages_native(
+            "fork", op, None, None, block_tables, seq_lens, ref_counts, parents, None, None, block_size, 0) is not None:
+        _emit(op, block_tables, "gfx950 page table fork")
+        return
     batch = _check_state(op, block_tables, seq_lens, ref_counts)
     rows = _row_values(op, "parents", parents, batch, block_tables.device)
     block_size = _check_block_size(op, block_size)
@@ -176,6 +186,10 @@ def kv_free_paged_sequences(
     Pages past the kept tokens lose an owner, and their table entries become -1.
     """
     op = "kv_free_paged_sequences"
+    if type(block_size) is int and block_size > 0 and _hip.pages_native(
+            "free", op, None, None, block_tables, seq_lens, ref_counts, keep_lens, None, None, block_size, 0) is not None:
+        _emit(op, block_tables, "gfx950 page release")
+        return
     batch = _check_state(op, block_tables, seq_lens, ref_counts)
     rows = _row_values(op, "keep_lens", keep_lens, batch, block_tables.device)
     block_size = _check_block_size(op, block_size)
@@ -202,6 +216,11 @@ def kv_compact_paged_blocks(
     scales and reference count; table entries that named it follow.  Pages from ``n`` on are free afterwards.
     """
     op = "kv_compact_paged_blocks"
+    got = _hip.pages_native("compact", op, key_cache, value_cache, block_tables, None, ref_counts, None, k_scales,
+                            v_scales, 0, 0)
+    if got is not None:
+        _emit(op, key_cache, "gfx950 page compaction")
+        return got[1]
     _check_state(op, block_tables, None, ref_counts)
     block_size, pool = _check_pool(op, key_cache, value_cache, k_scales, v_scales, ref_counts)
     device = block_tables.device
