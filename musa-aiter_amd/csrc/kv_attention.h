@@ -357,7 +357,7 @@ inline RowsArgs rows_args(const AttnCall& c, int size) {
   return a;
 }
 
-// kv_attention_wide.hip: a call without an even cut whose tiles have kWideRows rows.
+// kv_attention_wide.hip: a call with a row table, in tiles of kWideRows rows.
 constexpr int kWideRows = 128;
 hipError_t launch_wide(const AttnCall& c, hipStream_t stream);
 

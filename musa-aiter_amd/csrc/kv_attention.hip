@@ -845,16 +845,22 @@ int row_tiles(const AttnCall& c) {
   return rows * group <= 16 ? 1 : 2;
 }
 
-// Whether prompt chunks' form (kv_attention_wide.hip) takes the call: more rows than half a tile of it on average.
+constexpr int64_t kComputeUnits = 256;
+
+// Whether prompt chunks' form (kv_attention_wide.hip) takes the call.  It decodes a token tile once for 128 rows, the
+// other form for every 16 or 32, but goes through the tokens of a part one tile at a time where the other one's waves
+// take four at once.  Rows are those of a kv head and sequence, on average: past 64 it wins (8 x 68 rows against 4096
+// tokens: 67 us, the other form 96), from 33 on where its tiles fill the chip's 256 CUs (32 x 36 rows against 2000
+// tokens, 328 tiles: 72 against 109 us; 24 x 36 rows against ~1500, 62 tiles: 26 against 20), below not (32 x 32 rows:
+// 71 against 65).
 bool takes_wide(const AttnCall& c) {
-  return takes_rows(c) && c.starts != nullptr && c.head_dim <= 128 && c.batch > 0 &&
-         (c.rows + c.batch - 1) / c.batch * (c.heads / c.kv_heads) > kWideRows / 2;
+  if (!takes_rows(c) || c.starts == nullptr || c.head_dim > 128 || c.batch < 1) return false;
+  const int64_t rows = (c.rows + c.batch - 1) / c.batch * (c.heads / c.kv_heads);
+  return rows > 64 || (rows > 32 && tiles_bound(c, kWideRows) * c.kv_heads >= kComputeUnits);
 }
 
 // How an even cut is made: workgroups (what the chip holds at once, or one for each unit that the tables have room
 // for) and rows of a part.
-constexpr int64_t kComputeUnits = 256;
-
 struct FlowPlan {
   int64_t groups, slot_rows;
 };
@@ -936,7 +942,8 @@ bool attention_flows(const AttnCall& c) {
 }
 
 // How a call is cut.  Decode steps of more than 512 tokens: evenly (0).  Others: enough parts for four workgroups
-// per CU, none below 256 tokens (a turn of a workgroup's four waves).
+// per CU, none below 256 tokens (a turn of a workgroup's four waves); prompt chunks' tiles, of which a CU holds two, are
+// cut only where they would leave some without any.
 int64_t attention_splits(const AttnCall& c, int64_t longest) {
   if (attention_flows(c) && longest > 512) return 0;
   const int64_t groups = takes_wide(c)   ? tiles_bound(c, kWideRows) * c.kv_heads

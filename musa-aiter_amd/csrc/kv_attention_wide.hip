@@ -10,6 +10,13 @@
 // of its 32, so the lane holds tokens 16 h + r of query row x: one 16-token group, which lies in one block (scales
 // and masks are per lane), in the order in which V's operand, 8 tokens a lane, wants the weights.  Nothing crosses
 // lanes but the running maximum.  The rest (codes, scaling of queries and weights) is as in kv_attention.hip.
+//
+// Two chunks of ~1800 rows (32 heads, 8 kv heads, 128 dims) against 2048..8192 cached tokens: 515 us, 695 TFLOP/s;
+// 8192 rows against 16384 tokens: 830 TFLOP/s (a large library product of bf16 matrices: 1260).  The instructions of a
+// wave's tile (1024 cycles of matrix instructions, about 1900 of others, a third of them exponentials) bound it; two
+// waves per SIMD overlap them in part.  Tried and slower or no faster: 256-row tiles of eight waves (6% faster for the
+// largest calls, 5 to 25% slower elsewhere), the next tile's score products among this tile's exponentials (their
+// registers leave one wave per SIMD: 800 us), wave priorities.
 #include "kv_attention.h"
 
 namespace kvhip {
@@ -19,8 +26,12 @@ namespace {
 using f32x16 = float __attribute__((ext_vector_type(16)));
 
 constexpr int kTileTokens = 64;
+// The maximum that weights are taken relative to stays behind the running one by up to a factor of two, which their
+// 16 bits have place for: the sums so far are rescaled less often.
+constexpr float kLag = 1.0f;
 constexpr int kWaveRows = 32;
 static_assert(kWideRows == kWaveRows * kWavesPerBlock && kTileTokens == 16 * kWavesPerBlock, "a wave decodes one group");
+
 
 template <int CODEC>
 __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -44,7 +55,7 @@ template <int HDP>
 struct TokenTile {
   u32x4 k[2][HDP / 16][kWave];
   u32x4 v[2][2][HDP / 32][kWave];
-  f32x4 scales[kWavesPerBlock];
+  f32x4 scales[4];
 };
 
 // Slot of row 8 a + 4 h0 + b, dims half h.
@@ -61,25 +72,44 @@ struct GroupCodes {
   bool seen;
 };
 
+// A table entry on its way: what is done with it must not wait for it where it is loaded.
+struct Entry {
+  uint32_t lo, hi;
+  bool inside;
+};
+
+__device__ __forceinline__ Entry load_entry(const RowsArgs& a, const uint8_t* table, int32_t token, int32_t end) {
+  const uint32_t column = group_column(a, token < end ? token : end - 1);
+  const uint8_t* p = table + static_cast<uint64_t>(column) * (a.c.wide_tables ? 8 : 4);
+  return {load4(p), load4(p + (a.c.wide_tables ? 4 : 0)), token < end};
+}
+
+// Its block, or -1; the same for the whole wave.
+__device__ __forceinline__ int32_t entry_block(const RowsArgs& a, const Entry& e) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(e.lo), hi = __builtin_amdgcn_readfirstlane(e.hi);
+  return e.inside && lo < static_cast<uint32_t>(a.num_blocks) && (!a.c.wide_tables || hi == 0) ? static_cast<int32_t>(lo) : -1;
+}
+
 template <int HDP, bool EXACT>
 __device__ __forceinline__ void load_group(const RowsArgs& a, int32_t head, int32_t token, int32_t block,
                                            GroupCodes<HDP>& codes) {
   const AttnCall& c = a.c;
-  const int lane = lane_now();
-  const int64_t blk = block < 0 ? 0 : block;  // block 0, which every cache has; its scores are masked
+  const int lane = lane_id();
+  block = __builtin_amdgcn_readfirstlane(block);  // one for the wave: addresses are a scalar and 32 bits of a lane
+  const int64_t blk = block < 0 ? 0 : block;      // block 0, which every cache has; its scores are masked
   const int64_t off = static_cast<int64_t>(head) * a.hd * a.bs + group_place(a, token);
   const uint8_t* k = static_cast<const uint8_t*>(c.cache[0]) + blk * c.cache_block_stride[0] + off;
   const uint8_t* v = static_cast<const uint8_t*>(c.cache[1]) + blk * c.cache_block_stride[1] + off;
   const int octet = (lane >> 2) & (HDP / 8 - 1), quad = lane & 3, last = a.hd - 1;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int d = octet + j * (HDP / 8);
-    codes.k[j] = load4(k + (EXACT ? d : min(d, last)) * a.bs + 4 * quad);
+    const uint32_t at = (EXACT ? octet : min(octet + j * (HDP / 8), last)) * a.bs + 4 * quad;
+    codes.k[j] = load4(k + (EXACT ? j * (HDP / 8) * a.bs : 0) + at);
   }
 #pragma unroll
   for (int e = 0; e < HDP / kWave; ++e) {
-    const int d = lane + e * kWave;
-    codes.v[e] = ld16_cached(v + (EXACT ? d : min(d, last)) * a.bs);
+    const uint32_t at = (EXACT ? lane : min(lane + e * kWave, last)) * a.bs;
+    codes.v[e] = ld16_cached(v + (EXACT ? e * kWave * a.bs : 0) + at);
   }
   codes.ks = c.scale[0][blk * c.scale_block_stride[0] + head * c.scale_head_stride[0]];
   codes.vs = c.scale[1][blk * c.scale_block_stride[1] + head * c.scale_head_stride[1]];
@@ -170,12 +200,9 @@ __device__ __forceinline__ float read_query(const RowsArgs& a, const uint16_t* r
   return __builtin_ldexpf(static_cast<float>(a.c.softmax_scale) * kLog2e, Mma<CODEC>::kCodeShift - up);
 }
 
-// Waves per SIMD that the registers leave room for (without spills).
-template <int HDP, int CODEC, int DT>
-constexpr int kWideOccupancy = HDP > 64 && kQueryParts<CODEC, DT> > 1 ? 1 : 2;
 
 template <int HDP, bool EXACT, int CODEC, int DT>
-__global__ __launch_bounds__(kBlockThreads, (kWideOccupancy<HDP, CODEC, DT>))
+__global__ __launch_bounds__(kBlockThreads, 2)
 void attention_wide_kernel(const RowsArgs a, uint32_t tiles) {
   const AttnCall& c = a.c;
   __shared__ TokenTile<HDP> buffer[2];
@@ -201,11 +228,11 @@ void attention_wide_kernel(const RowsArgs a, uint32_t tiles) {
   int32_t token = static_cast<int32_t>(span.lo);
   const int mine_at = 16 * wave;  // the wave's group in a tile
   GroupCodes<HDP> codes;
-  int32_t next_block = -1;
+  Entry next_entry;
   if (token < last) {
-    const int32_t block = group_block(a, table, token + mine_at, last);
-    next_block = group_block(a, table, token + kTileTokens + mine_at, last);
-    load_group<HDP, EXACT>(a, head, token + mine_at, block, codes);
+    const Entry entry = load_entry(a, table, token + mine_at, last);
+    next_entry = load_entry(a, table, token + kTileTokens + mine_at, last);
+    load_group<HDP, EXACT>(a, head, token + mine_at, entry_block(a, entry), codes);
   }
 
   const Mma<CODEC> mma;
@@ -226,8 +253,9 @@ void attention_wide_kernel(const RowsArgs a, uint32_t tiles) {
   if (token < last) {
     decode_group<HDP, CODEC>(mma, codes, buffer[0]);
     if (token + kTileTokens < last) {
-      load_group<HDP, EXACT>(a, head, token + kTileTokens + mine_at, next_block, codes);
-      next_block = group_block(a, table, token + 2 * kTileTokens + mine_at, last);
+      const int32_t block = entry_block(a, next_entry);
+      next_entry = load_entry(a, table, token + 2 * kTileTokens + mine_at, last);
+      load_group<HDP, EXACT>(a, head, token + kTileTokens + mine_at, block, codes);
     }
   }
   __syncthreads();
@@ -244,12 +272,21 @@ void attention_wide_kernel(const RowsArgs a, uint32_t tiles) {
 #pragma unroll
         for (int part = 0; part < kQueryParts<CODEC, DT>; ++part) score[p] = mma32<CODEC>(k, q[part][s], score[p]);
       }
+    // Operands on their way three products ahead.
+    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+    for (int i = 0; i < HDP / 16 - 3; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
     // The next tile, into the buffer that was read before the last barrier.
     if (token + kTileTokens < last) {
       decode_group<HDP, CODEC>(mma, codes, buffer[now ^ 1]);
       if (token + 2 * kTileTokens < last) {
-        load_group<HDP, EXACT>(a, head, token + 2 * kTileTokens + mine_at, next_block, codes);
-        next_block = group_block(a, table, token + 3 * kTileTokens + mine_at, last);
+        const int32_t block = entry_block(a, next_entry);
+        next_entry = load_entry(a, table, token + 3 * kTileTokens + mine_at, last);
+        load_group<HDP, EXACT>(a, head, token + 2 * kTileTokens + mine_at, block, codes);
       }
     }
 
@@ -276,14 +313,14 @@ void attention_wide_kernel(const RowsArgs a, uint32_t tiles) {
       top = fmaxf(top, __builtin_fmaf(most, f[p], __builtin_amdgcn_fmed3f(__builtin_amdgcn_logf(scales[p][1]), -100.0f, 100.0f)));
     }
     top = fmaxf(top, other_half(top));
-    const float ref = top == -__builtin_inff() ? 0.0f : top;
-    if (ballot(top > m) != 0) {
-      const float fade = __builtin_amdgcn_exp2f(m - ref);
+    if (ballot(top > m + kLag) != 0) {
+      const float fade = __builtin_amdgcn_exp2f(m - (top == -__builtin_inff() ? 0.0f : top));
       l *= fade;
 #pragma unroll
       for (int i = 0; i < HDP / 32; ++i) acc[i] *= fade;
       m = top;
     }
+    const float ref = m == -__builtin_inff() ? 0.0f : m;
     u32x4 w[2][2][kParts];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
