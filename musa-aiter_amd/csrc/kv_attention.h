@@ -297,15 +297,27 @@ __device__ __forceinline__ int32_t group_place(const RowsArgs& a, int32_t token)
   return token - static_cast<int32_t>(group_column(a, token)) * a.bs;
 }
 
-// The block of the group, or -1.
-__device__ __forceinline__ int32_t group_block(const RowsArgs& a, const uint8_t* row, int32_t token, int32_t end) {
-  if (token >= end) return -1;
-  const int64_t blk = int_at(row, group_column(a, token), a.c.wide_tables);
-  return blk >= 0 && blk < a.num_blocks ? static_cast<int32_t>(blk) : -1;
-}
-
 __device__ __forceinline__ uint32_t load4(const uint8_t* p) {
   return *reinterpret_cast<const KVHIP_GLOBAL uint32_t*>(reinterpret_cast<uint64_t>(p));
+}
+
+// The table entry of a group, on its way: nothing is done with it where it is loaded, which would wait for it and for
+// the codes that were asked for before it.
+struct Entry {
+  uint32_t lo, hi;
+  bool inside;  // the group begins in front of `end`
+};
+
+__device__ __forceinline__ Entry load_entry(const RowsArgs& a, const uint8_t* row, int32_t token, int32_t end) {
+  const uint32_t column = group_column(a, min(token, end - 1));
+  const uint8_t* p = row + static_cast<uint64_t>(column) * (a.c.wide_tables ? 8 : 4);
+  return {load4(p), load4(p + (a.c.wide_tables ? 4 : 0)), token < end};
+}
+
+// Its block, or -1.
+__device__ __forceinline__ int32_t entry_block(const RowsArgs& a, const Entry& e) {
+  const bool good = e.inside && e.lo < static_cast<uint32_t>(a.num_blocks) && (!a.c.wide_tables || e.hi == 0);
+  return good ? static_cast<int32_t>(e.lo) : -1;
 }
 
 // Positions [lo, hi) that a row sees.

@@ -193,9 +193,17 @@ struct GroupIds {
   int32_t k, v;  // blocks of the groups whose keys and values the lane loads
 };
 
-__device__ __forceinline__ GroupIds tile_ids(const RowsArgs& a, const uint8_t* row, int32_t token, int32_t end) {
+struct GroupEntries {
+  Entry k, v;
+};
+
+__device__ __forceinline__ GroupEntries load_entries(const RowsArgs& a, const uint8_t* row, int32_t token, int32_t end) {
   const int lane = lane_now(), x = lane & 15, g = lane >> 4;
-  return {group_block(a, row, token + 16 * (x >> 2), end), group_block(a, row, token + 16 * g, end)};
+  return {load_entry(a, row, token + 16 * (x >> 2), end), load_entry(a, row, token + 16 * g, end)};
+}
+
+__device__ __forceinline__ GroupIds group_ids(const RowsArgs& a, const GroupEntries& e) {
+  return {entry_block(a, e.k), entry_block(a, e.v)};
 }
 
 // DIMS rows of the keys of 64 tokens: dword l is row d = first + 4 l + g of the lane's 4 tokens.  A group without a block reads block
@@ -295,15 +303,16 @@ __device__ __forceinline__ void key_products(const Mma<CODEC>& mma, const uint32
 
 // One step of the running softmax: scores in, weights (probability * value scale) out; rescales the state where
 // the maximum grew.
-template <int HDP, int CODEC>
+template <int HDP, int CODEC, typename SightOf>
 __device__ __forceinline__ void soften(f32x4* score, float factor, const GroupScales& scales, bool masked,
-                                       int32_t token, const Sight& sight, RowState<HDP>& s) {
+                                       int32_t token, SightOf sight_of, RowState<HDP>& s) {
   const float f = factor * scales.ks, vs = scales.vs;
   const bool seen = scales.seen;
 #pragma unroll
   for (int i = 0; i < 4; ++i) score[i] *= f;
   if (masked) {
     const int first = token + 16 * (lane_now() >> 4);
+    const Sight sight = sight_of();
     const int lo = sight.lo - first, hi = seen ? sight.hi - first : 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -388,7 +397,7 @@ constexpr int kJoinDims = 128;
 // Waves per SIMD that the registers of a variant leave room for (without spills; looked up in the compiler's report).
 constexpr int rows_occupancy(int hdp, bool exact, int tiles, int codec) {
   if (hdp * tiles > 128) return 1;
-  return tiles > 1 || (hdp == 128 && (!exact || codec == kE5M2)) ? 2 : 3;
+  return tiles > 1 || (hdp == 128 && !exact && codec == kE5M2) ? 2 : 3;
 }
 constexpr int kJoinStride = kJoinDims + 4;
 
@@ -400,6 +409,13 @@ struct Segment {
   int64_t parts, first_part;
   bool by_row;
 };
+
+// What row r of a tile sees.  (Worked out where a tile of tokens needs it: held, it would cost registers.)
+__device__ __forceinline__ Sight row_sight(const RowsArgs& a, const RowTile& tile, int32_t before, int32_t r) {
+  const int32_t at = tile.base + r, pos = before + at / a.group;
+  if (at >= tile.count * a.group) return {0, 0};
+  return {a.window > 0 ? max(pos - a.window + 1, 0) : 0, min(pos + 1, a.room)};
+}
 
 template <int HDP, int NT, int CODEC, int DT>
 struct RowsShared {
@@ -428,11 +444,13 @@ __device__ __forceinline__ void run_segment(const RowsArgs& a, const Segment& se
   int32_t token = seg.lo + wave * kWaveTokens;
   uint32_t k[kDims / 4];
   u32x4 v[kDims / 16];
-  GroupIds ids, next_ids;
+  GroupIds ids;
+  GroupEntries next_entries;
   GroupScales scales;
   if (token < last) {  // on their way while the queries are read
-    ids = tile_ids(a, row, token, last);
-    next_ids = tile_ids(a, row, token + kStep, last);
+    const GroupEntries entries = load_entries(a, row, token, last);
+    next_entries = load_entries(a, row, token + kStep, last);
+    ids = group_ids(a, entries);
     scales = load_scales(c, head, ids);
     load_keys<kDims, EXACT>(a, head_off, token, ids, 0, k);
     load_values<kDims, EXACT>(a, head_off, token, ids, 0, v);
@@ -442,18 +460,14 @@ __device__ __forceinline__ void run_segment(const RowsArgs& a, const Segment& se
   // Rows and what they see; the waves share the queries.
   QueryTiles<HDP, NT, CODEC, DT>& queries = shared.queries;
   RowState<HDP> state[NT];
-  Sight sight[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int32_t r = tile.base + 16 * n + x;
     const bool mine = r < in_seq;
     const int32_t i = mine ? r / group : 0, h = mine ? r - i * group : 0;
-    const int32_t pos = before + i;
     if (wave == n)
       queries.template fill<EXACT>(a, n, static_cast<const uint16_t*>(c.query) + (tile.first + i) * c.query_row_stride +
                                              (head * group + h) * c.query_head_stride, mine);
-    sight[n].hi = mine ? min(pos + 1, a.room) : 0;
-    sight[n].lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
     state[n].m = -__builtin_inff();
     state[n].l = 0.0f;
 #pragma unroll
@@ -472,10 +486,12 @@ __device__ __forceinline__ void run_segment(const RowsArgs& a, const Segment& se
       }
       // Loads return in order: table entries are read two tiles ahead, in front of the keys whose arrival they
       // would else be waited for with.
-      GroupIds later_ids;
+      GroupIds next_ids;
+      GroupEntries later_entries;
       GroupScales next_scales;
       if (next < last) {
-        later_ids = tile_ids(a, row, next + kStep, last);
+        next_ids = group_ids(a, next_entries);
+        later_entries = load_entries(a, row, next + kStep, last);
         next_scales = load_scales(c, head, next_ids);
         load_keys<kDims, EXACT>(a, head_off, next, next_ids, 0, k);
       }
@@ -483,7 +499,8 @@ __device__ __forceinline__ void run_segment(const RowsArgs& a, const Segment& se
       u32x4 p[NT][2][kWeightParts<CODEC, DT>];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        soften<HDP, CODEC>(score[n], queries.factor[n][x], scales, masked, token, sight[n], state[n]);
+        soften<HDP, CODEC>(score[n], queries.factor[n][x], scales, masked, token,
+                           [&] { return row_sight(a, tile, before, 16 * n + (lane_now() & 15)); }, state[n]);
         pack_weights<CODEC, DT>(score[n], 0, p[n][0]);
         pack_weights<CODEC, DT>(score[n], 1, p[n][1]);
       }
@@ -495,7 +512,7 @@ __device__ __forceinline__ void run_segment(const RowsArgs& a, const Segment& se
       if (next >= last) break;
       load_values<kDims, EXACT>(a, head_off, next, next_ids, 0, v);
       ids = next_ids;
-      next_ids = later_ids;
+      next_entries = later_entries;
       scales = next_scales;
       token = next;
     }
@@ -520,7 +537,7 @@ __device__ __forceinline__ void run_segment(const RowsArgs& a, const Segment& se
       for (int k = 0; k < kChunk / 16; ++k)
         *reinterpret_cast<f32x4*>(&shared.joined[wave][x][16 * k + 4 * (lane >> 4)]) = state[n].acc[d0 / 16 + k];
       __syncthreads();
-      const int at = threadIdx.x >> 4;
+      const int thread = reread(threadIdx.x), at = thread >> 4;
       const int32_t r = tile.base + 16 * n + at;
       if (r >= in_seq) continue;
       const int32_t i = r / group;
@@ -536,7 +553,7 @@ __device__ __forceinline__ void run_segment(const RowsArgs& a, const Segment& se
         fade[w] = __builtin_amdgcn_exp2f(shared.ml[w][at][0] - ref);
         sum += shared.ml[w][at][1] * fade[w];
       }
-      for (int k = threadIdx.x & 15; k < kChunk; k += 16) {
+      for (int k = thread & 15; k < kChunk; k += 16) {
         float o = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWavesPerBlock; ++w) o += shared.joined[w][at][k] * fade[w];
@@ -548,7 +565,7 @@ __device__ __forceinline__ void run_segment(const RowsArgs& a, const Segment& se
         }
         store_o<DT>(c.out, rh * a.hd + d0 + k, sum == 0.0f ? 0.0f : o / sum);
       }
-      if (d0 == 0 && (threadIdx.x & 15) == 0) {
+      if (d0 == 0 && (thread & 15) == 0) {
         if (seg.parts > 0) {
           part_ml(c, part)[0] = top;
           part_ml(c, part)[1] = sum;
@@ -867,12 +884,11 @@ struct FlowPlan {
 
 FlowPlan flow_plan(const AttnCall& c) {
   const int tiles = row_tiles(c), size = 16 * tiles;
-  const bool exact = c.head_dim == 64 || c.head_dim == 96 || c.head_dim == 128 || c.head_dim == 256;
-  const int hdp = c.head_dim <= 64 ? 64 : exact && c.head_dim == 96 ? 96 : c.head_dim <= 128 ? 128 : 256;
+  const int hdp = c.head_dim <= 64 ? 64 : c.head_dim == 96 ? 96 : c.head_dim <= 128 ? 128 : 256;
   const int64_t lines = tiles_bound(c, size) * c.kv_heads, group = c.heads / c.kv_heads;
   const int64_t turns = (c.max_blocks * c.block_size + kUnitTokens - 1) / kUnitTokens;
   const int64_t most = lines * (turns > 0 ? turns : 1);
-  const int64_t held = kComputeUnits * rows_occupancy(hdp, exact, tiles, c.codec);
+  const int64_t held = kComputeUnits * rows_occupancy(hdp, c.head_dim == hdp, tiles, c.codec);
   return {most < held ? most : held, group < size ? group : size};
 }
 

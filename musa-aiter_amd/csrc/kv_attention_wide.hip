@@ -72,31 +72,14 @@ struct GroupCodes {
   bool seen;
 };
 
-// A table entry on its way: what is done with it must not wait for it where it is loaded.
-struct Entry {
-  uint32_t lo, hi;
-  bool inside;
-};
-
-__device__ __forceinline__ Entry load_entry(const RowsArgs& a, const uint8_t* table, int32_t token, int32_t end) {
-  const uint32_t column = group_column(a, token < end ? token : end - 1);
-  const uint8_t* p = table + static_cast<uint64_t>(column) * (a.c.wide_tables ? 8 : 4);
-  return {load4(p), load4(p + (a.c.wide_tables ? 4 : 0)), token < end};
-}
-
-// Its block, or -1; the same for the whole wave.
-__device__ __forceinline__ int32_t entry_block(const RowsArgs& a, const Entry& e) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(e.lo), hi = __builtin_amdgcn_readfirstlane(e.hi);
-  return e.inside && lo < static_cast<uint32_t>(a.num_blocks) && (!a.c.wide_tables || hi == 0) ? static_cast<int32_t>(lo) : -1;
-}
-
 template <int HDP, bool EXACT>
 __device__ __forceinline__ void load_group(const RowsArgs& a, int32_t head, int32_t token, int32_t block,
                                            GroupCodes<HDP>& codes) {
   const AttnCall& c = a.c;
   const int lane = lane_id();
-  block = __builtin_amdgcn_readfirstlane(block);  // one for the wave: addresses are a scalar and 32 bits of a lane
-  const int64_t blk = block < 0 ? 0 : block;      // block 0, which every cache has; its scores are masked
+  // Addresses are a scalar (the block is the same for the wave) and 32 bits of a lane.  A group without a block reads
+  // block 0, which every cache has; its scores are masked.
+  const int64_t blk = block < 0 ? 0 : block;
   const int64_t off = static_cast<int64_t>(head) * a.hd * a.bs + group_place(a, token);
   const uint8_t* k = static_cast<const uint8_t*>(c.cache[0]) + blk * c.cache_block_stride[0] + off;
   const uint8_t* v = static_cast<const uint8_t*>(c.cache[1]) + blk * c.cache_block_stride[1] + off;
@@ -232,7 +215,7 @@ void attention_wide_kernel(const RowsArgs a, uint32_t tiles) {
   if (token < last) {
     const Entry entry = load_entry(a, table, token + mine_at, last);
     next_entry = load_entry(a, table, token + kTileTokens + mine_at, last);
-    load_group<HDP, EXACT>(a, head, token + mine_at, entry_block(a, entry), codes);
+    load_group<HDP, EXACT>(a, head, token + mine_at, __builtin_amdgcn_readfirstlane(entry_block(a, entry)), codes);
   }
 
   const Mma<CODEC> mma;
@@ -253,7 +236,7 @@ void attention_wide_kernel(const RowsArgs a, uint32_t tiles) {
   if (token < last) {
     decode_group<HDP, CODEC>(mma, codes, buffer[0]);
     if (token + kTileTokens < last) {
-      const int32_t block = entry_block(a, next_entry);
+      const int32_t block = __builtin_amdgcn_readfirstlane(entry_block(a, next_entry));
       next_entry = load_entry(a, table, token + 2 * kTileTokens + mine_at, last);
       load_group<HDP, EXACT>(a, head, token + kTileTokens + mine_at, block, codes);
     }
@@ -284,7 +267,7 @@ void attention_wide_kernel(const RowsArgs a, uint32_t tiles) {
     if (token + kTileTokens < last) {
       decode_group<HDP, CODEC>(mma, codes, buffer[now ^ 1]);
       if (token + 2 * kTileTokens < last) {
-        const int32_t block = entry_block(a, next_entry);
+        const int32_t block = __builtin_amdgcn_readfirstlane(entry_block(a, next_entry));
         next_entry = load_entry(a, table, token + 3 * kTileTokens + mine_at, last);
         load_group<HDP, EXACT>(a, head, token + 2 * kTileTokens + mine_at, block, codes);
       }
