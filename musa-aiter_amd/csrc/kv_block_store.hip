@@ -17,7 +17,11 @@
 // the tokens of columns 4 tg .. 4 tg + 3 and dims 8 pc .. 8 pc + 7, so that four codes of a dim are one dword of
 // the cache; two exchanges between the four lanes of a piece (v_permlane32_swap, v_permlane16_swap) then give
 // every lane whole 16-column rows of two dims.  Other shapes go element by element.
-// What bounds it: few tokens, latency (a token's row, its block's scale, the stores); many, memory.
+// What bounds it: few tokens, latency (a token's row, its block's scale, the stores); many, memory and the ten or so
+// operations that a value takes (E4M3, whose small quotients are more often there to be flushed, is the slower).
+// Measured: 64 tokens of 8 x 128 bf16 into pages of 16, 5.9 us; 30977 tokens, 52 us with the check of the slots
+// (3.6 TB/s; a large copy 4.7); 16 layers of 4001 tokens fp16 into pages of 64, 116 us (179 with the pieces read
+// twice), of bf16 as E4M3 135 us.
 #include "kv_serving.h"
 
 namespace kvhip {
@@ -150,16 +154,50 @@ __device__ __forceinline__ uint32_t group_tokens(const COLUMNS& token_of, int64_
 }
 
 template <int LDT>
-__device__ __forceinline__ void most_of(const Piece<LDT>* x, float* most, bool* odd) {
+__device__ __forceinline__ float most_of(const Piece<LDT>* x, float most) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float v = fabsf(x[i].at(j));
-      const bool finite = v < __builtin_inff();
-      *odd |= !finite;
-      *most = fmaxf(*most, finite ? v : 0.0f);
+      most = fmaxf(most, v < __builtin_inff() ? v : 0.0f);
     }
+  return most;
+}
+
+// The largest magnitude bits of the pieces, for 16-bit values those of two in the halves of a dword: one or two
+// operations a value, where values with their infinities and NaN left out (most_of) take five.
+template <int LDT>
+__device__ __forceinline__ uint32_t top_bits(const Piece<LDT>* x, uint32_t top) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int w = 0; w < (LDT == kLinF32 ? 8 : 4); ++w) {
+      if constexpr (LDT == kLinF32)
+        top = max(top, x[i].raw[w >> 2][w & 3] & 0x7FFFFFFFu);
+      else
+        top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
+                                                                     __builtin_bit_cast(u16x2, x[i].raw[0][w] & 0x7FFF7FFFu)));
+    }
+  return top;
+}
+
+// The magnitude behind a lane's top_bits; with infinities and NaN at or past kInfinity.
+template <int LDT>
+constexpr uint32_t kInfinity = LDT == kLinF32 ? 0x7F800000u : LDT == kLinF16 ? 0x7C00u : 0x7F80u;
+
+template <int LDT>
+__device__ __forceinline__ uint32_t wave_top(uint32_t top) {
+  if constexpr (LDT != kLinF32) top = max(top & 0xFFFFu, top >> 16);
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o)));
+  return __builtin_amdgcn_readfirstlane(top);
+}
+
+template <int LDT>
+__device__ __forceinline__ float top_value(uint32_t bits) {
+  if constexpr (LDT == kLinF32) return __uint_as_float(bits);
+  else return lin_to_f32<LDT>(static_cast<uint16_t>(bits));
 }
 
 // Bytes of columns 4 k .. 4 k + 3 that are written, as a mask of the dword.
@@ -195,39 +233,63 @@ __device__ __forceinline__ uint32_t recode(uint32_t w, float before, float now) 
   return out;
 }
 
-// HOLD: the block is one group of at most 128 dims, whose pieces stay in registers between the two passes; else
-// the second pass reads them again.
-template <int CODEC, int LDT, bool HOLD, typename COLUMNS>
+// HELD > 0: the block is HELD groups of at most 128 dims, whose pieces stay in registers between the two passes; else
+// the second pass reads them again (from memory: what the chip's waves read between the two is more than its L2).
+template <int CODEC, int LDT, int HELD, typename COLUMNS>
 __device__ __forceinline__ void store_unit_pieces(const Unit& u, const COLUMNS& token_of) {
-  const int groups = HOLD ? 1 : static_cast<int>(u.bs >> 4), chunks = HOLD ? 1 : static_cast<int>((u.hd + 127) >> 7);
+  constexpr int kHeld = HELD > 0 ? HELD : 1;
+  const int groups = HELD > 0 ? HELD : static_cast<int>(u.bs >> 4);
+  const int chunks = HELD > 0 ? 1 : static_cast<int>((u.hd + 127) >> 7);
   const float before = *u.scale;
-  float most = 0.0f;
-  bool odd = false;
-  int32_t tok[4];
-  uint32_t written = 0;
-  Piece<LDT> x[4];
-  for (int g = 0; g < groups; ++g) {
-    written = group_tokens(token_of, g, tok);
-    if (written == 0) continue;
-    for (int ch = 0; ch < chunks; ++ch) {
-      load_pieces<LDT>(u, tok, ch, x);
-      most_of<LDT>(x, &most, &odd);
+  int32_t tok[kHeld][4];
+  uint32_t mask[kHeld], top = 0;
+  Piece<LDT> pieces[kHeld][4];
+  // The groups' pieces one after the other, or all that are held.
+  auto each_group = [&](auto&& see) {
+    if constexpr (HELD > 0) {
+#pragma unroll
+      for (int g = 0; g < HELD; ++g) see(pieces[g]);
+    } else {
+      for (int g = 0; g < groups; ++g) {
+        if (group_tokens(token_of, g, tok[0]) == 0) continue;
+        for (int ch = 0; ch < chunks; ++ch) {
+          load_pieces<LDT>(u, tok[0], ch, pieces[0]);
+          see(pieces[0]);
+        }
+      }
     }
+  };
+  if constexpr (HELD > 0) {  // all on their way together
+#pragma unroll
+    for (int g = 0; g < HELD; ++g) mask[g] = group_tokens(token_of, g, tok[g]);
+#pragma unroll
+    for (int g = 0; g < HELD; ++g) load_pieces<LDT>(u, tok[g], 0, pieces[g]);
   }
-  most = wave_max(most);
+  each_group([&](const Piece<LDT>* x) { top = top_bits<LDT>(x, top); });
+  top = wave_top<LDT>(top);
+  const bool odd = top >= kInfinity<LDT>;
+  float most = 0.0f;
+  if (odd) {
+    each_group([&](const Piece<LDT>* x) { most = most_of<LDT>(x, most); });
+    most = wave_max(most);
+  } else {
+    most = top_value<LDT>(top);
+  }
   const bool anew = token_of(0) >= 0 || scale_refused(before);
   const float now = new_scale<CODEC>(most, before, anew);
   const bool same = !anew && now == before;
   // The quotient with one hoisted reciprocal is exact for scales in [2^-60, 2^60) and every finite value: a value
   // so small that its residuals underflow has a quotient below 2^-40, which is flushed either way.
-  const bool exact = ballot(odd) == 0 && now < 0x1p60f;
+  const bool exact = !odd && now < 0x1p60f;
   const float r = div_rn(1.0f, now);
   const int tg = lane_id() >> 4, pc = lane_id() & 15;
+#pragma unroll kHeld
   for (int g = 0; g < groups; ++g) {
-    if (!HOLD) written = group_tokens(token_of, g, tok);
+    const uint32_t written = HELD > 0 ? mask[HELD > 0 ? g : 0] : group_tokens(token_of, g, tok[0]);
+    Piece<LDT>* x = pieces[HELD > 0 ? g : 0];
     if (written == 0 && same) continue;
     for (int ch = 0; ch < chunks; ++ch) {
-      if (!HOLD) load_pieces<LDT>(u, tok, ch, x);
+      if (HELD == 0) load_pieces<LDT>(u, tok[0], ch, x);
       uint32_t w[8];
       u32x4 row[2];
 #pragma unroll
@@ -265,14 +327,15 @@ __device__ __forceinline__ void store_unit_pieces(const Unit& u, const COLUMNS& 
   if (lane_id() == 0) *u.scale = now;
 }
 
-enum StoreForm : int { kElements = 0, kPieces = 1, kHeldPieces = 2 };
+// By elements, by pieces, or by pieces of which a block's kHeldPieces + n - 1 groups are held.
+enum StoreForm : int { kElements = 0, kPieces = 1, kHeldPieces = 2, kHeldPieces2 = 3, kHeldPieces4 = 5 };
 
 template <int CODEC, int LDT, int FORM, typename COLUMNS>
 __device__ __forceinline__ void store_one(const BlockStoreParams& p, int64_t block, int64_t layer, int64_t unit,
                                           const COLUMNS& token_of) {
   const Unit u = unit_of(p, LDT == kLinF32 ? 4 : 2, block, layer, unit >> 1, static_cast<int>(unit & 1));
   if constexpr (FORM == kElements) store_unit<CODEC, LDT>(u, token_of);
-  else store_unit_pieces<CODEC, LDT, FORM == kHeldPieces>(u, token_of);
+  else store_unit_pieces<CODEC, LDT, FORM - kPieces>(u, token_of);
 }
 
 // Few tokens: one workgroup per (token, four units, layer), which makes its block's columns from all the slots.
@@ -387,7 +450,11 @@ hipError_t launch_typed(const BlockStoreParams& p, hipStream_t stream) {
     all |= reinterpret_cast<uint64_t>(p.lin[kv]) | reinterpret_cast<uint64_t>(p.cache[kv]) |
            static_cast<uint64_t>(p.block_stride[kv]) | static_cast<uint64_t>(p.num_layers > 1 ? p.layer_stride[kv] : 0);
   if (all % 16 != 0 || p.head_dim % 8 != 0) return launch_form<CODEC, LDT, kElements>(p, stream);
-  if (p.block_size == 16 && p.head_dim <= 128) return launch_form<CODEC, LDT, kHeldPieces>(p, stream);
+  if (p.head_dim <= 128) {
+    if (p.block_size == 16) return launch_form<CODEC, LDT, kHeldPieces>(p, stream);
+    if (p.block_size == 32) return launch_form<CODEC, LDT, kHeldPieces2>(p, stream);
+    if (p.block_size == 64) return launch_form<CODEC, LDT, kHeldPieces4>(p, stream);
+  }
   return launch_form<CODEC, LDT, kPieces>(p, stream);
 }
 
