@@ -13,6 +13,8 @@
 namespace kvhip {
 namespace {
 
+using i32x4 = int32_t __attribute__((ext_vector_type(4)));
+
 constexpr int kScanThreads = 1024;
 constexpr int kScanWaves = kScanThreads / kWave;
 constexpr int kPerThread = 8;                               // pages a thread looks at per step of a scan
@@ -33,7 +35,7 @@ struct PagesArgs {
   int64_t* src;      // moved pages
   int64_t* dst;
   int64_t* a;        // fork: new rows; extend: first need of each row; compact: new id of pages >= live
-  int64_t* b;        // fork: new lengths; extend: old lengths
+  int64_t* b;        // fork: new lengths
   int64_t* list;     // extend: free pages taken
 };
 
@@ -158,11 +160,9 @@ struct ExtendRow {
 template <typename IT>
 __global__ __launch_bounds__(kScanThreads) void pages_extend_kernel(const PagesArgs a) {
   const musa_aiter_hip_pages_call& c = a.c;
-  IT* lens = static_cast<IT*>(c.lens);
   IT* refs = static_cast<IT*>(c.refs);
-  IT* tables = static_cast<IT*>(c.tables);
   __shared__ int64_t part[kScanWaves];
-  __shared__ int32_t grown[kScanThreads];  // partial last page that a row grows into, or -1
+  __shared__ alignas(16) int32_t grown[kScanThreads];  // partial last page that a row grows into, or -1
   __shared__ int too_long, shared_pages;
   if (threadIdx.x == 0) too_long = 0;
   // What every row needs, and the sum in front of it.
@@ -198,8 +198,15 @@ __global__ __launch_bounds__(kScanThreads) void pages_extend_kernel(const PagesA
         grown[threadIdx.x] = theirs;
         __syncthreads();
         const int until = from < base ? kScanThreads : static_cast<int>(threadIdx.x);
-        if (owners > 1)
-          for (int o = 0; o < until; ++o) earlier += grown[o] == last;
+        if (owners > 1) {
+          int o = 0;
+#pragma unroll 4
+          for (; o + 4 <= until; o += 4) {
+            const i32x4 g = *reinterpret_cast<const i32x4*>(grown + o);
+            earlier += (g[0] == last) + (g[1] == last) + (g[2] == last) + (g[3] == last);
+          }
+          for (; o < until; ++o) earlier += grown[o] == last;
+        }
       }
       copy = owners > 1 && earlier < owners - 1;
     }
@@ -233,7 +240,7 @@ __global__ __launch_bounds__(kScanThreads) void pages_extend_kernel(const PagesA
     a.head->fits = fits;
     *c.result = too_long ? -(int64_t{1} << 62) : free_all - need_all;
   }
-  // The rows, a wave each; the copies' pairs keep the rows' order through a second sum.
+  // The copies' pairs, in the rows' order.
   int64_t moves = 0;
   for (int64_t base = 0; base < c.batch; base += kScanThreads) {
     const int64_t b = base + threadIdx.x;
@@ -248,27 +255,6 @@ __global__ __launch_bounds__(kScanThreads) void pages_extend_kernel(const PagesA
     moves += sum;
   }
   if (threadIdx.x == 0) a.head->moves = moves;
-  __syncthreads();  // rows are read above, written below
-  for (int64_t b = threadIdx.x >> 6; b < c.batch; b += kScanWaves) {
-    const ExtendRow<IT> r(c, b);
-    if (lane_id() == 0) a.b[b] = r.len;
-    if (!fits || r.grow == 0) continue;
-    IT* row = tables + b * c.table_stride;
-    const int64_t first = a.a[b] >> 1;
-    const int copy = static_cast<int>(a.a[b] & 1);
-    if (copy && lane_id() == 0) {
-      const int64_t page = a.list[first];
-      add_ref(refs, r.last, -1);
-      refs[page] = 1;
-      row[r.had - 1] = static_cast<IT>(page);
-    }
-    for (int64_t j = r.had + lane_id(); j < r.has; j += kWave) {
-      const int64_t page = a.list[first + copy + j - r.had];
-      refs[page] = 1;
-      row[j] = static_cast<IT>(page);
-    }
-    if (lane_id() == 0) lens[b] = static_cast<IT>(r.len + r.grow);
-  }
 }
 
 // ----- compact ----------------------------------------------------------------------------------
@@ -357,21 +343,46 @@ __device__ __forceinline__ void move_pages(const PagesArgs& a) {
   }
 }
 
+// The rows, a workgroup each (one after the other by the scan's single workgroup they took 15 us for 128 rows), and
+// the copies.
 template <typename IT, int VEC>
 __global__ __launch_bounds__(kBlockThreads) void pages_extend_finish_kernel(const PagesArgs a) {
   const musa_aiter_hip_pages_call& c = a.c;
+  IT* lens = static_cast<IT*>(c.lens);
+  IT* refs = static_cast<IT*>(c.refs);
   const bool fits = a.head->fits != 0;
-  const int64_t threads = static_cast<int64_t>(gridDim.x) * kBlockThreads;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlockThreads + threadIdx.x; i < c.batch * c.max_new;
-       i += threads) {
-    const int64_t b = i / c.max_new, k = i - b * c.max_new;
-    int64_t slot = -1;
-    if (fits && k < row_value(c, b)) {
-      const int64_t pos = a.b[b] + k, j = pos / c.block_size;
-      const int64_t page = static_cast<const IT*>(c.tables)[b * c.table_stride + j];
-      if (page >= 0 && page < c.num_blocks) slot = page * c.block_size + (pos - j * c.block_size);
+  for (int64_t b = blockIdx.x; b < c.batch; b += gridDim.x) {
+    const ExtendRow<IT> r(c, b);
+    const int64_t grow = fits ? r.grow : 0;
+    const int64_t first = a.a[b] >> 1;
+    const int copy = static_cast<int>(a.a[b] & 1);
+    __syncthreads();  // every wave has read the row
+    IT* row = static_cast<IT*>(c.tables) + b * c.table_stride;
+    if (grow > 0) {
+      if (threadIdx.x == 0) {
+        if (copy) {
+          const int64_t page = a.list[first];
+          add_ref(refs, r.last, -1);
+          refs[page] = 1;
+          row[r.had - 1] = static_cast<IT>(page);
+        }
+        lens[b] = static_cast<IT>(r.len + grow);
+      }
+      for (int64_t j = r.had + threadIdx.x; j < r.has; j += kBlockThreads) {
+        const int64_t page = a.list[first + copy + j - r.had];
+        refs[page] = 1;
+        row[j] = static_cast<IT>(page);
+      }
     }
-    c.slots[i] = slot;
+    for (int64_t k = threadIdx.x; k < c.max_new; k += kBlockThreads) {
+      int64_t slot = -1;
+      if (k < grow) {
+        const int64_t pos = r.len + k, j = pos / c.block_size;
+        const int64_t page = j >= r.had ? a.list[first + copy + j - r.had] : copy ? a.list[first] : r.open ? r.last : -1;
+        if (page >= 0) slot = page * c.block_size + (pos - j * c.block_size);
+      }
+      c.slots[b * c.max_new + k] = slot;
+    }
   }
   move_pages<VEC>(a);
 }
@@ -421,8 +432,7 @@ PagesArgs lay_out(const musa_aiter_hip_pages_call& c, PagesKind kind) {
     a.src = p;
     a.dst = a.src + c.batch;
     a.a = a.dst + c.batch;
-    a.b = a.a + c.batch;
-    a.list = a.b + c.batch;
+    a.list = a.a + c.batch;
   } else {
     a.src = p;
     a.dst = a.src + c.num_blocks;
@@ -448,7 +458,7 @@ hipError_t launch_typed(const musa_aiter_hip_pages_call& c, PagesKind kind, hipS
   const bool wide_copy = copy_width(c) == 16;
   if (kind == kPagesExtend) {
     hipLaunchKernelGGL(HIP_KERNEL_NAME(pages_extend_kernel<IT>), dim3(1), dim3(kScanThreads), 0, stream, a);
-    const dim3 grid(finish_groups(c, c.batch, c.batch * c.max_new));
+    const dim3 grid(finish_groups(c, c.batch, c.batch));
     if (wide_copy)
       hipLaunchKernelGGL(HIP_KERNEL_NAME(pages_extend_finish_kernel<IT, 16>), grid, threads, 0, stream, a);
     else
@@ -469,7 +479,7 @@ hipError_t launch_typed(const musa_aiter_hip_pages_call& c, PagesKind kind, hipS
 int64_t pages_workspace(const musa_aiter_hip_pages_call& c, PagesKind kind) {
   int64_t words = kHeaderWords;
   if (kind == kPagesFork) words += c.batch + (c.batch * c.max_blocks * (c.wide ? 8 : 4) + 7) / 8;
-  else if (kind == kPagesExtend) words += 4 * c.batch + c.num_blocks;
+  else if (kind == kPagesExtend) words += 3 * c.batch + c.num_blocks;
   else if (kind == kPagesCompact) words += 3 * c.num_blocks;
   else return 0;
   return 8 * words;
