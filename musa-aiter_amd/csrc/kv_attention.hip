@@ -142,6 +142,9 @@ __global__ __launch_bounds__(kBlockThreads) void attention_any_kernel(const Attn
 // two bf16 summands, 11 + 11 in two fp16 summands where the output is fp16 and one rounding would show).
 // The value scale of a block enters the running maximum, m = max(s_j + log2 vs_j), so that the weights fit fp16
 // whatever the scales are; l = sum 2^(s_j - m) needs no such care in fp32.
+// Memory bounds long decode steps: 64 rows of 256 to 8192 tokens (32 heads, 8 kv heads, 128 dims) 114 us, 4.95 TB/s
+// (a large copy 4.7), one row of 131072 tokens 106 us.  Short ones are a chain of dependent loads: 8 rows of up to 500
+// tokens 11 us.
 // Query rows as B operands, in LDS (in registers they would cost every wave 16 for 128 dims and a third wave per
 // SIMD its place): element j of step s of lane (x, g) is d = 32 s + 4 j + g of row x.
 template <int HDP, int NT, int CODEC, int DT>
@@ -605,7 +608,7 @@ void attention_rows_kernel(const RowsArgs a) {
 }
 
 // The even cut of a decode step.  Sequences differ in length, so equal parts of each leave most of the chip waiting
-// for the longest (64 sequences of 256 to 8192 tokens: 3.8 TB/s, against 5.1 TB/s where all are equally long).
+// for the longest (64 sequences of 256 to 8192 tokens: 143 us in one part each).
 // Here a unit is 256 tokens (a turn of a workgroup's four waves) of a line, one (sequence, row tile, kv head); the lines
 // of all sequences stand one behind another, and workgroup i of n takes units [i * all / n, (i + 1) * all / n).
 // Only its first line may have begun, and only its last one may go on, in another workgroup: their parts are 2 i
@@ -844,9 +847,10 @@ hipError_t launch_any(const AttnCall& c, hipStream_t stream) {
 }
 
 // Whether the matrix-core form takes the call: 16-bit queries, up to 256 dims, 16-token groups that lie in one
-// block and begin at multiples of 16 bytes.
+// block and begin at multiples of 16 bytes, places in a block and head that 32 bits hold.
 bool takes_rows(const AttnCall& c) {
-  if (c.dtype == kLinF32 || c.head_dim > 256 || c.block_size % 16 != 0) return false;
+  if (c.dtype == kLinF32 || c.head_dim > 256 || c.block_size % 16 != 0 || c.head_dim * c.block_size >= 1 << 30)
+    return false;
   uint64_t all = 0;
   for (int kv = 0; kv < 2; ++kv)
     all |= reinterpret_cast<uint64_t>(c.cache[kv]) | static_cast<uint64_t>(c.cache_block_stride[kv]);
@@ -882,13 +886,18 @@ struct FlowPlan {
   int64_t groups, slot_rows;
 };
 
+// Workgroups of the rows and flow kernels that a CU holds.
+int held_by_a_unit(const AttnCall& c) {
+  const int hdp = c.head_dim <= 64 ? 64 : c.head_dim == 96 ? 96 : c.head_dim <= 128 ? 128 : 256;
+  return rows_occupancy(hdp, c.head_dim == hdp, row_tiles(c), c.codec);
+}
+
 FlowPlan flow_plan(const AttnCall& c) {
   const int tiles = row_tiles(c), size = 16 * tiles;
-  const int hdp = c.head_dim <= 64 ? 64 : c.head_dim == 96 ? 96 : c.head_dim <= 128 ? 128 : 256;
   const int64_t lines = tiles_bound(c, size) * c.kv_heads, group = c.heads / c.kv_heads;
   const int64_t turns = (c.max_blocks * c.block_size + kUnitTokens - 1) / kUnitTokens;
   const int64_t most = lines * (turns > 0 ? turns : 1);
-  const int64_t held = kComputeUnits * rows_occupancy(hdp, c.head_dim == hdp, tiles, c.codec);
+  const int64_t held = kComputeUnits * held_by_a_unit(c);
   return {most < held ? most : held, group < size ? group : size};
 }
 
@@ -957,16 +966,26 @@ bool attention_flows(const AttnCall& c) {
          c.batch < (int64_t{1} << 31) / turns / (c.kv_heads + c.heads);
 }
 
-// How a call is cut.  Decode steps of more than 512 tokens: evenly (0).  Others: enough parts for four workgroups
-// per CU, none below 256 tokens (a turn of a workgroup's four waves); prompt chunks' tiles, of which a CU holds two, are
-// cut only where they would leave some without any.
+// How a call is cut.  Decode steps of sequences longer than kFlowFrom: evenly (0).  An even cut costs its join and its
+// search and gains where lengths differ: 64 rows of 64 to 8192 tokens 117 us, by parts 134; of 64 to 4000 62 against 64;
+// of 64 to 2000 43 against 38; and where all are equally long, 4096, 116 against 103.
+// Others: as many parts as give the chip's CUs two workgroups each, or one where a CU holds no more, in whole turns of
+// 256 tokens (8 rows of 1000 tokens: 12.9 us in four parts, 16.1 in one; 64 rows: 26.5 in one, 33 in two; 32 x 32
+// rows, one workgroup a CU: 42 in one, 58 in two).  Up to 512 tokens: one (8 rows of 500: 11.0 us, in two parts 12.6).
+constexpr int64_t kFlowFrom = 4096;
+
 int64_t attention_splits(const AttnCall& c, int64_t longest) {
-  if (attention_flows(c) && longest > 512) return 0;
-  const int64_t groups = takes_wide(c)   ? tiles_bound(c, kWideRows) * c.kv_heads
-                         : takes_rows(c) ? tiles_bound(c, 16 * row_tiles(c)) * c.kv_heads
-                                         : c.rows * c.heads;
-  int64_t splits = groups <= 0 ? 1 : takes_wide(c) ? 512 / groups : (1024 + groups - 1) / groups;
-  const int64_t most = longest / 256;
+  if (attention_flows(c) && longest > kFlowFrom) return 0;
+  int64_t groups = c.rows * c.heads, wanted = 4 * kComputeUnits;
+  if (takes_wide(c)) {
+    groups = tiles_bound(c, kWideRows) * c.kv_heads;
+    wanted = 2 * kComputeUnits;
+  } else if (takes_rows(c)) {
+    groups = tiles_bound(c, 16 * row_tiles(c)) * c.kv_heads;
+    wanted = kComputeUnits * (held_by_a_unit(c) > 1 ? 2 : 1);
+  }
+  const int64_t most = longest <= 2 * kTurnTokens ? 1 : (longest - 1) / kTurnTokens + 1;
+  int64_t splits = groups > 0 ? wanted / groups : 1;
   splits = splits < most ? splits : most;
   return splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : splits;
 }

@@ -147,7 +147,8 @@ def test_chunks_captured_and_replayed():
 def test_even_cut(hd, fmt, dtype, window, heads):
     lens = [0, 1, 2500, 64, 0, 513, 0]
     case = Case(lens=lens, heads=heads, kv_heads=1, hd=hd, fmt=fmt, dtype=dtype, window=window, seed=hd, index=torch.int64)
-    case.check(*_go(case))
+    case.check(*_go(case, max_seq_len=1 << 20))  # a hint: decode steps of long sequences are cut evenly
+    case.check(*_go(case, max_seq_len=2500))
 
 
 @pytest.mark.parametrize("batch,longest", [(1, 9000), (70, 700), (200, 530)])
@@ -156,6 +157,7 @@ def test_even_cut_of_few_and_many_sequences(batch, longest):
     lens = rng.integers(0, longest, size=batch)
     lens[-1] = longest
     case = Case(lens=lens, heads=8, kv_heads=4, hd=64, seed=batch)
+    case.check(*_go(case, max_seq_len=1 << 20))
     case.check(*_go(case))
 
 
@@ -193,3 +195,27 @@ def test_places_past_32_bits():
         torch.cuda.synchronize()
         assert torch.equal(got, want)
         del big, c
+
+
+def test_even_cut_captured_and_replayed_on_two_streams():
+    case = Case(lens=[700, 1300, 20, 0, 5000], heads=8, kv_heads=2, hd=128, seed=19)
+    args, kw = case.args()
+    musa_aiter.kv_paged_attention_fp8(*args, **kw)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(musa_aiter.kv_paged_attention_fp8(*args, **kw, return_lse=True))
+        graphs.append(graph)
+    for rep in range(3):
+        args[0].copy_(torch.randn(args[0].shape))
+        args[4].copy_(torch.from_numpy(np.maximum(case.lens - 31 * rep, 0)))
+        torch.cuda.synchronize()
+        for graph in graphs:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                graph.replay()
+        torch.cuda.synchronize()
+        want = musa_aiter.kv_paged_attention_fp8(*args, **kw, return_lse=True)
+        for got in outs:
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), rep
