@@ -870,14 +870,12 @@ constexpr int64_t kComputeUnits = 256;
 
 // Whether prompt chunks' form (kv_attention_wide.hip) takes the call.  It decodes a token tile once for 128 rows, the
 // other form for every 16 or 32, but goes through the tokens of a part one tile at a time where the other one's waves
-// take four at once.  Rows are those of a kv head and sequence, on average: past 64 it wins (8 x 68 rows against 4096
-// tokens: 67 us, the other form 96), from 33 on where its tiles fill the chip's 256 CUs (32 x 36 rows against 2000
-// tokens, 328 tiles: 72 against 109 us; 24 x 36 rows against ~1500, 62 tiles: 26 against 20), below not (32 x 32 rows:
-// 71 against 65).
+// take four at once.  Rows are those of a kv head and sequence, on average: 32 x 96 rows against 2000 tokens 80 us, the
+// other form 118, 8 x 128 against 4096 tokens 60 against 70, 8 x 68: 67 both; 32 x 36 rows 73 against 77, but with 64
+// dims (64 x 40 rows) 84 against 65.
 bool takes_wide(const AttnCall& c) {
-  if (!takes_rows(c) || c.starts == nullptr || c.head_dim > 128 || c.batch < 1) return false;
-  const int64_t rows = (c.rows + c.batch - 1) / c.batch * (c.heads / c.kv_heads);
-  return rows > 64 || (rows > 32 && tiles_bound(c, kWideRows) * c.kv_heads >= kComputeUnits);
+  return takes_rows(c) && c.starts != nullptr && c.head_dim <= 128 && c.batch > 0 &&
+         (c.rows + c.batch - 1) / c.batch * (c.heads / c.kv_heads) > 64;
 }
 
 // How an even cut is made: workgroups (what the chip holds at once, or one for each unit that the tables have room
