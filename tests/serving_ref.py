@@ -1,5 +1,5 @@
 """Plain 64-bit implementations of the block-scaled FP8 store, the attention over such a cache and the page
-bookkeeping, one element or one step at a time on the CPU.  Checkers, not product code."""
+bookkeeping, one element or one step at a time on the CPU.  Oracles, not product code."""
 
 from __future__ import annotations
 
