@@ -274,15 +274,33 @@ __device__ __forceinline__ RowTile find_tile(const RowsArgs& a, int32_t index, i
   return {-1, 0, 0, 0};
 }
 
-// Zeroes this worker's share of the rows that belong to no sequence.
+// Zeroes heads [head, head + heads) of this workgroup's share of the rows that belong to no sequence.  Its waves look at
+// 64 rows together, at the sequences that have some of them (one row after the other took 45 us for 3800 rows in 21
+// tiles), and take turns at the rows that are left.
 template <int DT>
-__device__ __forceinline__ void fill_loose_rows(const AttnCall& c, int64_t worker, int64_t workers) {
-  for (int64_t t = worker; t < c.rows; t += workers) {
-    if (row_sequence(c, t).seq >= 0) continue;
-    for (int64_t d = threadIdx.x; d < c.heads * c.head_dim; d += kBlockThreads)
-      store_o<DT>(c.out, t * c.heads * c.head_dim + d, 0.0f);
-    if (c.lse != nullptr)
-      for (int64_t h = threadIdx.x; h < c.heads; h += kBlockThreads) c.lse[t * c.heads + h] = -__builtin_inff();
+__device__ __forceinline__ void fill_loose_rows(const AttnCall& c, int64_t worker, int64_t workers, int64_t head,
+                                                int64_t heads) {
+  const int lane = lane_id();
+  for (int64_t t0 = worker * kWave; t0 < c.rows; t0 += workers * kWave) {
+    bool owned = t0 + lane >= c.rows;
+    for (int64_t b0 = 0; b0 < c.batch; b0 += kWave) {
+      SeqRows r{0, 0};
+      if (b0 + lane < c.batch) r = seq_rows(c, b0 + lane);
+      uint64_t some = ballot(r.count > 0 && r.first < t0 + kWave && r.first + r.count > t0);
+      for (; some != 0; some &= some - 1) {
+        const int src = __builtin_ctzll(some);
+        const int64_t first = readlane64(r.first, src), count = readlane64(r.count, src);
+        owned |= t0 + lane >= first && t0 + lane < first + count;
+      }
+    }
+    int turn = 0;
+    for (uint64_t loose = ballot(!owned); loose != 0; loose &= loose - 1, ++turn) {
+      if (turn % kWavesPerBlock != wave_in_block()) continue;
+      const int64_t at = (t0 + __builtin_ctzll(loose)) * c.heads + head;
+      for (int64_t d = lane; d < heads * c.head_dim; d += kWave) store_o<DT>(c.out, at * c.head_dim + d, 0.0f);
+      if (c.lse != nullptr)
+        for (int64_t h = lane; h < heads; h += kWave) c.lse[at + h] = -__builtin_inff();
+    }
   }
 }
 

@@ -588,7 +588,8 @@ void attention_rows_kernel(const RowsArgs a) {
   __shared__ RowsShared<HDP, NT, CODEC, DT> shared;
   const int32_t head = blockIdx.y, split = blockIdx.z;
   const RowTile tile = find_tile(a, blockIdx.x, 16 * NT);
-  if (c.starts != nullptr && c.fill_rows && head == 0 && split == 0) fill_loose_rows<DT>(c, blockIdx.x, gridDim.x);
+  if (c.starts != nullptr && c.fill_rows && split == 0)
+    fill_loose_rows<DT>(c, blockIdx.x, gridDim.x, head * a.group, a.group);
   if (tile.seq < 0) return;
   const Reach reach = tile_reach(a, tile, 16 * NT);
   const Span span = part_span(reach.begin, reach.end, split, a.splits);

@@ -195,12 +195,13 @@ void attention_wide_kernel(const RowsArgs a, uint32_t tiles) {
   const uint32_t at = blockIdx.x / kv_heads;
   const int32_t head = static_cast<int32_t>(blockIdx.x - at * kv_heads), split = static_cast<int32_t>(at % a.splits);
   const int32_t index = static_cast<int32_t>(tiles - 1 - at / a.splits);
+  const int32_t group = a.group;
   const RowTile tile = find_tile(a, index, kWideRows);
-  if (c.starts != nullptr && c.fill_rows && head == 0 && split == 0) fill_loose_rows<DT>(c, index, tiles);
+  if (c.starts != nullptr && c.fill_rows && split == 0) fill_loose_rows<DT>(c, index, tiles, head * group, group);
   if (tile.seq < 0) return;
   const Reach reach = tile_reach(a, tile, kWideRows);
   const Span span = part_span(reach.begin, reach.end, split, a.splits);
-  const int32_t group = a.group, in_seq = tile.count * group;
+  const int32_t in_seq = tile.count * group;
   const int lane = lane_id(), x = lane & 31, h = lane >> 5, wave = wave_in_block();
   const uint8_t* table = static_cast<const uint8_t*>(c.tables) + tile.seq * c.table_stride * (c.wide_tables ? 8 : 4);
 
