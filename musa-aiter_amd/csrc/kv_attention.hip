@@ -872,7 +872,7 @@ constexpr int64_t kComputeUnits = 256;
 // Whether prompt chunks' form (kv_attention_wide.hip) takes the call.  It decodes a token tile once for 128 rows, the
 // other form for every 16 or 32, but goes through the tokens of a part one tile at a time where the other one's waves
 // take four at once.  Rows are those of a kv head and sequence, on average: 32 x 96 rows against 2000 tokens 80 us, the
-// other form 118, 8 x 128 against 4096 tokens 60 against 70, 8 x 68: 67 both; 32 x 36 rows 73 against 77, but with 64
+// other form 118, 8 x 128 against 4096 tokens 60 against 70, 8 x 68: 48 against 67; 32 x 36 rows 73 against 77, but with 64
 // dims (64 x 40 rows) 84 against 65.
 bool takes_wide(const AttnCall& c) {
   return takes_rows(c) && c.starts != nullptr && c.head_dim <= 128 && c.batch > 0 &&
@@ -970,7 +970,9 @@ bool attention_flows(const AttnCall& c) {
 // of 64 to 2000 43 against 38; and where all are equally long, 4096, 116 against 103.
 // Others: as many parts as give the chip's CUs two workgroups each, or one where a CU holds no more, in whole turns of
 // 256 tokens (8 rows of 1000 tokens: 12.9 us in four parts, 16.1 in one; 64 rows: 26.5 in one, 33 in two; 32 x 32
-// rows, one workgroup a CU: 42 in one, 58 in two).  Up to 512 tokens: one (8 rows of 500: 11.0 us, in two parts 12.6).
+// rows, one workgroup a CU: 42 in one, 58 in two).  Up to 512 tokens: one (8 rows of 500: 11.0 us, in two parts 12.6);
+// prompt chunks, whose many rows make parts dear, up to 1024 (1000 rows of 4 heads against 1000 tokens: 40 us, in two
+// parts 54; 64 rows against 2000: 66, in eight 24).
 constexpr int64_t kFlowFrom = 4096;
 
 int64_t attention_splits(const AttnCall& c, int64_t longest) {
@@ -983,10 +985,13 @@ int64_t attention_splits(const AttnCall& c, int64_t longest) {
     groups = tiles_bound(c, 16 * row_tiles(c)) * c.kv_heads;
     wanted = kComputeUnits * (held_by_a_unit(c) > 1 ? 2 : 1);
   }
-  const int64_t most = longest <= 2 * kTurnTokens ? 1 : (longest - 1) / kTurnTokens + 1;
+  const int64_t whole = takes_wide(c) ? 4 * kTurnTokens : 2 * kTurnTokens;
+  const int64_t most = longest <= whole ? 1 : (longest - 1) / kTurnTokens + 1;
   int64_t splits = groups > 0 ? wanted / groups : 1;
   splits = splits < most ? splits : most;
-  return splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : splits;
+  splits = splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : splits;
+  const int64_t per = (most + splits - 1) / splits;
+  return (most + per - 1) / per;  // none that would be left without a turn
 }
 
 int64_t attention_workspace(const AttnCall& c) {
