@@ -274,9 +274,13 @@ __device__ __forceinline__ RowTile find_tile(const RowsArgs& a, int32_t index, i
   return {-1, 0, 0, 0};
 }
 
-// Zeroes heads [head, head + heads) of this workgroup's share of the rows that belong to no sequence.  Its waves look at
-// 64 rows together, at the sequences that have some of them (one row after the other took 45 us for 3800 rows in 21
-// tiles), and take turns at the rows that are left.
+// Whether rows that belong to no sequence are written: their outputs with fill_rows, their logarithms in every case (they
+// are -inf, whoever brought the output).
+__device__ __forceinline__ bool writes_loose_rows(const AttnCall& c) { return c.fill_rows || c.lse != nullptr; }
+
+// Writes heads [head, head + heads) of this workgroup's share of those rows.  Its waves look at 64 rows together, at the
+// sequences that have some of them (one row after the other took 45 us for 3800 rows in 21 tiles), and take turns at the
+// rows that are left.
 template <int DT>
 __device__ __forceinline__ void fill_loose_rows(const AttnCall& c, int64_t worker, int64_t workers, int64_t head,
                                                 int64_t heads) {
@@ -297,7 +301,8 @@ __device__ __forceinline__ void fill_loose_rows(const AttnCall& c, int64_t worke
     for (uint64_t loose = ballot(!owned); loose != 0; loose &= loose - 1, ++turn) {
       if (turn % kWavesPerBlock != wave_in_block()) continue;
       const int64_t at = (t0 + __builtin_ctzll(loose)) * c.heads + head;
-      for (int64_t d = lane; d < heads * c.head_dim; d += kWave) store_o<DT>(c.out, at * c.head_dim + d, 0.0f);
+      if (c.fill_rows)
+        for (int64_t d = lane; d < heads * c.head_dim; d += kWave) store_o<DT>(c.out, at * c.head_dim + d, 0.0f);
       if (c.lse != nullptr)
         for (int64_t h = lane; h < heads; h += kWave) c.lse[at + h] = -__builtin_inff();
     }

@@ -31,8 +31,9 @@ __global__ __launch_bounds__(kBlockThreads) void attention_any_kernel(const Attn
   const RowSeq row = row_sequence(c, t);
   const int64_t seq = row.seq;
   if (seq < 0) {
-    if (!c.fill_rows || split != 0) return;
-    for (int64_t d = threadIdx.x; d < c.head_dim; d += kBlockThreads) store_o<DT>(c.out, rh * c.head_dim + d, 0.0f);
+    if (split != 0) return;
+    if (c.fill_rows)
+      for (int64_t d = threadIdx.x; d < c.head_dim; d += kBlockThreads) store_o<DT>(c.out, rh * c.head_dim + d, 0.0f);
     if (c.lse != nullptr && threadIdx.x == 0) c.lse[rh] = -__builtin_inff();
     return;
   }
@@ -588,7 +589,7 @@ void attention_rows_kernel(const RowsArgs a) {
   __shared__ RowsShared<HDP, NT, CODEC, DT> shared;
   const int32_t head = blockIdx.y, split = blockIdx.z;
   const RowTile tile = find_tile(a, blockIdx.x, 16 * NT);
-  if (c.starts != nullptr && c.fill_rows && split == 0)
+  if (c.starts != nullptr && writes_loose_rows(c) && split == 0)
     fill_loose_rows<DT>(c, blockIdx.x, gridDim.x, head * a.group, a.group);
   if (tile.seq < 0) return;
   const Reach reach = tile_reach(a, tile, 16 * NT);

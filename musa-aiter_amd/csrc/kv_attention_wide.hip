@@ -197,7 +197,8 @@ void attention_wide_kernel(const RowsArgs a, uint32_t tiles) {
   const int32_t index = static_cast<int32_t>(tiles - 1 - at / a.splits);
   const int32_t group = a.group;
   const RowTile tile = find_tile(a, index, kWideRows);
-  if (c.starts != nullptr && c.fill_rows && split == 0) fill_loose_rows<DT>(c, index, tiles, head * group, group);
+  if (c.starts != nullptr && writes_loose_rows(c) && split == 0)
+    fill_loose_rows<DT>(c, index, tiles, head * group, group);
   if (tile.seq < 0) return;
   const Reach reach = tile_reach(a, tile, kWideRows);
   const Span span = part_span(reach.begin, reach.end, split, a.splits);
