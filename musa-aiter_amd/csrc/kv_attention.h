@@ -328,13 +328,23 @@ __device__ __forceinline__ uint32_t load4(const uint8_t* p) {
 // the codes that were asked for before it.
 struct Entry {
   uint32_t lo, hi;
-  bool inside;  // the group begins in front of `end`
+  bool inside;  // the group has tokens that are seen, or are only masked next to some
 };
 
 __device__ __forceinline__ Entry load_entry(const RowsArgs& a, const uint8_t* row, int32_t token, int32_t end) {
   const uint32_t column = group_column(a, min(token, end - 1));
   const uint8_t* p = row + static_cast<uint64_t>(column) * (a.c.wide_tables ? 8 : 4);
   return {load4(p), load4(p + (a.c.wide_tables ? 4 : 0)), token < end};
+}
+
+// The same in the first tile of a part, which is rounded down to whole tiles: groups that end at or in front of `begin`,
+// where the window of the first row does, are not taken.  Their pages may be anybody's by then, and a scale that is no
+// number there would go through its weight of zero into the sums.
+__device__ __forceinline__ Entry load_first_entry(const RowsArgs& a, const uint8_t* row, int32_t token, int32_t begin,
+                                                  int32_t end) {
+  Entry e = load_entry(a, row, token, end);
+  e.inside = e.inside && token + 16 > begin;
+  return e;
 }
 
 // Its block, or -1.

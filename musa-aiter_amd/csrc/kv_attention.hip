@@ -206,6 +206,13 @@ __device__ __forceinline__ GroupEntries load_entries(const RowsArgs& a, const ui
   return {load_entry(a, row, token + 16 * (x >> 2), end), load_entry(a, row, token + 16 * g, end)};
 }
 
+__device__ __forceinline__ GroupEntries load_first_entries(const RowsArgs& a, const uint8_t* row, int32_t token,
+                                                           int32_t begin, int32_t end) {
+  const int lane = lane_now(), x = lane & 15, g = lane >> 4;
+  return {load_first_entry(a, row, token + 16 * (x >> 2), begin, end),
+          load_first_entry(a, row, token + 16 * g, begin, end)};
+}
+
 __device__ __forceinline__ GroupIds group_ids(const RowsArgs& a, const GroupEntries& e) {
   return {entry_block(a, e.k), entry_block(a, e.v)};
 }
@@ -452,7 +459,7 @@ __device__ __forceinline__ void run_segment(const RowsArgs& a, const Segment& se
   GroupEntries next_entries;
   GroupScales scales;
   if (token < last) {  // on their way while the queries are read
-    const GroupEntries entries = load_entries(a, row, token, last);
+    const GroupEntries entries = load_first_entries(a, row, token, reach.begin, last);
     next_entries = load_entries(a, row, token + kStep, last);
     ids = group_ids(a, entries);
     scales = load_scales(c, head, ids);

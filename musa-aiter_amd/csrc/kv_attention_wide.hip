@@ -215,7 +215,7 @@ void attention_wide_kernel(const RowsArgs a, uint32_t tiles) {
   GroupCodes<HDP> codes;
   Entry next_entry;
   if (token < last) {
-    const Entry entry = load_entry(a, table, token + mine_at, last);
+    const Entry entry = load_first_entry(a, table, token + mine_at, reach.begin, last);
     next_entry = load_entry(a, table, token + kTileTokens + mine_at, last);
     load_group<HDP, EXACT>(a, head, token + mine_at, __builtin_amdgcn_readfirstlane(entry_block(a, entry)), codes);
   }

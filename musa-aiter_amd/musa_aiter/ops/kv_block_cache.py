@@ -201,8 +201,9 @@ def kv_paged_attention_fp8(
     Tables, lengths and row starts (any integer type) are read on the device only: nothing is synchronised.  A
     position without a table entry, or whose entry lies outside the cache, is not seen.  A row that sees nothing
     gives zeros (``lse`` -inf).  Rows of ``query`` that belong to no sequence (a padded batch) are left as they
-    are in ``out``, and are zeros in a new tensor; their ``lse`` is -inf either way.  Scales are 0 (a block of zeros) or lie in [2**-60, 2**60], and
-    may be expanded, e.g. ``per_head.expand(blocks, kv_heads)``.  Codes decode as in kv_paged_fp8_to_linear.
+    are in ``out``, and are zeros in a new tensor; their ``lse`` is -inf either way.  Scales of blocks that a call's
+    rows see are 0 (a block of zeros) or lie in [2**-60, 2**60]; scales may be expanded, e.g.
+    ``per_head.expand(blocks, kv_heads)``.  Codes decode as in kv_paged_fp8_to_linear.
 
     ``max_seq_len``, an upper bound of ``seq_lens`` that the caller knows, only decides how the work is cut;
     by default it is what ``block_tables`` has room for.  Returns the output, in ``query``'s type, and with
