@@ -99,7 +99,8 @@ typedef struct musa_aiter_hip_pages_call {
   void* refs;
   const void* rows;     /* per row: parents (fork), tokens kept (free), new tokens (extend) */
   int64_t* slots;       /* extend: [batch, max_new] */
-  int64_t* result;      /* extend: free pages left, -(pages missing), or -2^62 (a row outgrows its table);
+  int64_t* result;      /* extend: free pages left, -(pages missing), or -2^62 (a row outgrows its table
+                           or the type of lens);
                            compact: pages in use */
   void* workspace;
   int64_t workspace_bytes;

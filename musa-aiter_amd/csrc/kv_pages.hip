@@ -137,6 +137,9 @@ __global__ __launch_bounds__(kBlockThreads) void pages_fork_kernel(const PagesAr
 // A page that r owners share is copied by all the rows that grow into it but the last, and by all of them if
 // somebody else owns it too: row b copies iff fewer than r - 1 rows before it grow into the same page.
 template <typename IT>
+constexpr int64_t kMostTokens = sizeof(IT) == 8 ? INT64_MAX : INT32_MAX;  // that a row's length can say
+
+template <typename IT>
 struct ExtendRow {
   int64_t len, grow, had, has, last;
   bool open;  // grows into a partial last page
@@ -176,7 +179,7 @@ __global__ __launch_bounds__(kScanThreads) void pages_extend_kernel(const PagesA
     __syncthreads();
     if (b < c.batch) {
       const ExtendRow<IT> r(c, b);
-      if (r.has > c.max_blocks) too_long = 1;
+      if (r.has > c.max_blocks || r.len + r.grow > kMostTokens<IT>) too_long = 1;
       need = r.has - r.had;
       if (r.open) {
         last = static_cast<int32_t>(r.last);

@@ -119,7 +119,7 @@ def kv_extend_paged_sequences(
     Returns ``(slots, pages_left)``: int64 ``[batch, max_new]`` slots of the new tokens, -1 past ``new_lens[b]``
     (``slots.view(-1)`` is a slot_mapping), and an int64 scalar: the pages still free, or, if it is negative, that
     nothing was done and all slots are -1, since so many pages were missing (-2**62: since a row of
-    ``block_tables`` is too short).
+    ``block_tables`` is too short, or int32 ``seq_lens`` for its length).
     """
     op = "kv_extend_paged_sequences"
     if type(max_new) is int and max_new >= 0:
