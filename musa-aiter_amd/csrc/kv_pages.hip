@@ -43,7 +43,8 @@ __device__ __forceinline__ int64_t row_value(const musa_aiter_hip_pages_call& c,
   return c.wide_rows ? static_cast<const int64_t*>(c.rows)[b] : static_cast<const int32_t*>(c.rows)[b];
 }
 
-__device__ __forceinline__ int64_t pages_of(int64_t len, int64_t bs) { return len <= 0 ? 0 : (len + bs - 1) / bs; }
+// (In this form no length, however wrong, runs past int64.)
+__device__ __forceinline__ int64_t pages_of(int64_t len, int64_t bs) { return len <= 0 ? 0 : (len - 1) / bs + 1; }
 
 // Entries of a row that its length covers (a length past the row's end owns the whole row).
 __device__ __forceinline__ int64_t owned_of(const musa_aiter_hip_pages_call& c, int64_t len) {
@@ -146,7 +147,7 @@ struct ExtendRow {
 
   __device__ ExtendRow(const musa_aiter_hip_pages_call& c, int64_t b) {
     len = static_cast<const IT*>(c.lens)[b];
-    len = len < 0 ? 0 : len;
+    len = len < 0 ? 0 : len > INT64_MAX / 2 ? INT64_MAX / 2 : len;  // such a row outgrows every table
     grow = row_value(c, b);
     grow = grow < 0 ? 0 : grow > c.max_new ? c.max_new : grow;
     had = pages_of(len, c.block_size);
