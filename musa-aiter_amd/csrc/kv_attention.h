@@ -232,6 +232,18 @@ struct RowsArgs {
   int32_t slot_rows;  // even cut: rows of a part
 };
 
+// The reference m that weights are taken relative to is max(score + log2(value scale)), so that weight * value scale fits
+// 16 bits.  A score past kLiftedScores (in base 2) is too coarse for that sum: rounded, it may lie so far below that the
+// weights overflow (half a step of 2^26 is 4, a factor of 16).  There m is the score itself, the weights are at most one,
+// and value scales up to 4 fit.  For the same reason its product with the scales is rounded before m is taken off:
+// unrounded, it may pass m by half a step.
+constexpr float kLiftedScores = 0x1p22f;
+
+__device__ __forceinline__ float score_lift(float score, float value_scale) {
+  const float lift = __builtin_amdgcn_fmed3f(__builtin_amdgcn_logf(value_scale), -100.0f, 100.0f);
+  return fabsf(score) > kLiftedScores ? 0.0f : lift;
+}
+
 constexpr int32_t kMostRoom = 1 << 29;
 // Lengths past it see what a row of kMostRoom positions would show them.
 constexpr int32_t kMostLen = 3 << 29;

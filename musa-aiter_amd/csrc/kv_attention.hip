@@ -142,7 +142,7 @@ __global__ __launch_bounds__(kBlockThreads) void attention_any_kernel(const Attn
 // summands of bf16 hold an fp16 query).  Probabilities times value scale are rounded to 11 bits (8 + 8 bits in
 // two bf16 summands, 11 + 11 in two fp16 summands where the output is fp16 and one rounding would show).
 // The value scale of a block enters the running maximum, m = max(s_j + log2 vs_j), so that the weights fit fp16
-// whatever the scales are; l = sum 2^(s_j - m) needs no such care in fp32.
+// whatever the scales are (see score_lift); l = sum 2^(s_j - m) needs no such care in fp32.
 // Memory bounds long decode steps: 64 rows of 256 to 8192 tokens (32 heads, 8 kv heads, 128 dims) 114 us, 4.95 TB/s
 // (a large copy 4.7), one row of 131072 tokens 106 us.  Short ones are a chain of dependent loads: 8 rows of up to 500
 // tokens 11 us.
@@ -336,8 +336,7 @@ __device__ __forceinline__ void soften(f32x4* score, float factor, const GroupSc
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) most = fmaxf(most, score[i][r]);
-  const float lift = __builtin_amdgcn_fmed3f(__builtin_amdgcn_logf(vs), -100.0f, 100.0f);
-  const float top = fmaxf(s.m, groups_max(most + lift));
+  const float top = fmaxf(s.m, groups_max(most + score_lift(most, vs)));
   const float ref = top == -__builtin_inff() ? 0.0f : top;
   if (ballot(top > s.m) != 0) {
     const float fade = __builtin_amdgcn_exp2f(s.m - ref);
