@@ -139,13 +139,14 @@ __global__ __launch_bounds__(kBlockThreads) void attention_any_kernel(const Attn
 // bits fall on fp16's fields; the all-ones code is the ordinary 480 * 2^-8), E5M2 as bf16 times 2^-112.  Codes of
 // exponent 0 are zeros: for fp16 a multiplication by one flushes them, with the mode register's fp16 denormals
 // off; for bf16 their bits are masked.  Query rows are scaled by a power of two so that 16 bits hold them (two
-// summands of bf16 hold an fp16 query).  Probabilities times value scale are rounded to 11 bits (8 + 8 bits in
+// summands of bf16 hold an fp16 query); next to E4M3 codes what is 2^-28 of a row's largest and less becomes zero there,
+// as the weights below it do.  Probabilities times value scale are rounded to 11 bits (8 + 8 bits in
 // two bf16 summands, 11 + 11 in two fp16 summands where the output is fp16 and one rounding would show).
 // The value scale of a block enters the running maximum, m = max(s_j + log2 vs_j), so that the weights fit fp16
 // whatever the scales are (see score_lift); l = sum 2^(s_j - m) needs no such care in fp32.
-// Memory bounds long decode steps: 64 rows of 256 to 8192 tokens (32 heads, 8 kv heads, 128 dims) 114 us, 4.95 TB/s
-// (a large copy 4.7), one row of 131072 tokens 106 us.  Short ones are a chain of dependent loads: 8 rows of up to 500
-// tokens 11 us.
+// Memory bounds long decode steps: 64 rows of 295 to 8192 tokens (254565 in all; 32 heads, 8 kv heads, 128 dims) 116 us,
+// 4.5 TB/s (a large copy 4.7), two rows of 131000 and 108683 tokens 106 us, 4.6 TB/s.  Short ones are a chain of dependent
+// loads: 4 rows of up to 500 tokens 11 us.
 // Query rows as B operands, in LDS (in registers they would cost every wave 16 for 128 dims and a third wave per
 // SIMD its place): element j of step s of lane (x, g) is d = 32 s + 4 j + g of row x.
 template <int HDP, int NT, int CODEC, int DT>

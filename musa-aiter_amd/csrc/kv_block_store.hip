@@ -19,8 +19,8 @@
 // every lane whole 16-column rows of two dims.  Other shapes go element by element.
 // What bounds it: few tokens, latency (a token's row, its block's scale, the stores); many, memory and the ten or so
 // operations that a value takes (E4M3, whose small quotients are more often there to be flushed, is the slower).
-// Measured: 64 tokens of 8 x 128 bf16 into pages of 16, 5.9 us; 30977 tokens, 52 us with the check of the slots
-// (3.6 TB/s; a large copy 4.7); 16 layers of 4001 tokens fp16 into pages of 64, 116 us (179 with the pieces read
+// Measured: 64 tokens of 8 x 128 bf16 into pages of 16, 5.2 us; 30977 tokens, 52 us with the check of the slots
+// (3.7 TB/s; a large copy 4.7); 16 layers of 4001 tokens fp16 into pages of 64, 116 us (179 with the pieces read
 // twice), of bf16 as E4M3 135 us.
 #include "kv_serving.h"
 

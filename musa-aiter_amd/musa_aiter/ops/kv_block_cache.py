@@ -208,7 +208,12 @@ def kv_paged_attention_fp8(
 
     ``max_seq_len``, an upper bound of ``seq_lens`` that the caller knows, only decides how the work is cut;
     by default it is what ``block_tables`` has room for.  Returns the output, in ``query``'s type, and with
-    ``return_lse`` also the float32 ``[T, heads]`` logarithms of the rows' softmax sums.
+    ``return_lse`` also the float32 ``[T, heads]`` logarithms of the rows' softmax sums.  There is no backward pass:
+    the output carries no gradient, also where ``query`` requires one.
+
+    Sums and softmax statistics are float32.  With float32 queries everything is; with 16-bit queries weights are
+    rounded to at least 11 bits, and weights (times value scale), and next to E4M3 codes query components, below 2**-28
+    of a row's largest may count as zero.
     """
     op = "kv_paged_attention_fp8"
     native = _NATIVE_FORMATS.get(fp8_format)
