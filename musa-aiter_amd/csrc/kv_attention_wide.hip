@@ -14,9 +14,9 @@
 // Chunks of 2048 and 1753 rows (32 heads, 8 kv heads, 128 dims; 3769 and 8192 cached tokens): 420 us, 770 TFLOP/s; 8192
 // rows against 16384 tokens: 1922 us, 860 TFLOP/s (a large library product of bf16 matrices: 1260).  The first dozen calls
 // after a pause take 530 us.  The instructions of a wave's tile (1024 cycles of matrix instructions, about 1900 of others, a
-// third of them exponentials) bound it; the two waves of a SIMD mostly take turns: 31% and 57% of its cycles.  Tried and slower or no faster: 256-row tiles of eight waves (6% faster for the
-// largest calls, 5 to 25% slower elsewhere), the next tile's score products among this tile's exponentials (their
-// registers leave one wave per SIMD: 800 us), wave priorities.
+// third of them exponentials) bound it; the two waves of a SIMD mostly take turns: 31% and 57% of its cycles.  Tried and
+// slower or no faster: 256-row tiles of eight waves (6% faster for the largest calls, 5 to 25% slower elsewhere), the next
+// tile's score products among this tile's exponentials (their registers leave one wave per SIMD: 800 us), wave priorities.
 #include "kv_attention.h"
 
 namespace kvhip {
