@@ -56,7 +56,7 @@ int musa_aiter_hip_block_store(const musa_aiter_hip_block_store_call* call, void
  * outside the cache are not seen; a row that sees nothing gives 0 and lse -inf.  Rows of no sequence are
  * zeroed in out with fill_rows, else left as they are there; their lse is -inf.  Scales of blocks that rows
  * see are 0 or lie in [2^-60, 2^60]; query values are at most 2^100 in size, and E4M3 value scales at most 4
- * where a row's scores pass 2^22.
+ * where a row's scores pass 2^24.
  * splits (1 to 64) parts of each sequence run side by side; 0 cuts the sequences of a decode step (starts NULL,
  * 16-bit queries, head_dim <= 256, blocks of multiples of 16 tokens at 16-byte addresses) into even shares of
  * the chip.  Unless splits is 1, `workspace` holds musa_aiter_hip_attention_workspace bytes. */

@@ -233,11 +233,10 @@ struct RowsArgs {
 };
 
 // The reference m that weights are taken relative to is max(score + log2(value scale)), so that weight * value scale fits
-// 16 bits.  A score past kLiftedScores (in base 2) is too coarse for that sum: rounded, it may lie so far below that the
-// weights overflow (half a step of 2^26 is 4, a factor of 16).  There m is the score itself, the weights are at most one,
-// and value scales up to 4 fit.  For the same reason its product with the scales is rounded before m is taken off:
-// unrounded, it may pass m by half a step.
-constexpr float kLiftedScores = 0x1p22f;
+// 16 bits.  Rounded to a score's steps that sum may lie half a step too low: below 2^25 (in base 2) by 1, a factor of 2 that
+// there is place for, from there on by 2 and more.  Past kLiftedScores m is therefore the score itself; the weights are at
+// most one then, and value scales up to 4 fit.
+constexpr float kLiftedScores = 0x1p25f;
 
 __device__ __forceinline__ float score_lift(float score, float value_scale) {
   const float lift = __builtin_amdgcn_fmed3f(__builtin_amdgcn_logf(value_scale), -100.0f, 100.0f);

@@ -29,6 +29,9 @@ constexpr int kTileTokens = 64;
 // The maximum that weights are taken relative to stays behind the running one by up to a factor of two, which their
 // 16 bits have place for: the sums so far are rescaled less often.
 constexpr float kLag = 1.0f;
+// A product with the scales that is not rounded may pass a maximum that is, by half a step of it.  Past kFusedScores
+// products are rounded first, and the maximum stays behind by nothing: m + 1 is no number among steps of 2.
+constexpr float kFusedScores = 0x1p22f;
 constexpr int kWaveRows = 32;
 static_assert(kWideRows == kWaveRows * kWavesPerBlock && kTileTokens == 16 * kWavesPerBlock, "a wave decodes one group");
 
@@ -298,7 +301,7 @@ void attention_wide_kernel(const RowsArgs a, uint32_t tiles) {
       for (int r = 1; r < 16; ++r) most[p] = fmaxf(most[p], score[p][r]);
       lift[p] = score_lift(0.0f, scales[p][1]);
     }
-    // Rounds the products first where a maximum is coarse (see kLiftedScores).
+    // For a maximum that is coarse: past kFusedScores.
     auto round_products = [&] {
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
@@ -314,9 +317,9 @@ void attention_wide_kernel(const RowsArgs a, uint32_t tiles) {
     };
     if (coarse) round_products();
     float top = highest();
-    if (ballot(top > m + kLag) != 0) {
+    if (ballot(top > m + (coarse ? 0.0f : kLag)) != 0) {
       // A maximum becomes coarse only here.  (Looked for in every tile it took 2% more time.)
-      if (!coarse && ballot(fabsf(top) > kLiftedScores && top > -__builtin_inff()) != 0) {
+      if (!coarse && ballot(fabsf(top) > kFusedScores && top > -__builtin_inff()) != 0) {
         coarse = true;
         round_products();
         top = highest();

@@ -204,7 +204,7 @@ def kv_paged_attention_fp8(
     are in ``out``, and are zeros in a new tensor; their ``lse`` is -inf either way.  Scales of blocks that a call's
     rows see are 0 (a block of zeros) or lie in [2**-60, 2**60]; scales may be expanded, e.g.
     ``per_head.expand(blocks, kv_heads)``.  Codes decode as in kv_paged_fp8_to_linear.  Query values are at most
-    2**100 in size; E4M3 value scales are at most 4 where a row's scores pass 2**22.
+    2**100 in size; E4M3 value scales are at most 4 where a row's scores pass 2**24.
 
     ``max_seq_len``, an upper bound of ``seq_lens`` that the caller knows, only decides how the work is cut;
     by default it is what ``block_tables`` has room for.  Returns the output, in ``query``'s type, and with

@@ -25,8 +25,8 @@ FORMS = [dict(lens=[40, 130, 700], hd=64), dict(lens=[5000, 130], hd=128), dict(
          dict(lens=[40, 130], rows=[2, 9], hd=64, dtype="fp32")]
 
 
-def _check(fmt, form, up, key_scale, value_scale=0.01):
-    """Query values of 2^up and a half of it."""
+def _check(fmt, form, up, key_scale, value_scale=0.01, below=None):
+    """Query values of 2^up and a half of it; rows that have scores (in base 2) of `below` and more get smaller ones."""
     case = Case(heads=4, kv_heads=2, seed=30, fmt=fmt, **form)
     rng = np.random.default_rng(2)
     hd = case.query.shape[2]
@@ -42,6 +42,9 @@ def _check(fmt, form, up, key_scale, value_scale=0.01):
     case.scales[1] *= value_scale / 0.01
     table = ref.decode_table(fmt)
     score = np.einsum("thd,hd->th", signs.numpy(), np.repeat(table[key[0, :, :, 0]], 2, axis=0))
+    if below is not None:
+        past = 2 * np.abs(score) * 2.0 ** up * key_scale * hd ** -0.5 * np.log2(np.e) >= below
+        signs, score = signs / np.where(past, 16.0, 1.0)[..., None], score / np.where(past, 16.0, 1.0)
     clear = np.abs(score) >= 0.5  # the others' scores nearly cancel
     case.query = (signs * 2.0 ** up).to(case.dtype)
     assert torch.isfinite(case.query).all()
@@ -101,3 +104,41 @@ def test_large_queries_over_blocks_of_zeros(fmt, form):
     args, kw = case.args()
     out, lse = musa_aiter.kv_paged_attention_fp8(*args, **kw, return_lse=True)
     case.check(out, lse)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("form", FORMS[:5])
+@pytest.mark.parametrize("value_scale", [64.0, 2.0 ** 30])
+def test_large_value_scales_below_the_coarse_scores(fmt, form, value_scale):
+    """Scores (in base 2) of up to 2^25 next to value scales of any size."""
+    for up in (16, 18, 20, 21, 22):
+        _check(fmt, form, up, 1.0, value_scale, below=2.0 ** 25)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("form", [dict(lens=[900, 300], rows=None), dict(lens=[200, 150], rows=[4, 3]),
+                                  dict(lens=[900, 300], rows=[100, 90])])
+@pytest.mark.parametrize("up", [20, 22, 23, 24, 25, 26])
+@pytest.mark.parametrize("rising", [True, False])
+def test_scores_that_differ_by_a_step(fmt, form, up, rising):
+    """Scores of 2^up + 0, 2, 4, ...: neighbours in float32, whose differences decide.  Products and sums may be rounded to
+    a step, so what is asked of the output is that it lies among the values: a mean of them in 64 bits has no larger size,
+    and the rounding adds 2^-7 of it at most (the weights' 2^-11 and the output's 2^-8)."""
+    case = Case(heads=2, kv_heads=2, hd=64, seed=33, fmt=fmt, **form)
+    one, step = {"e4m3": (7 << 3, 1 << 3), "e5m2": (15 << 2, 1 << 2)}[fmt]
+    case.cache[0][:] = 0
+    case.cache[0][:, :, 0, :] = one
+    for b, n in enumerate(case.lens):
+        for pos in range(int(n)):  # 2, 4, 8, 16, ... in this order, or the other way round
+            j = pos * 7 // int(n) if rising else 6 - pos * 7 // int(n)
+            case.cache[0][case.tables[b, pos // 16], :, 1, pos % 16] = one + (j + 1) * step
+    case.query[:] = 0
+    case.query[..., 0], case.query[..., 1] = 2.0 ** up, 1.0
+    case.scales[0][:] = 1.0
+    case.scales[1][:] = 3.5
+    args, kw = case.args()
+    out, lse = musa_aiter.kv_paged_attention_fp8(*args, **kw, softmax_scale=float(np.log(2.0)), return_lse=True)
+    got = out.double().cpu().numpy()
+    assert np.isfinite(got).all() and torch.isfinite(lse).all()
+    assert np.abs(got).max() <= 3.5 * np.abs(ref.decode_table(fmt)).max() * (1 + 2.0 ** -7)
+    assert (np.abs(lse.double().cpu().numpy() / np.log(2.0) - 2.0 ** up) <= 300 + 2.0 ** (up - 21)).all()
