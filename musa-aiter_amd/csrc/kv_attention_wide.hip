@@ -11,8 +11,8 @@
 // and masks are per lane), in the order in which V's operand, 8 tokens a lane, wants the weights.  Nothing crosses
 // lanes but the running maximum.  The rest (codes, scaling of queries and weights) is as in kv_attention.hip.
 //
-// Chunks of 2048 and 1753 rows (32 heads, 8 kv heads, 128 dims; 3769 and 8192 cached tokens): 420 us, 770 TFLOP/s; 8192
-// rows against 16384 tokens: 1922 us, 860 TFLOP/s (a large library product of bf16 matrices: 1260).  The first dozen calls
+// Chunks of 2048 and 1753 rows (32 heads, 8 kv heads, 128 dims; 3769 and 8192 cached tokens): 413 to 430 us, 750 to 785
+// TFLOP/s; 8192 rows against 16384 tokens: 1920 to 1980 us, 830 to 860 TFLOP/s (a large library product of bf16 matrices: 1260).  The first dozen calls
 // after a pause take 530 us.  The instructions of a wave's tile (1024 cycles of matrix instructions, about 1900 of others, a
 // third of them exponentials) bound it; the two waves of a SIMD mostly take turns: 31% and 57% of its cycles.  Tried and
 // slower or no faster: 256-row tiles of eight waves (6% faster for the largest calls, 5 to 25% slower elsewhere), the next
