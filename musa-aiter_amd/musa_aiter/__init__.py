@@ -87,6 +87,12 @@ from musa_aiter.ops.kv_transfer import (
     reset_kv_transfer_stats,
 )
 from musa_aiter.ops.kv_block_cache import kv_linear_to_paged_fp8_block, kv_paged_attention_fp8
+from musa_aiter.ops.kv_paged_attention import (
+    kv_accumulate_attention_weights,
+    kv_evict_paged_tokens,
+    kv_paged_attention,
+    kv_paged_attention_tree,
+)
 from musa_aiter.ops.kv_pages import (
     kv_compact_paged_blocks,
     kv_extend_paged_sequences,

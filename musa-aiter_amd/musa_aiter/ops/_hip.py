@@ -140,6 +140,12 @@ _SIGNATURES: dict[str, list] = {
     "musa_aiter_hip_pages_extend": [ctypes.c_char_p, _c_void_p],
     "musa_aiter_hip_pages_compact": [ctypes.c_char_p, _c_void_p],
     "musa_aiter_hip_pages_workspace": [ctypes.c_char_p, _i64],
+    # Operators on paged caches of plain values (musa_aiter_kv_paged_attention.h): packed call, stream.
+    "musa_aiter_hip_paged_attention": [ctypes.c_char_p, _c_void_p],
+    "musa_aiter_hip_paged_attention_workspace": [ctypes.c_char_p],
+    "musa_aiter_hip_attention_weights": [ctypes.c_char_p, _c_void_p],
+    "musa_aiter_hip_evict": [ctypes.c_char_p, _c_void_p],
+    "musa_aiter_hip_evict_workspace": [ctypes.c_char_p],
 }
 
 _RESTYPES = {
@@ -151,6 +157,8 @@ _RESTYPES = {
     "musa_aiter_hip_attention_splits": ctypes.c_int64,
     "musa_aiter_hip_attention_workspace": ctypes.c_int64,
     "musa_aiter_hip_pages_workspace": ctypes.c_int64,
+    "musa_aiter_hip_paged_attention_workspace": ctypes.c_int64,
+    "musa_aiter_hip_evict_workspace": ctypes.c_int64,
 }
 
 _lock = threading.Lock()
@@ -952,6 +960,90 @@ def pages(kind: str, *, op: str, device: torch.device, tables: torch.Tensor, len
             workspace = torch.empty(size, dtype=torch.uint8, device=device)
             struct.pack_into("<Qq", call, _PAGES_WORKSPACE_AT, workspace.data_ptr(), size)
         rc = fn("musa_aiter_hip_pages_" + kind)(bytes(call), stream_ptr(device))
+        del workspace
+    check(rc, op)
+
+
+# ----- operators on paged caches of plain values (include/musa_aiter_kv_paged_attention.h) ----------
+
+# musa_aiter_hip_paged_attention_call: query, out, lse, caches, tables, lens, starts, masks, weights, workspace, its
+# bytes, eight sizes, query strides, block strides, table stride, mask words and stride, window, sinks, longest, tokens
+# and strides of the weights, softmax scale, six flags.
+_CACHE_ATTENTION_CALL = struct.Struct("<11Qq8q2q2qq2q2qq3qd6i")
+_CACHE_ATTENTION_WORKSPACE_AT = 80
+
+
+def _cache_attention_call(query, out, lse, caches, tables, lens, starts, masks, weights, sizes, window, sinks, longest,
+                          softmax_scale, dtype, fill_rows) -> bytearray:
+    key, value = caches[0], caches[-1]
+    size = key.element_size()
+    return bytearray(_CACHE_ATTENTION_CALL.pack(
+        query.data_ptr(), _data(out), _data(lse), key.data_ptr(), value.data_ptr(), tables.data_ptr(), lens.data_ptr(),
+        _data(starts), _data(masks), _data(weights), 0, 0, *sizes, query.stride(0), query.stride(1),
+        key.stride(0) * size, value.stride(0) * size, tables.stride(0), 0 if masks is None else masks.shape[1],
+        0 if masks is None else masks.stride(0), window, sinks, longest, 0 if weights is None else weights.shape[2],
+        0 if weights is None else weights.stride(0), 0 if weights is None else weights.stride(1), softmax_scale, dtype,
+        tables.dtype is torch.int64, lens.dtype is torch.int64, starts is not None and starts.dtype is torch.int64,
+        fill_rows, 0))
+
+
+def paged_attention(*, op: str, query: torch.Tensor, out: torch.Tensor, lse: torch.Tensor | None, caches,
+                    tables: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor | None,
+                    masks: torch.Tensor | None, sizes, window: int, sinks: int, longest: int, softmax_scale: float,
+                    dtype: int, fill_rows: bool) -> None:
+    """Attention over a paged cache of plain values; the parts' workspace comes from torch's caching allocator."""
+    if sizes[0] == 0:
+        return
+    device = query.device
+    call = _cache_attention_call(query, out, lse, caches, tables, lens, starts, masks, None, sizes, window, sinks,
+                                 longest, softmax_scale, dtype, fill_rows)
+    with on_device(device):
+        workspace = None
+        size = fn("musa_aiter_hip_paged_attention_workspace")(bytes(call))
+        if size > 0:
+            workspace = torch.empty(size, dtype=torch.uint8, device=device)
+            struct.pack_into("<Qq", call, _CACHE_ATTENTION_WORKSPACE_AT, workspace.data_ptr(), size)
+        rc = fn("musa_aiter_hip_paged_attention")(bytes(call), stream_ptr(device))
+        del workspace
+    check(rc, op)
+
+
+def attention_weights(*, op: str, weights: torch.Tensor, query: torch.Tensor, lse: torch.Tensor, caches,
+                      tables: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor | None, sizes, window: int,
+                      sinks: int, longest: int, softmax_scale: float, dtype: int) -> None:
+    """The weight that tokens gather, added to ``weights``."""
+    if sizes[0] == 0:
+        return
+    device = query.device
+    call = _cache_attention_call(query, None, lse, caches, tables, lens, starts, None, weights, sizes, window, sinks,
+                                 longest, softmax_scale, dtype, False)
+    with on_device(device):
+        rc = fn("musa_aiter_hip_attention_weights")(bytes(call), stream_ptr(device))
+    check(rc, op)
+
+
+# musa_aiter_hip_evict_call: caches, weights, tables, lens, keep, refs, kept, workspace, its bytes, seven sizes and the
+# element's bytes, layer and block strides, tokens and strides of the weights, table stride, sinks, recent, four flags.
+_EVICT_CALL = struct.Struct("<9Qq8q2q2q4qq2q4i")
+_EVICT_WORKSPACE_AT = 64
+
+
+def evict(*, op: str, caches, weights: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, keep: torch.Tensor,
+          refs: torch.Tensor | None, kept: torch.Tensor, sizes, sinks: int, recent: int) -> None:
+    """The eviction; the marks of the tokens that stay come from torch's caching allocator."""
+    device, size = caches[0].device, caches[0].element_size()
+    layered = caches[0].dim() == 5
+    call = bytearray(_EVICT_CALL.pack(
+        caches[0].data_ptr(), caches[1].data_ptr(), weights.data_ptr(), tables.data_ptr(), lens.data_ptr(),
+        keep.data_ptr(), _data(refs), kept.data_ptr(), 0, 0, *sizes, size,
+        *(c.stride(0) * size if layered else 0 for c in caches), *(c.stride(-4) * size for c in caches),
+        weights.shape[-1], weights.stride(0) if layered else 0, weights.stride(-3), weights.stride(-2),
+        tables.stride(0), sinks, recent, *(t is not None and t.dtype is torch.int64 for t in (tables, lens, keep, refs))))
+    with on_device(device):
+        size = fn("musa_aiter_hip_evict_workspace")(bytes(call))
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        struct.pack_into("<Qq", call, _EVICT_WORKSPACE_AT, workspace.data_ptr(), size)
+        rc = fn("musa_aiter_hip_evict")(bytes(call), stream_ptr(device))
         del workspace
     check(rc, op)
 

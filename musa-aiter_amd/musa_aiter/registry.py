@@ -173,3 +173,11 @@ _serving("kv_extend_paged_sequences", "kvpages", _PAGES,
 _serving("kv_fork_paged_sequences", "kvpages", _PAGES, "Rows take over other rows' pages by reference count.")
 _serving("kv_free_paged_sequences", "kvpages", _PAGES, "Rows are cut or ended and their pages released.")
 _serving("kv_compact_paged_blocks", "kvpages", _PAGES, "Pages in use move to the front of the cache; tables follow.")
+# Paged caches of plain values: attention over them, and the eviction of what it does not look at.
+_serving("kv_paged_attention", "kvattention", _FLOAT,
+         "Causal attention (decode, draft and prompt rows) over a paged cache, with a window and visible first tokens.")
+_serving("kv_paged_attention_tree", "kvattention", _FLOAT, "Attention of trees of drafted tokens over a paged cache.")
+_serving("kv_accumulate_attention_weights", "kvattention", _FLOAT,
+         "Adds up the attention weight that every cached token gets.")
+_serving("kv_evict_paged_tokens", "kvattention", ("float32", "float16", "bfloat16", "uint8", "float8_e4m3fn", "float8_e5m2"),
+         "Keeps the first, the last and the heaviest tokens of every sequence and kv head, moved to the front.")
