@@ -76,7 +76,8 @@ __device__ __forceinline__ View make_view(const CacheArgs& a, int32_t seq, int32
     w.length = w.end;
   } else {
     w.gap = begin16 - w.front;
-    w.length = w.front + max(w.end - begin16, 0);
+    // A window past the end (a length past the table's room) leaves the first tokens, up to the end.
+    w.length = w.end > begin16 ? w.front + w.end - begin16 : min(w.front, w.end);
   }
   return w;
 }
@@ -234,7 +235,7 @@ __device__ __forceinline__ float log_sum(float m, float l) {
 
 // Arguments of a launch in tiles of `size` rows (0: the form for any shape, a line per row and head).
 CacheArgs cache_args(const CacheAttnCall& c, int size);
-// Whether the caches' blocks can be read 8 tokens at a time.
+// Whether the caches' blocks can be read, and the output be written, as the matrix-core forms do.
 bool tiles_fit(const CacheAttnCall& c);
 
 }  // namespace catt

@@ -5,7 +5,7 @@
 //
 // over the positions j that the row sees.  One pass over the cache with a running maximum and sum in base 2; parts of a
 // line (a row tile and a kv head) that run side by side leave (m, l, acc) in a workspace and a second launch joins them.
-#include "kv_cache_attention.h"
+#include "kv_cache_attention_tiles.h"
 
 namespace kvhip {
 namespace catt {
@@ -158,21 +158,39 @@ constexpr int64_t kAnyPart = 1024;    // positions of a part of the form for any
 constexpr int64_t kAnyParts = 64;
 constexpr int64_t kAnyGroups = 8192;  // workgroups from which on a line is not cut further
 
-// How a call is cut.
+// How a call is cut.  size: rows of a tile (0: the form for any shape).
 struct Plan {
-  int64_t lines, parts, part, slot_rows, tiles;
+  int64_t size, lines, parts, part, slot_rows, tiles;
 };
+
+constexpr int64_t kTurnPlaces = kTilePlaces * kWavesPerBlock;
+constexpr int64_t kRowsGroups = 8192;
+
+// Parts of a multiple of `unit` places each: no more than give `groups` workgroups, and `most` of a line.
+void cut(Plan& p, int64_t places, int64_t unit, int64_t groups, int64_t most) {
+  int64_t parts = groups / (p.lines > 0 ? p.lines : 1);
+  parts = parts < 1 ? 1 : parts < most ? parts : most;
+  p.part = ((places + parts - 1) / parts + unit - 1) / unit * unit;
+  p.parts = (places + p.part - 1) / p.part;
+}
 
 Plan make_plan(const CacheAttnCall& c) {
   Plan p{};
+  if (tiles_fit(c)) {
+    const int64_t group = c.heads / c.kv_heads;
+    const int64_t seq_rows = (c.starts == nullptr || c.batch == 0 ? 1 : (c.rows + c.batch - 1) / c.batch) * group;
+    p.size = seq_rows <= 16 || c.head_dim > 128 ? 16 : 32;
+    CacheArgs a = cache_args(c, static_cast<int>(p.size));
+    p.tiles = tiles_bound(a.r.c, static_cast<int>(p.size));
+    if (p.tiles < 1) p.tiles = 1;  // rows of no sequence
+    p.lines = p.tiles * c.kv_heads;
+    p.slot_rows = c.starts == nullptr && group < p.size ? group : p.size;
+    cut(p, most_places(c, static_cast<int>(p.size)), kTurnPlaces, kRowsGroups, 256);
+    return p;
+  }
   p.lines = c.rows * c.heads;
   p.slot_rows = 1;
-  const int64_t places = most_places(c, 1);
-  int64_t parts = kAnyGroups / (p.lines > 0 ? p.lines : 1);
-  parts = parts < 1 ? 1 : parts < kAnyParts ? parts : kAnyParts;
-  p.part = (places + parts - 1) / parts;
-  p.part = p.part < kAnyPart ? kAnyPart : (p.part + kBlockThreads - 1) / kBlockThreads * kBlockThreads;
-  p.parts = (places + p.part - 1) / p.part;
+  cut(p, most_places(c, 1), kAnyPart, kAnyGroups, kAnyParts);
   return p;
 }
 
@@ -183,10 +201,15 @@ int64_t plan_workspace(const CacheAttnCall& c, const Plan& p) {
 
 template <int DT>
 hipError_t launch(const CacheAttnCall& c, const Plan& p, CacheArgs a, hipStream_t stream) {
-  cache_any_kernel<DT><<<dim3(c.rows, c.heads, p.parts), kBlockThreads, 0, stream>>>(a);
+  hipError_t err;
+  if (p.size > 0) {
+    err = launch_rows(a, static_cast<int>(p.size / 16), stream);
+  } else {
+    cache_any_kernel<DT><<<dim3(c.rows, c.heads, p.parts), kBlockThreads, 0, stream>>>(a);
+    err = hipGetLastError();
+  }
+  if (err != hipSuccess) return err;
   if (p.parts > 1) {
-    hipError_t err = hipGetLastError();
-    if (err != hipSuccess) return err;
     cache_join_kernel<DT><<<dim3(p.lines, p.slot_rows), kBlockThreads, 0, stream>>>(a);
   }
   return hipGetLastError();
@@ -196,7 +219,9 @@ hipError_t launch(const CacheAttnCall& c, const Plan& p, CacheArgs a, hipStream_
 
 bool tiles_fit(const CacheAttnCall& c) {
   if (c.dtype != kLinF16 && c.dtype != kLinBF16) return false;
-  if (c.block_size % 8 != 0) return false;
+  const int64_t hd = c.head_dim;
+  if (c.block_size % 8 != 0 || (hd != 64 && hd != 96 && hd != 128 && hd != 192 && hd != 256)) return false;
+  if ((reinterpret_cast<uint64_t>(c.out) & 7) != 0 || c.kv_heads > 65535) return false;
   for (int kv = 0; kv < 2; ++kv)
     if (c.cache[kv] != nullptr && ((reinterpret_cast<uint64_t>(c.cache[kv]) | c.cache_block_stride[kv]) & 15) != 0)
       return false;
@@ -263,7 +288,7 @@ int64_t cache_attention_workspace(const CacheAttnCall& c) { return catt::plan_wo
 
 hipError_t launch_cache_attention(const CacheAttnCall& c, hipStream_t stream) {
   const catt::Plan p = catt::make_plan(c);
-  catt::CacheArgs a = catt::cache_args(c, 0);
+  catt::CacheArgs a = catt::cache_args(c, static_cast<int>(p.size));
   a.part = static_cast<int32_t>(p.part);
   a.parts = static_cast<int32_t>(p.parts);
   a.slot_rows = static_cast<int32_t>(p.slot_rows);
