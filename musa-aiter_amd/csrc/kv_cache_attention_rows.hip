@@ -60,7 +60,6 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_rows_kernel(const Cach
 
   stage_queries<DT, HD, NT>(a, tile, kv_head, tile_rows, queries);
   if (threadIdx.x == 0) odd_rows = 0;
-  __syncthreads();
 
   // Each lane's row of every 16: what it sees, its maximum and sum.
   RowSight sight[NT];
@@ -82,9 +81,35 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_rows_kernel(const Cach
   const uint8_t* key = static_cast<const uint8_t*>(c.cache[0]) + (static_cast<int64_t>(kv_head) * HD + g) * row_bytes;
   const uint8_t* value = static_cast<const uint8_t*>(c.cache[1]) + (static_cast<int64_t>(kv_head) * HD + x) * row_bytes;
 
-  auto one_tile = [&](auto dirty_tag, const Unit& unit) {
-    constexpr bool kDirty = decltype(dirty_tag)::value;
-    const uint8_t* k = key + unit.block * c.cache_block_stride[0] + unit.place * 2;
+  // Loads go in groups of 8 (8 KiB of the wave), one or two of them on their way at any time: kSteps of K, as many of V,
+  // then the next tile's.
+  u32x4 ahead[2][8];
+  const uint8_t* k_unit;     // of the tile whose K is being loaded
+  const uint8_t* v_unit[4];  // units r of the tile at hand
+  // The addresses go on by steps, through `stepped`: the compiler would keep a register pair for each of the offsets.
+  auto load_k = [&](int ks) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ahead[ks & 1][i] = ld16_cached(k_unit);
+      k_unit = stepped(k_unit + 4 * row_bytes);
+    }
+  };
+  auto load_v = [&](int group) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = (group * 8 + i) / kDimTiles;
+      ahead[(kSteps + group) & 1][i] = ld16_cached(v_unit[r]);
+      v_unit[r] = stepped(v_unit[r] + 16 * row_bytes);
+    }
+  };
+  // masked: some row does not see some of the positions.  (Two copies of the body, with and without masks, spill.)
+  auto one_tile = [&](bool masked, const Unit& unit, const Unit& next, bool more) {
+    uint32_t bits[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      v_unit[r] = value + __shfl(unit.block, 4 * g + r) * c.cache_block_stride[1] + __shfl(unit.place, 4 * g + r) * 2;
+      bits[r] = __shfl(unit.bits, 4 * g + r);
+    }
     f32x4 s[NT][8];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -92,44 +117,39 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_rows_kernel(const Cach
       for (int t = 0; t < 8; ++t) s[nt][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) {
-      u32x4 raw[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) raw[i] = ld16_cached(k + (32 * ks + 4 * i) * row_bytes);
       u32x4 q[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) q[nt] = queries[(nt * kSteps + ks) * kWave + lane];
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
-        const u32x4 tokens = token_dims(raw, t);
+        const u32x4 tokens = token_dims(ahead[ks & 1], t);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s[nt][t] = Mma16<DT>::mma(tokens, q[nt], s[nt][t]);
       }
+      if (ks + 2 < kSteps) load_k(ks + 2);
+      else load_v(ks + 2 - kSteps);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    uint32_t bits[4] = {};
-    int32_t block[4], place[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      block[r] = __shfl(unit.block, 4 * g + r);
-      place[r] = __shfl(unit.place, 4 * g + r);
-      if constexpr (kDirty) bits[r] = __shfl(unit.bits, 4 * g + r);
-    }
+    k_unit = key + next.block * c.cache_block_stride[0] + next.place * 2;
     u32x4 weight[NT][2][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float top = m[nt];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        uint32_t seen = 0;
-        if constexpr (kDirty)
-          seen = bits[r] & row_bits(a, w, sight[nt], position(w, v0 + 8 * (unit_v + 2 * r)));
+      for (int t = 0; t < 8; ++t) s[nt][t] *= a.factor;
+      if (masked) {
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          float score = s[nt][t][r] * a.factor;
-          if constexpr (kDirty) score = (seen >> t & 1u) != 0 ? score : -__builtin_inff();
-          s[nt][t][r] = score;
-          top = fmaxf(top, score);
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t seen = bits[r] & row_bits(a, w, sight[nt], position(w, v0 + 8 * (unit_v + 2 * r)));
+#pragma unroll
+          for (int t = 0; t < 8; ++t)
+            if ((seen >> t & 1u) == 0) s[nt][t][r] = -__builtin_inff();
         }
       }
+      float top = m[nt];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) top = fmaxf(top, s[nt][t][r]);
       top = groups_max(top);
       const float ref = (top == -__builtin_inff() ? 0.0f : top) - kTop<DT>;
       if (ballot(top != m[nt]) != 0) {
@@ -152,30 +172,42 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_rows_kernel(const Cach
         }
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const uint8_t* v = value + block[r] * c.cache_block_stride[1] + place[r] * 2;
-      u32x4 keep{};
-      if constexpr (kDirty) keep = token_masks(bits[r]);
+    for (int group = 0; group < kSteps; ++group) {
+      u32x4 (&values)[8] = ahead[(kSteps + group) & 1];
+      if (masked) {  // what no row sees may be no number
 #pragma unroll
-      for (int dt = 0; dt < kDimTiles; ++dt) {
-        u32x4 values = ld16_cached(v + 16 * dt * row_bytes);
-        if constexpr (kDirty) values &= keep;
+        for (int i = 0; i < 8; ++i) values[i] &= token_masks(bits[(group * 8 + i) / kDimTiles]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = (group * 8 + i) / kDimTiles, dt = (group * 8 + i) % kDimTiles;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          acc[nt][dt] = Mma16<DT>::mma(values, weight[nt][0][r], acc[nt][dt]);
-          acc[nt][dt] = Mma16<DT>::mma(values, weight[nt][1][r], acc[nt][dt]);
+          acc[nt][dt] = Mma16<DT>::mma(values[i], weight[nt][0][r], acc[nt][dt]);
+          acc[nt][dt] = Mma16<DT>::mma(values[i], weight[nt][1][r], acc[nt][dt]);
         }
       }
+      if (group + 2 < kSteps) load_v(group + 2);
+      else if (more) load_k(group + 2 - kSteps);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  for (; v0 < hi; v0 += kWavesPerBlock * kTilePlaces) {
-    const Unit unit = resolve_unit(a, w, entry, v0 + 8 * unit_k, hi);
-    entry = load_unit(a, w, table, v0 + kWavesPerBlock * kTilePlaces + 8 * unit_k, hi);
-    if (ballot(unit.bits != 0xFFu) != 0 || !all_rows_see(a, w, v0))
-      one_tile(std::true_type{}, unit);
-    else
-      one_tile(std::false_type{}, unit);
+  Unit unit = resolve_unit(a, w, entry, v0 + 8 * unit_k, hi);
+  entry = load_unit(a, w, table, v0 + kWavesPerBlock * kTilePlaces + 8 * unit_k, hi);
+  if (v0 < hi) {
+    k_unit = key + unit.block * c.cache_block_stride[0] + unit.place * 2;
+    load_k(0);
+    load_k(1);
+  }
+  __syncthreads();
+  while (v0 < hi) {
+    const int32_t v1 = v0 + kWavesPerBlock * kTilePlaces;
+    const Unit next = resolve_unit(a, w, entry, v1 + 8 * unit_k, hi);
+    entry = load_unit(a, w, table, v1 + kWavesPerBlock * kTilePlaces + 8 * unit_k, hi);
+    one_tile(ballot(unit.bits != 0xFFu) != 0 || !all_rows_see(a, w, v0), unit, next, v1 < hi);
+    unit = next;
+    v0 = v1;
   }
 
   // The waves' sums, 16 rows at a time.

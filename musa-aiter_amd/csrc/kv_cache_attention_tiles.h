@@ -94,6 +94,11 @@ __device__ __forceinline__ u32x4 token_masks(uint32_t bits) {
   return out;
 }
 
+__device__ __forceinline__ const uint8_t* stepped(const uint8_t* p) {
+  asm volatile("" : "+v"(p));
+  return p;
+}
+
 // Row and head of the in_tile-th row of a tile.
 struct TilePlace {
   int64_t row, head;
