@@ -69,7 +69,7 @@ def _compile(src: Path, obj: Path) -> None:
         sys.stderr.write("\n".join(noise) + "\n")
 
 
-HOST_SOURCES = ("kv_host.cpp", "kv_host_serving.cpp")
+HOST_SOURCES = ("kv_host.cpp", "kv_host_serving.cpp", "kv_host_paged_attention.cpp")
 HOST_MODULE = "_kv_host"
 
 

@@ -341,7 +341,8 @@ py::tuple paged_call(const py::handle& key_cache, const py::handle& value_cache,
 
 }  // namespace
 
-void add_serving_calls(py::module_& m);  // kv_host_serving.cpp
+void add_serving_calls(py::module_& m);          // kv_host_serving.cpp
+void add_paged_attention_calls(py::module_& m);  // kv_host_paged_attention.cpp
 
 PYBIND11_MODULE(_kv_host, m) {
   m.doc() = "Host-side tensor checks and address tables for the MI355X KV path";
@@ -352,6 +353,7 @@ PYBIND11_MODULE(_kv_host, m) {
   m.def("two_x_nl_rows", &two_x_nl_rows);
   m.def("paged_call", &paged_call);
   add_serving_calls(m);
+  add_paged_attention_calls(m);
   m.attr("NOT_TAKEN") = kNotTaken;
   m.attr("OK") = static_cast<int>(kOk);
   m.attr("SHAPE") = static_cast<int>(kShape);

@@ -8,53 +8,14 @@
 #include <cstdint>
 
 #include "kv_host_calls.h"
+#include "kv_host_checks.h"
 #include "musa_aiter_kv_serving.h"
 
 namespace py = pybind11;
 
 namespace {
 
-constexpr int64_t kNotTaken = -2;
-
-const at::Tensor* plain(const py::handle& h, int64_t device) {
-  if (!THPVariable_CheckExact(h.ptr())) return nullptr;
-  const at::Tensor& t = THPVariable_Unpack(h.ptr());
-  return t.is_cuda() && t.device().index() == device ? &t : nullptr;
-}
-
-bool index_kind(at::ScalarType t) { return t == at::kInt || t == at::kLong; }
-bool fp8_kind(at::ScalarType t) { return t == at::kByte || t == at::kFloat8_e4m3fn || t == at::kFloat8_e5m2; }
-bool float_kind(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
-int float_id(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kHalf ? 1 : 2; }
-
-// The trailing [kv_heads, head_dim, block_size] of every block is packed, and no extent is empty or expanded.
-bool packed_blocks(const at::Tensor& c) {
-  const int64_t n = c.dim();
-  int64_t want = 1;
-  for (int64_t i = n - 1; i >= n - 3; --i) {
-    if (c.size(i) < 1 || (c.size(i) != 1 && c.stride(i) != want)) return false;
-    want *= c.size(i);
-  }
-  for (int64_t i = 0; i < n - 3; ++i)
-    if (c.size(i) < 1 || (c.size(i) != 1 && c.stride(i) == 0)) return false;
-  return true;
-}
-
-bool rows_packed(const at::Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }
-
-py::tuple not_taken() { return py::make_tuple(kNotTaken, py::none(), py::none()); }
-
-// A call whose tensors do not fit in memory is left to Python too, which raises torch's own error for it.
-template <typename... Args>
-auto taken_or_left(py::tuple (*call)(Args...)) {
-  return [call](Args... args) {
-    try {
-      return call(args...);
-    } catch (const c10::OutOfMemoryError&) {
-      return not_taken();
-    }
-  };
-}
+using namespace kv_host;
 
 // kv_paged_attention_fp8.  `longest` < 0: what the tables have room for.  Returns (status, out, lse or None).
 py::tuple attention_call(const py::handle& query_h, const py::handle& key_h, const py::handle& value_h,

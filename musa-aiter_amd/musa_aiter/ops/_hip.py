@@ -1127,3 +1127,48 @@ def pages_native(kind: str, op, key_cache, value_cache, tables, lens, refs, rows
         return None
     check(rc, op)
     return slots, result
+
+
+def paged_attention_native(op, query, key_cache, value_cache, tables, lens, masks, starts, out, longest: int,
+                           softmax_scale: float, window: int, sinks: int, with_lse: bool):
+    """(out, lse) of one attention call over caches of plain values, or None."""
+    if type(query) is not torch.Tensor or not query.is_cuda:
+        return None
+    index = torch._C._cuda_getDevice()
+    rc, result, lse = (_host or host()).paged_attention_call(
+        query, key_cache, value_cache, tables, lens, masks, starts, out, longest, softmax_scale, window, sinks, with_lse,
+        _entry("musa_aiter_hip_paged_attention"), _entry("musa_aiter_hip_paged_attention_workspace"),
+        torch._C._cuda_getCurrentRawStream(index), index)
+    if rc == _host.NOT_TAKEN:
+        return None
+    check(rc, op)
+    return result, lse
+
+
+def attention_weights_native(op, weights, query, key_cache, tables, lens, lse, starts, longest: int,
+                             softmax_scale: float, window: int, sinks: int):
+    """One call that adds to the gathered weights: True, or None."""
+    if type(query) is not torch.Tensor or not query.is_cuda:
+        return None
+    index = torch._C._cuda_getDevice()
+    rc = (_host or host()).attention_weights_call(
+        weights, query, key_cache, tables, lens, lse, starts, longest, softmax_scale, window, sinks,
+        _entry("musa_aiter_hip_attention_weights"), torch._C._cuda_getCurrentRawStream(index), index)
+    if rc == _host.NOT_TAKEN:
+        return None
+    check(rc, op)
+    return True
+
+
+def evict_native(op, key_cache, value_cache, weights, tables, lens, keep, refs, sinks: int, recent: int):
+    """The lengths that one eviction leaves, or None."""
+    if type(key_cache) is not torch.Tensor or not key_cache.is_cuda:
+        return None
+    index = torch._C._cuda_getDevice()
+    rc, kept, _ = (_host or host()).evict_call(
+        key_cache, value_cache, weights, tables, lens, keep, refs, sinks, recent, _entry("musa_aiter_hip_evict"),
+        _entry("musa_aiter_hip_evict_workspace"), torch._C._cuda_getCurrentRawStream(index), index)
+    if rc == _host.NOT_TAKEN:
+        return None
+    check(rc, op)
+    return kept

@@ -82,7 +82,7 @@ class _Rows:
         self.query, self.device = query, device
         self._caches, self._indices = caches, (block_tables, seq_lens, query_starts)
         self._shape = (rows, batch, heads, nh, hd, bs, nb, width)
-        self._scale, self._window, self._sinks = scale, int(window or 0), int(sinks) if window else 0
+        self._scale, self._window, self._sinks = scale, min(int(window or 0), _MAX_ROOM), min(int(sinks), _MAX_ROOM) if window else 0
         self._longest = width * bs if max_seq_len is None else min(int(max_seq_len), 1 << 62)
 
     def call(self) -> dict:
@@ -96,6 +96,18 @@ class _Rows:
             tables=_index_rows(tables), lens=_index_rows(lens), starts=None if starts is None else _index_rows(starts),
             sizes=self._shape, window=self._window, sinks=self._sinks, longest=self._longest,
             softmax_scale=self._scale, dtype=_LIN_DTYPE[query.dtype])
+
+
+def _native_sight(query: torch.Tensor, max_seq_len, softmax_scale, window, sinks) -> tuple | None:
+    """(longest, scale, window, sinks) as the host module takes them, or None for what the checks have to look at."""
+    if not (window is None or type(window) is int and 0 < window < 1 << 62) \
+            or not (type(sinks) is int and 0 <= sinks < 1 << 62) \
+            or not (max_seq_len is None or type(max_seq_len) is int and 0 <= max_seq_len < 1 << 62) \
+            or not (softmax_scale is None or type(softmax_scale) is float and math.isfinite(softmax_scale)) \
+            or query.dim() != 3 or query.shape[2] < 1:
+        return None
+    return (-1 if max_seq_len is None else max_seq_len, query.shape[2] ** -0.5 if softmax_scale is None else softmax_scale,
+            window or 0, sinks)
 
 
 def _attention(op: str, rows: _Rows, masks: torch.Tensor | None, out: torch.Tensor | None, return_lse: bool):
@@ -150,6 +162,13 @@ def kv_paged_attention(
     weights keep its 11 bits down to 2**-28 of a row's largest, bfloat16 ones 8 bits); with float32 ones nothing is.
     """
     op = "kv_paged_attention"
+    sight = _native_sight(query, max_seq_len, softmax_scale, window, sinks)
+    if sight is not None:
+        got = _hip.paged_attention_native(op, query, key_cache, value_cache, block_tables, seq_lens, None, query_starts,
+                                          out, *sight, return_lse)
+        if got is not None:
+            _emit(op, query, "gfx950 paged attention")
+            return got if return_lse else got[0]
     rows = _Rows(op, query, (key_cache, value_cache), block_tables, seq_lens, query_starts, max_seq_len, softmax_scale,
                  window, sinks)
     got = _attention(op, rows, None, out, return_lse)
@@ -182,6 +201,13 @@ def kv_paged_attention_tree(
     Everything else is as in kv_paged_attention.
     """
     op = "kv_paged_attention_tree"
+    sight = _native_sight(query, max_seq_len, softmax_scale, None, 0)
+    if sight is not None and tree_masks is not None:
+        got = _hip.paged_attention_native(op, query, key_cache, value_cache, block_tables, seq_lens, tree_masks,
+                                          query_starts, out, *sight, return_lse)
+        if got is not None:
+            _emit(op, query, "gfx950 paged attention of draft trees")
+            return got if return_lse else got[0]
     rows = _Rows(op, query, (key_cache, value_cache), block_tables, seq_lens, query_starts, max_seq_len, softmax_scale,
                  None, 0)
     if tree_masks.dim() != 2 or tree_masks.shape[0] != rows.rows or tree_masks.shape[1] < 1:
@@ -217,6 +243,11 @@ def kv_accumulate_attention_weights(
     ``lse`` is -inf give nothing.  Sums are float32 and made in the same order in every call: no atomics.
     """
     op = "kv_accumulate_attention_weights"
+    sight = _native_sight(query, max_seq_len, softmax_scale, window, sinks)
+    if sight is not None and _hip.attention_weights_native(op, weights, query, key_cache, block_tables, seq_lens, lse,
+                                                           query_starts, *sight):
+        _emit(op, query, "gfx950 gathered attention weights")
+        return
     rows = _Rows(op, query, (key_cache,), block_tables, seq_lens, query_starts, max_seq_len, softmax_scale, window,
                  sinks)
     if weights.dim() != 3 or tuple(weights.shape[:2]) != (rows.batch, rows.kv_heads):
@@ -268,6 +299,12 @@ def kv_evict_paged_tokens(
     caller knows that no two sequences share a page.
     """
     op = "kv_evict_paged_tokens"
+    if type(sinks) is int and 0 <= sinks < 1 << 62 and type(recent) is int and 0 <= recent < 1 << 62:
+        kept = _hip.evict_native(op, key_cache, value_cache, weights, block_tables, seq_lens, keep_lens, ref_counts,
+                                 sinks, recent)
+        if kept is not None:
+            _emit(op, key_cache, "gfx950 eviction by gathered weight")
+            return kept
     if key_cache.dtype != value_cache.dtype or key_cache.element_size() not in (1, 2, 4):
         raise ValueError(f"{op}: caches must share one dtype of 1, 2 or 4 bytes")
     layered = key_cache.dim() == 5
