@@ -4,7 +4,7 @@
 //
 // with the scores s_j of kv_cache_attention.hip and the logarithms it returned.  A token's sum is made by one
 // workgroup, in the same order in every run: no atomics.
-#include "kv_cache_attention.h"
+#include "kv_cache_attention_tiles.h"
 
 namespace kvhip {
 namespace catt {
@@ -52,14 +52,181 @@ __global__ __launch_bounds__(kBlockThreads) void weights_any_kernel(const CacheA
   }
 }
 
+// ----- matrix-core form -----------------------------------------------------------------------------
+// A wave keeps the keys of 128 positions (16 units of 8, see kv_cache_attention_rows.hip) as operands in registers and
+// goes through the rows, 16 at a time: S^T = K Q^T.  Each lane adds up the weights that its row of every 16 gives its 32
+// positions; the lanes' sums meet at the end.  Lane (x, g) holds the dims 32 k + 8 g + i of K here, so that 16 bytes of a
+// query are an operand as they are.
+// With few rows the waves of a workgroup take different positions (bound by the read of K: all of a wave's 32 loads are
+// on their way at once), with many the same positions and a quarter of the rows each (bound by 32 exponentials of a
+// quarter of the full rate next to 32 products).
+constexpr int kManyTiles = 4;  // row tiles of a sequence from which on the waves share positions
+
+__device__ __forceinline__ float sum_of_16(float v) {  // over lanes that differ in x
+#define KVHIP_ROTATE(n) \
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x120 + n, 0xF, 0xF, false))
+  KVHIP_ROTATE(8);
+  KVHIP_ROTATE(4);
+  KVHIP_ROTATE(2);
+  KVHIP_ROTATE(1);
+#undef KVHIP_ROTATE
+  return v;
+}
+
+template <int DT, int HD>
+__global__ __launch_bounds__(kBlockThreads, HD <= 128 ? 2 : 1) void weights_tile_kernel(const CacheArgs a) {
+  constexpr int kSteps = HD / 32;
+  const AttnCall& c = a.r.c;
+  const int lane = lane_id(), wave = wave_in_block(), x = lane & 15, g = lane >> 4;
+  const int32_t seq = blockIdx.y, kv_head = blockIdx.z, group = a.r.group;
+  __shared__ __attribute__((aligned(16))) float sums[kWavesPerBlock][kTilePlaces];
+  const SeqRows seq_rows_ = seq_rows(c, seq);
+  if (seq_rows_.count == 0) return;
+  const int32_t count = static_cast<int32_t>(seq_rows_.count), rows = count * group;
+  const View w = make_view(a, seq, count, 0, count - 1);
+  const bool many = a.parts > 1;  // the waves share positions
+  const int32_t stride = many ? kTilePlaces : kTilePlaces * kWavesPerBlock;
+  const uint8_t* table = static_cast<const uint8_t*>(c.tables) +
+                         static_cast<int64_t>(seq) * c.table_stride * (c.wide_tables ? 8 : 4);
+  const int64_t row_bytes = static_cast<int64_t>(a.r.bs) * 2;
+  const float* lse_of = c.lse + seq_rows_.first * c.heads + static_cast<int64_t>(kv_head) * group;
+  const uint16_t* query = static_cast<const uint16_t*>(c.query) + seq_rows_.first * c.query_row_stride +
+                          static_cast<int64_t>(kv_head) * group * c.query_head_stride + 8 * g;
+  for (int32_t base = blockIdx.x * stride; base < w.length; base += gridDim.x * stride) {
+    const int32_t v0 = base + (many ? 0 : wave * kTilePlaces);
+    const UnitEntry entry = load_unit(a, w, table, v0 + 8 * x, w.length);
+    const Unit unit = resolve_unit(a, w, entry, v0 + 8 * x, w.length);
+    u32x4 keys[kSteps][8];
+    {
+      u32x4 raw[kSteps][8];
+      const uint8_t* k = static_cast<const uint8_t*>(c.cache[0]) + unit.block * c.cache_block_stride[0] +
+                         unit.place * 2 + (static_cast<int64_t>(kv_head) * HD + 8 * g) * row_bytes;
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) {
+        const uint8_t* from = k;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          raw[ks][i] = ld16_cached(from);
+          from = stepped(from + row_bytes);
+        }
+        k = stepped(k + 32 * row_bytes);
+      }
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) keys[ks][t] = token_dims(raw[ks], t);
+    }
+    uint32_t bits[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) bits[r] = __shfl(unit.bits, 4 * g + r);
+    const bool whole = ballot(unit.bits != 0xFFu) == 0;
+    // Positions of the tile: none of them is past last, none but first ones in front of from.
+    const int32_t from = v0 < w.front ? 0 : v0 + w.gap, last = position(w, v0 + kTilePlaces - 1);
+    f32x4 sum[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) sum[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    const int32_t step = many ? 16 * kWavesPerBlock : 16;
+    // Rows in front of the tile's first position see none of it.
+    int32_t at0 = many ? 16 * wave : 0;
+    const int32_t skip = max(from - w.before, 0);
+    if (skip >= count || v0 >= w.length) at0 = rows;
+    else at0 += skip * group / step * step;
+    for (; at0 < rows; at0 += step) {
+      const int32_t at = min(at0 + x, rows - 1), i = at / group;
+      const int64_t row = i, head = at - i * group;
+      const float lse = lse_of[row * c.heads + head];
+      const uint16_t* q = query + row * c.query_row_stride + head * c.query_head_stride;
+      u32x4 rows16[kSteps];
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) rows16[ks] = ld16_cached(reinterpret_cast<const uint8_t*>(q + 32 * ks));
+      f32x4 s[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) s[t] = Mma16<DT>::mma(keys[ks][t], rows16[ks], s[t]);
+      }
+      const float less = lse * kLog2e;
+      const bool gives = at0 + x < rows && lse != -__builtin_inff();
+      const int32_t pos_lo = w.before + at0 / group, pos_hi = w.before + min(at0 + 15, rows - 1) / group;
+      const bool plain = whole && v0 >= w.front && last <= pos_lo && (a.window == 0 || from > pos_hi - a.window) &&
+                         ballot(!gives) == 0;
+      if (plain) {
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum[t][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], a.factor, -less));
+      } else {
+        const RowSight sight{w.before + i, nullptr};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t seen = gives ? bits[r] & row_bits(a, w, sight, position(w, v0 + 8 * (4 * g + r))) : 0;
+#pragma unroll
+          for (int t = 0; t < 8; ++t) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], a.factor, -less));
+            sum[t][r] += (seen >> t & 1u) != 0 ? p : 0.0f;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const float all = sum_of_16(sum[t][r]);
+        if (x == 0) sums[wave][32 * g + 8 * r + t] = all;
+      }
+    __syncthreads();
+    float* weights = a.weights + seq * a.weight_row_stride + kv_head * a.weight_head_stride;
+    for (int32_t n = threadIdx.x; n < stride; n += kBlockThreads) {
+      const int32_t token = position(w, base + n);
+      float all = many ? 0.0f : sums[n / kTilePlaces][n % kTilePlaces];
+      if (many)
+        for (int k = 0; k < kWavesPerBlock; ++k) all += sums[k][n];
+      // What no row sees, behind the end among it, gathered nothing and is not written.
+      if (base + n < w.length && token < a.weight_tokens && all != 0.0f) weights[token] += all;
+    }
+    __syncthreads();
+  }
+}
+
 template <int DT>
-hipError_t launch(const CacheAttnCall& c, const CacheArgs& a, hipStream_t stream) {
+hipError_t launch_tiles(const CacheArgs& a, dim3 grid, hipStream_t stream) {
+  switch (a.r.hd) {
+    case 64: weights_tile_kernel<DT, 64><<<grid, kBlockThreads, 0, stream>>>(a); break;
+    case 96: weights_tile_kernel<DT, 96><<<grid, kBlockThreads, 0, stream>>>(a); break;
+    case 128: weights_tile_kernel<DT, 128><<<grid, kBlockThreads, 0, stream>>>(a); break;
+    case 192: weights_tile_kernel<DT, 192><<<grid, kBlockThreads, 0, stream>>>(a); break;
+    default: weights_tile_kernel<DT, 256><<<grid, kBlockThreads, 0, stream>>>(a); break;
+  }
+  return hipGetLastError();
+}
+
+// Whether 16 bytes of a query row can be read at a time.
+bool queries_fit(const CacheAttnCall& c) {
+  return ((reinterpret_cast<uint64_t>(c.query) | 2 * c.query_row_stride | 2 * c.query_head_stride) & 15) == 0;
+}
+
+template <int DT>
+hipError_t launch(const CacheAttnCall& c, CacheArgs a, hipStream_t stream) {
   const int64_t room = c.max_blocks * c.block_size;
   int64_t longest = c.longest < room ? c.longest : room;
   if (longest > c.weight_tokens) longest = c.weight_tokens;
-  int64_t groups = (longest + kBlockThreads - 1) / kBlockThreads;
+  const bool tiles = DT != kLinF32 && tiles_fit(c) && queries_fit(c);
+  int64_t share = kBlockThreads;
+  if (tiles) {
+    const int64_t seq_rows = c.starts == nullptr ? 1 : (c.rows + c.batch - 1) / c.batch;
+    const bool many = seq_rows * (c.heads / c.kv_heads) > 16 * (kManyTiles - 1);
+    a.parts = many ? kWavesPerBlock : 1;
+    share = many ? kTilePlaces : kTilePlaces * kWavesPerBlock;
+  }
+  int64_t groups = (longest + share - 1) / share;
   groups = groups < 1 ? 1 : groups < 4096 ? groups : 4096;
-  weights_any_kernel<DT><<<dim3(groups, c.batch, c.kv_heads), kBlockThreads, 0, stream>>>(a);
+  const dim3 grid(groups, c.batch, c.kv_heads);
+  if constexpr (DT != kLinF32)
+    if (tiles) return launch_tiles<DT>(a, grid, stream);
+  weights_any_kernel<DT><<<grid, kBlockThreads, 0, stream>>>(a);
   return hipGetLastError();
 }
 
