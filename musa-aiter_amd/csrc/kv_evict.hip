@@ -1,8 +1,7 @@
 // Eviction from a paged cache by gathered attention weight: kv_evict_paged_tokens.
 //
 // Two launches.  The first decides, one workgroup per line (a layer, row and kv head): a radix select finds the weight
-// of the last token that stays, a pass in order marks the tokens (one bit each, in the workspace) and moves their
-// weights.  The second moves the tokens' values.  A token's new position is never behind its old one, so a wave that
+// of the lightest token that stays, then the tokens are marked (one bit each, in the workspace) and their weights moved.  The second moves the tokens' values.  A token's new position is never behind its old one, so a wave that
 // goes through a line in order, with a step's loads ahead of its stores, can move it in place; lines and head
 // dimensions are independent of each other.
 #include "kv_cache_attention.h"
@@ -15,6 +14,7 @@ using attn::int_at;
 struct EvictArgs {
   EvictCall c;
   int64_t words;  // of 64 positions, of a line
+  int64_t lines;
 };
 
 // Tokens that a line keeps, or -1 where it stays as it is.
@@ -22,7 +22,11 @@ __device__ __forceinline__ int64_t* line_keep(const EvictArgs& a, int64_t line) 
   return static_cast<int64_t*>(a.c.workspace) + line;
 }
 __device__ __forceinline__ uint64_t* line_bits(const EvictArgs& a, int64_t line) {
-  return static_cast<uint64_t*>(a.c.workspace) + a.c.layers * a.c.batch * a.c.kv_heads + line * a.words;
+  return static_cast<uint64_t*>(a.c.workspace) + a.lines + line * a.words;
+}
+// The weights of the tokens that stay, until all of the old ones are read.
+__device__ __forceinline__ float* line_weights(const EvictArgs& a, int64_t line) {
+  return reinterpret_cast<float*>(line_bits(a, a.lines)) + line * a.words * kWave;
 }
 
 __device__ __forceinline__ int64_t row_block(const EvictCall& c, int64_t row, int64_t token) {
@@ -36,33 +40,54 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u ^ ((u >> 31) != 0 ? 0xFFFFFFFFu : 0x80000000u);
 }
 
-constexpr int kDigit = 8;
-constexpr int kBins = 1 << kDigit;
-static_assert(kBins == kBlockThreads, "a thread per bin");
+// The deciding launch: 16 waves of a workgroup take a 16th of the line each, 64 positions at a time; the first kHeld
+// steps stay in registers (lines of up to 8192 tokens are read once).  Three digits of 11, 11 and 10 bits: 2048 bins, two a
+// thread.
+constexpr int kSelectWaves = 16;
+constexpr int kSelectThreads = kSelectWaves * kWave;
+constexpr int kHeld = 8;
+constexpr int kBins = 2 * kSelectThreads;
 
-__global__ __launch_bounds__(kBlockThreads) void evict_select_kernel(const EvictArgs a) {
+__global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const EvictArgs a) {
   const EvictCall& c = a.c;
   const int64_t line = blockIdx.x;
   const int64_t head = line % c.kv_heads, row = line / c.kv_heads % c.batch, layer = line / c.kv_heads / c.batch;
   const int lane = lane_id(), wave = wave_in_block();
   __shared__ int32_t bad;
-  __shared__ uint32_t bins[kWavesPerBlock][kBins];
-  __shared__ uint32_t above[kBins + 1];
+  __shared__ uint32_t bins[kBins];
+  __shared__ uint32_t wave_of[kSelectWaves][2];
   __shared__ uint32_t digit_found, need_left;
-  __shared__ uint32_t more_of[kWavesPerBlock], same_of[kWavesPerBlock];
 
   const int64_t said = int_at(c.lens, row, c.wide_lens), asked = int_at(c.keep, row, c.wide_keep);
   const int64_t len = said < 0 ? 0 : said, room = c.max_blocks * c.block_size;
-  if (threadIdx.x == 0) bad = asked < 0 || asked >= len || len > room ? 1 : 0;
-  __syncthreads();
-  if (bad == 0) {
-    bool miss = false;
-    for (int64_t p = threadIdx.x; p * c.block_size < len; p += kBlockThreads) {
+  float* weights = c.weights + layer * c.weight_layer_stride + row * c.weight_row_stride + head * c.weight_head_stride;
+  // A wave's positions: [seg * wave, seg * (wave + 1)), at most 2^29 in a line.
+  const int32_t used = static_cast<int32_t>(len < room ? len : room);
+  const int32_t seg = ((used + kSelectThreads - 1) / kSelectThreads) * kWave;
+  const int32_t p0 = seg * wave + lane, steps = min(seg, max(used - seg * wave, 0) + kWave - 1) / kWave;
+  auto weight_at = [&](int32_t p) { return p < used && p < c.weight_tokens ? weights[p] : 0.0f; };
+  float held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = i < steps ? weight_at(p0 + i * kWave) : 0.0f;
+  // f(position, weight) for all steps of the wave, in order.
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (i < steps) f(p0 + i * kWave, held[i]);
+#pragma unroll 4
+    for (int32_t i = kHeld; i < steps; ++i) f(p0 + i * kWave, weight_at(p0 + i * kWave));
+  };
+
+  bool miss = asked < 0 || asked >= len || len > room;
+  if (!miss) {
+    for (int64_t p = threadIdx.x; p * c.block_size < len; p += kSelectThreads) {
       const int64_t blk = int_at(c.tables, row * c.table_stride + p, c.wide_tables);
       miss |= blk < 0 || blk >= c.num_blocks || (c.refs != nullptr && int_at(c.refs, blk, c.wide_refs) > 1);
     }
-    if (miss) bad = 1;
   }
+  if (threadIdx.x == 0) bad = 0;
+  __syncthreads();
+  if (miss) bad = 1;
   __syncthreads();
   const bool stays = bad != 0;
   if (threadIdx.x == 0) {
@@ -71,82 +96,93 @@ __global__ __launch_bounds__(kBlockThreads) void evict_select_kernel(const Evict
   }
   if (stays) return;
 
-  const int64_t keep = asked;
-  const int64_t first = c.sinks < keep ? c.sinks : keep;
-  const int64_t recent = c.recent < keep - first ? c.recent : keep - first;
-  const int64_t from = first, to = len - recent;  // where the heaviest are looked for
-  float* weights = c.weights + layer * c.weight_layer_stride + row * c.weight_row_stride + head * c.weight_head_stride;
-  auto weight_at = [&](int64_t p) { return p < c.weight_tokens ? weights[p] : 0.0f; };
+  const int32_t keep = static_cast<int32_t>(asked);
+  const int32_t first = static_cast<int32_t>(c.sinks < keep ? c.sinks : keep);
+  const int32_t recent = static_cast<int32_t>(c.recent < keep - first ? c.recent : keep - first);
+  const int32_t from = first, to = used - recent;  // where the heaviest are looked for
 
   // The key of the lightest one that stays, digit by digit from the top, and how many of that key stay.
   uint32_t key = 0, need = static_cast<uint32_t>(keep - first - recent);
   const bool choose = need > 0;
-  for (int shift = 32 - kDigit; choose && shift >= 0; shift -= kDigit) {
-    for (int x = 0; x < kWavesPerBlock; ++x) bins[x][threadIdx.x] = 0;
+  int above_digit = 32;
+  for (int shift : {21, 10, 0}) {
+    if (!choose) break;
+    const int width = above_digit - shift;
+    bins[threadIdx.x] = bins[threadIdx.x + kSelectThreads] = 0;
     __syncthreads();
-    for (int64_t p = from + threadIdx.x; p < to; p += kBlockThreads) {
-      const uint32_t k = weight_key(weight_at(p));
-      if (shift + kDigit == 32 || k >> (shift + kDigit) == key >> (shift + kDigit))
-        atomicAdd(&bins[wave][k >> shift & (kBins - 1)], 1u);
+    each([&](int32_t p, float weight) {
+      const uint32_t k = weight_key(weight);
+      if (p >= from && p < to && (above_digit == 32 || k >> above_digit == key >> above_digit))
+        atomicAdd(&bins[k >> shift & ((1u << width) - 1)], 1u);
+    });
+    __syncthreads();
+    // Keys whose digit is at least that of the thread's two bins.
+    const uint32_t low = bins[2 * threadIdx.x], high = bins[2 * threadIdx.x + 1];
+    uint32_t upto = low + high;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const uint32_t y = __shfl_down(upto, o);
+      if (lane + o < kWave) upto += y;
     }
+    if (lane == 0) wave_of[wave][0] = upto;
     __syncthreads();
-    // above[t]: keys whose digit is t or more.
-    uint32_t mine = 0;
-    for (int x = 0; x < kWavesPerBlock; ++x) mine += bins[x][threadIdx.x];
-    above[threadIdx.x] = mine;
-    if (threadIdx.x == 0) above[kBins] = 0;
-    __syncthreads();
-    for (int o = 1; o < kBins; o <<= 1) {
-      const uint32_t add = threadIdx.x + o < kBins ? above[threadIdx.x + o] : 0;
-      __syncthreads();
-      above[threadIdx.x] += add;
-      __syncthreads();
-    }
-    const uint32_t next = above[threadIdx.x + 1];
-    if (above[threadIdx.x] >= need && next < need) {
-      digit_found = threadIdx.x;
-      need_left = need - next;
+    for (int x = wave + 1; x < kSelectWaves; ++x) upto += wave_of[x][0];
+    const uint32_t past_low = upto - low, past_high = past_low - high;
+    if (past_low >= need && past_high < need) {
+      digit_found = 2 * threadIdx.x + 1;
+      need_left = need - past_high;
+    } else if (upto >= need && past_low < need) {
+      digit_found = 2 * threadIdx.x;
+      need_left = need - past_low;
     }
     __syncthreads();
     key |= digit_found << shift;
     need = need_left;
-    __syncthreads();
+    above_digit = shift;
   }
 
-  // In order: the marks, and the weights to their new places.  `rank` tokens stay in front of a step, `same` of them
-  // with the key itself.
-  uint64_t* bits = line_bits(a, line);
-  int64_t rank = 0;
-  uint32_t same = 0;
-  for (int64_t base = 0; base < len; base += kBlockThreads) {
-    const int64_t p = base + threadIdx.x;
-    const float weight = p < len ? weight_at(p) : 0.0f;
+  // What stays: counted by each wave (lighter ones of the key itself only as far as they are needed, so both counts),
+  // then marked, with the weights on their way to their places.
+  auto kind = [&](int32_t p, float weight, uint64_t& sure, uint64_t& equal) {
     const uint32_t k = weight_key(weight);
-    const bool always = p < first || (p >= to && p < len), between = choose && p >= from && p < to;
-    const uint64_t equal = ballot(between && k == key);
-    if (lane == 0) same_of[wave] = __popcll(equal);
-    __syncthreads();
-    uint32_t in_front = same;
-    for (int x = 0; x < kWavesPerBlock; ++x) {
-      if (x < wave) in_front += same_of[x];
-      same += same_of[x];
-    }
-    in_front += __popcll(equal & ((uint64_t{1} << lane) - 1));
-    const bool stay = always || (between && (k > key || (k == key && in_front < need)));
-    const uint64_t mark = ballot(stay);
-    if (lane == 0) {
-      more_of[wave] = __popcll(mark);
-      if (base + wave * kWave < len) bits[(base >> 6) + wave] = mark;
-    }
-    __syncthreads();  // also: every weight of this step is read
-    int64_t dst = rank + __popcll(mark & ((uint64_t{1} << lane) - 1));
-    for (int x = 0; x < kWavesPerBlock; ++x) {
-      if (x < wave) dst += more_of[x];
-      rank += more_of[x];
-    }
-    if (stay && dst < c.weight_tokens) weights[dst] = weight;
+    const bool between = choose && p >= from && p < to;
+    equal = ballot(between && k == key);
+    sure = ballot(p < used && (p < from || p >= to || (between && k > key)));
+  };
+  uint32_t sure_count = 0, equal_count = 0;
+  each([&](int32_t p, float weight) {
+    uint64_t sure, equal;
+    kind(p, weight, sure, equal);
+    sure_count += __popcll(sure);
+    equal_count += __popcll(equal);
+  });
+  __syncthreads();
+  if (lane == 0) {
+    wave_of[wave][0] = sure_count;
+    wave_of[wave][1] = equal_count;
   }
-  for (int64_t p = keep + threadIdx.x; p < len && p < c.weight_tokens; p += kBlockThreads) weights[p] = 0.0f;
+  __syncthreads();
+  uint32_t rank = 0, same = 0;
+  for (int x = 0; x < wave; ++x) {
+    rank += wave_of[x][0];
+    same += wave_of[x][1];
+  }
+  rank += min(same, need);
+  uint64_t* bits = line_bits(a, line);
+  float* moved = line_weights(a, line);
+  const uint64_t lower = (uint64_t{1} << lane) - 1;
+  each([&](int32_t p, float weight) {
+    uint64_t sure, equal;
+    kind(p, weight, sure, equal);
+    const uint64_t mark = sure | ballot((equal >> lane & 1) != 0 && same + __popcll(equal & lower) < need);
+    if (lane == 0) bits[p >> 6] = mark;
+    if ((mark >> lane & 1) != 0) moved[rank + __popcll(mark & lower)] = weight;
+    rank += __popcll(mark);
+    same += __popcll(equal);
+  });
+  __syncthreads();
+  const int32_t last = static_cast<int32_t>(used < c.weight_tokens ? used : c.weight_tokens);
+  for (int32_t p = threadIdx.x; p < last; p += kSelectThreads) weights[p] = p < keep ? moved[p] : 0.0f;
 }
 
 // ----- moving values, any element size and block size ----------------------------------------------
@@ -172,7 +208,7 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_any_kernel(const Evi
     return base + blk * c.cache_block_stride[kv] + token % bs * ELT;
   };
   int64_t rank = 0;
-  for (int64_t word = 0; rank < keep; ++word) {
+  for (int64_t word = 0; rank < keep && word < a.words; ++word) {
     const uint64_t mark = static_cast<uint64_t>(uniform64(static_cast<int64_t>(bits[word])));
     const int64_t src = word * kWave + lane_id();
     const int64_t dst = rank + __popcll(mark & ((uint64_t{1} << lane_id()) - 1));
@@ -190,28 +226,139 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_any_kernel(const Evi
   }
 }
 
+// ----- moving 16-bit values of blocks of multiples of 8 tokens ---------------------------------------
+// A wave takes 8 head dimensions of a line and goes through its tokens 64 at a time: 16 bytes a lane, whole pieces of
+// the blocks' rows, kAhead steps on their way.  What stays is put into a ring of 128 places per dim in LDS, and leaves
+// it 64 tokens at a time as 16 bytes a lane again.  Bound by the read of every block that keeps a token (lines of 128
+// bytes hold the same 16 tokens of four dims, so single tokens are no cheaper to read).
+constexpr int kAhead = 8;
+constexpr int kRing = 128;
+constexpr int kRingPitch = kRing + 8;
+constexpr int kEntries = 4096;  // of a table row, in LDS, and
+constexpr int kMarks = 1024;    // words of marks; further ones are read where they are used
+
+__global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictArgs a, const int log_pieces) {
+  const EvictCall& c = a.c;
+  const int64_t line = blockIdx.x;
+  const int kv = blockIdx.z, lane = lane_id(), wave = wave_in_block();
+  __shared__ __attribute__((aligned(16))) uint16_t rings[kWavesPerBlock][kMoveDims * kRingPitch + 8];
+  __shared__ int32_t entries[kEntries];
+  __shared__ uint64_t marks[kMarks];
+  const int64_t keep64 = uniform64(*line_keep(a, line));
+  if (keep64 <= 0) return;
+  const int32_t keep = static_cast<int32_t>(keep64), bs = static_cast<int32_t>(c.block_size);
+  const int64_t head = line % c.kv_heads, row = line / c.kv_heads % c.batch, layer = line / c.kv_heads / c.batch;
+  const int32_t len = static_cast<int32_t>(int_at(c.lens, row, c.wide_lens));
+  const int32_t steps = (len + kWave - 1) / kWave;
+  const uint64_t* bits = line_bits(a, line);
+  for (int64_t p = threadIdx.x; p < kEntries && p * bs < len; p += kBlockThreads)
+    entries[p] = static_cast<int32_t>(int_at(c.tables, row * c.table_stride + p, c.wide_tables));
+  for (int32_t p = threadIdx.x; p < kMarks && p < steps; p += kBlockThreads) marks[p] = bits[p];
+  __syncthreads();
+  const int32_t d0 = (blockIdx.y * kWavesPerBlock + wave) * kMoveDims;
+  if (d0 >= c.head_dim) return;
+  // Lane: dim and unit of 8 tokens, pieces of a row of a block next to each other.
+  const int dim = lane >> log_pieces & 7;
+  const int unit = (lane & ((1 << log_pieces) - 1)) | (lane >> (log_pieces + 3) << log_pieces);
+  const bool mine = d0 + dim < c.head_dim;
+  uint8_t* base = static_cast<uint8_t*>(c.cache[kv]) + layer * c.cache_layer_stride[kv];
+  const int64_t in_block = (head * c.head_dim + min(d0 + dim, static_cast<int32_t>(c.head_dim) - 1)) * bs * 2;
+  auto place = [&](int32_t token) {
+    const uint32_t column = static_cast<uint32_t>(token) / static_cast<uint32_t>(bs);
+    const int64_t blk = column < kEntries ? entries[column] : row_block(c, row, token);
+    return base + blk * c.cache_block_stride[kv] + in_block + (token - static_cast<int32_t>(column) * bs) * 2;
+  };
+  uint16_t* ring = rings[wave];
+  uint16_t* mine_ring = ring + dim * kRingPitch;
+  const uint32_t dump = kMoveDims * kRingPitch;  // where the values go that do not stay
+  auto mark_of = [&](int32_t step) {
+    if (step >= steps) return uint64_t{0};
+    return static_cast<uint64_t>(uniform64(static_cast<int64_t>(step < kMarks ? marks[step] : bits[step])));
+  };
+
+  // Units that keep nothing read the beginning of the line's first page, all lanes the same 16 bytes.
+  auto load = [&](int32_t step) {
+    const bool some = (mark_of(step) >> (8 * unit) & 0xFF) != 0;
+    return ld16_cached(some ? place(step * kWave + 8 * unit) : base);
+  };
+  u32x4 ahead[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) ahead[i] = load(i);
+  int32_t rank = 0, out = 0;  // tokens in the ring so far, and of them those that left it
+  for (int32_t step0 = 0; rank < keep && step0 < steps; step0 += kAhead) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int32_t step = step0 + i;
+      const uint64_t mark = mark_of(step);
+      const u32x4 values = ahead[i];
+      if (mark != 0) {
+        const uint32_t stay = static_cast<uint32_t>(mark >> (8 * unit)) & 0xFFu;
+        uint32_t at = rank + __popcll(mark & ((uint64_t{1} << (8 * unit)) - 1));
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const uint32_t bit = stay >> t & 1u;
+          const uint32_t to = bit != 0 ? dim * kRingPitch + (at & (kRing - 1)) : dump;
+          ring[to] = static_cast<uint16_t>(elem16(values, t));
+          at += bit;
+        }
+        rank += __popcll(mark);
+        __builtin_amdgcn_wave_barrier();
+        if (rank - out >= kWave) {
+          const u32x4 full = *reinterpret_cast<const u32x4*>(mine_ring + (out & (kRing - 1)) + 8 * unit);
+          if (mine) st16_cached(place(out + 8 * unit), full);
+          out += kWave;
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
+      ahead[i] = load(step + kAhead);
+    }
+  }
+  const int32_t left = keep - out - 8 * unit;  // of this lane's last unit
+  if (mine && left > 0) {
+    const uint16_t* from = mine_ring + (out & (kRing - 1)) + 8 * unit;
+    uint8_t* to = place(out + 8 * unit);
+    if (left >= 8) st16_cached(to, *reinterpret_cast<const u32x4*>(from));
+    else
+      for (int t = 0; t < left; ++t)
+        reinterpret_cast<KVHIP_GLOBAL uint16_t*>(reinterpret_cast<uint64_t>(to))[t] = from[t];
+  }
+}
+
+// log2 of the 16-byte pieces of a block's row that neighbouring lanes take, or -1 where the kernel does not fit.
+int move_pieces(const EvictCall& c) {
+  if (c.element_bytes != 2 || c.block_size % 8 != 0) return -1;
+  for (int kv = 0; kv < 2; ++kv)
+    if (((reinterpret_cast<uint64_t>(c.cache[kv]) | c.cache_layer_stride[kv] | c.cache_block_stride[kv]) & 15) != 0) return -1;
+  const int64_t pieces = c.block_size / 8;
+  return pieces % 8 == 0 ? 3 : pieces == 4 ? 2 : pieces == 2 ? 1 : 0;
+}
+
 EvictArgs evict_args(const EvictCall& c) {
   EvictArgs a{};
   a.c = c;
   a.words = (c.max_blocks * c.block_size + kWave - 1) / kWave;
+  a.lines = c.layers * c.batch * c.kv_heads;
   return a;
 }
 
 }  // namespace
 
 int64_t evict_workspace(const EvictCall& c) {
-  return c.layers * c.batch * c.kv_heads * (evict_args(c).words + 1) * 8;
+  const EvictArgs a = evict_args(c);
+  return a.lines * (8 + a.words * (8 + kWave * 4));
 }
 
 hipError_t launch_evict(const EvictCall& c, hipStream_t stream) {
   const EvictArgs a = evict_args(c);
   const int64_t lines = c.layers * c.batch * c.kv_heads;
-  evict_select_kernel<<<dim3(lines), kBlockThreads, 0, stream>>>(a);
+  evict_select_kernel<<<dim3(lines), kSelectThreads, 0, stream>>>(a);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   const int64_t slices = (c.head_dim + kMoveDims * kWavesPerBlock - 1) / (kMoveDims * kWavesPerBlock);
   const dim3 grid(lines, slices, 2);
-  if (c.element_bytes == 1) evict_move_any_kernel<1><<<grid, kBlockThreads, 0, stream>>>(a);
+  const int pieces = move_pieces(c);
+  if (pieces >= 0) evict_move_kernel<<<grid, kBlockThreads, 0, stream>>>(a, pieces);
+  else if (c.element_bytes == 1) evict_move_any_kernel<1><<<grid, kBlockThreads, 0, stream>>>(a);
   else if (c.element_bytes == 2) evict_move_any_kernel<2><<<grid, kBlockThreads, 0, stream>>>(a);
   else evict_move_any_kernel<4><<<grid, kBlockThreads, 0, stream>>>(a);
   return hipGetLastError();
