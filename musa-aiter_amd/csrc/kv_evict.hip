@@ -228,95 +228,120 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_any_kernel(const Evi
 
 // ----- moving 16-bit values of blocks of multiples of 8 tokens ---------------------------------------
 // A wave takes 8 head dimensions of a line and goes through its tokens 64 at a time: 16 bytes a lane, whole pieces of
-// the blocks' rows, kAhead steps on their way.  What stays is put into a ring of 128 places per dim in LDS, and leaves
-// it 64 tokens at a time as 16 bytes a lane again.  Bound by the read of every block that keeps a token (lines of 128
-// bytes hold the same 16 tokens of four dims, so single tokens are no cheaper to read).
+// the blocks' rows, kAhead steps on their way, the table entry of one more.  What stays is put behind one another in LDS,
+// and leaves it 64 tokens at a time as 16 bytes a lane again.  Bound by the read of every block that keeps a token (lines
+// of 128 bytes hold the same 16 tokens of four dims, so single tokens are no cheaper to read).
 constexpr int kAhead = 8;
-constexpr int kRing = 128;
-constexpr int kRingPitch = kRing + 8;
-constexpr int kEntries = 4096;  // of a table row, in LDS, and
-constexpr int kMarks = 1024;    // words of marks; further ones are read where they are used
+constexpr int kHoldPitch = 2 * kWave + 8;  // tokens of a dim in LDS: less than 64, and 64 more
+// Bytes of LDS for a table row and a line's marks.  Where they need more, each step reads its own from memory, which
+// waits for all loads that are on their way.
+constexpr int64_t kMostStaged = 96 * 1024;
 
-__global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictArgs a, const int log_pieces) {
+struct MoveShape {
+  int log_pieces;  // neighbouring lanes take this many pieces of 16 bytes of a block's row (log2)
+  int log_block;   // log2(block_size), or -1
+};
+
+template <bool STAGED>
+__global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictArgs a, const MoveShape shape) {
   const EvictCall& c = a.c;
   const int64_t line = blockIdx.x;
   const int kv = blockIdx.z, lane = lane_id(), wave = wave_in_block();
-  __shared__ __attribute__((aligned(16))) uint16_t rings[kWavesPerBlock][kMoveDims * kRingPitch + 8];
-  __shared__ int32_t entries[kEntries];
-  __shared__ uint64_t marks[kMarks];
+  __shared__ __attribute__((aligned(16))) uint16_t holds[kWavesPerBlock][kMoveDims * kHoldPitch + 8];
+  extern __shared__ uint64_t marks[];  // the line's words, then the row's entries
+  int32_t* entries = reinterpret_cast<int32_t*>(marks + a.words);
   const int64_t keep64 = uniform64(*line_keep(a, line));
   if (keep64 <= 0) return;
   const int32_t keep = static_cast<int32_t>(keep64), bs = static_cast<int32_t>(c.block_size);
   const int64_t head = line % c.kv_heads, row = line / c.kv_heads % c.batch, layer = line / c.kv_heads / c.batch;
-  const int32_t len = static_cast<int32_t>(int_at(c.lens, row, c.wide_lens));
+  const int32_t len = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(int_at(c.lens, row, c.wide_lens)));
   const int32_t steps = (len + kWave - 1) / kWave;
   const uint64_t* bits = line_bits(a, line);
-  for (int64_t p = threadIdx.x; p < kEntries && p * bs < len; p += kBlockThreads)
-    entries[p] = static_cast<int32_t>(int_at(c.tables, row * c.table_stride + p, c.wide_tables));
-  for (int32_t p = threadIdx.x; p < kMarks && p < steps; p += kBlockThreads) marks[p] = bits[p];
-  __syncthreads();
+  if constexpr (STAGED) {
+    for (int64_t p = threadIdx.x; p * bs < len; p += kBlockThreads)
+      entries[p] = static_cast<int32_t>(int_at(c.tables, row * c.table_stride + p, c.wide_tables));
+    for (int32_t p = threadIdx.x; p < steps; p += kBlockThreads) marks[p] = bits[p];
+    __syncthreads();
+  }
   const int32_t d0 = (blockIdx.y * kWavesPerBlock + wave) * kMoveDims;
   if (d0 >= c.head_dim) return;
   // Lane: dim and unit of 8 tokens, pieces of a row of a block next to each other.
-  const int dim = lane >> log_pieces & 7;
-  const int unit = (lane & ((1 << log_pieces) - 1)) | (lane >> (log_pieces + 3) << log_pieces);
+  const int dim = lane >> shape.log_pieces & 7;
+  const int unit8 = 8 * ((lane & ((1 << shape.log_pieces) - 1)) | (lane >> (shape.log_pieces + 3) << shape.log_pieces));
   const bool mine = d0 + dim < c.head_dim;
-  uint8_t* base = static_cast<uint8_t*>(c.cache[kv]) + layer * c.cache_layer_stride[kv];
-  const int64_t in_block = (head * c.head_dim + min(d0 + dim, static_cast<int32_t>(c.head_dim) - 1)) * bs * 2;
-  auto place = [&](int32_t token) {
-    const uint32_t column = static_cast<uint32_t>(token) / static_cast<uint32_t>(bs);
-    const int64_t blk = column < kEntries ? entries[column] : row_block(c, row, token);
-    return base + blk * c.cache_block_stride[kv] + in_block + (token - static_cast<int32_t>(column) * bs) * 2;
+  const uint8_t* plane = static_cast<const uint8_t*>(c.cache[kv]) + layer * c.cache_layer_stride[kv];
+  const uint8_t* base = plane + (head * c.head_dim + min(d0 + dim, static_cast<int32_t>(c.head_dim) - 1)) * bs * 2;
+  const uint32_t block_bytes = static_cast<uint32_t>(c.cache_block_stride[kv]);
+  auto column_of = [&](int32_t token) {
+    return shape.log_block >= 0 ? token >> shape.log_block : static_cast<int32_t>(static_cast<uint32_t>(token) / static_cast<uint32_t>(bs));
   };
-  uint16_t* ring = rings[wave];
-  uint16_t* mine_ring = ring + dim * kRingPitch;
-  const uint32_t dump = kMoveDims * kRingPitch;  // where the values go that do not stay
+  auto entry_of = [&](int32_t token) -> uint32_t {  // of a position below len
+    if constexpr (STAGED) return entries[column_of(token)];
+    else return static_cast<uint32_t>(row_block(c, row, token));
+  };
+  auto address = [&](uint32_t entry, int32_t token) {
+    const int32_t place = shape.log_block >= 0 ? token & (bs - 1) : token - column_of(token) * bs;
+    return base + static_cast<uint64_t>(entry) * block_bytes + place * 2;
+  };
   auto mark_of = [&](int32_t step) {
-    if (step >= steps) return uint64_t{0};
-    return static_cast<uint64_t>(uniform64(static_cast<int64_t>(step < kMarks ? marks[step] : bits[step])));
+    if constexpr (STAGED) return marks[min(step, steps - 1)];
+    else return bits[min(step, steps - 1)];
   };
 
-  // Units that keep nothing read the beginning of the line's first page, all lanes the same 16 bytes.
-  auto load = [&](int32_t step) {
-    const bool some = (mark_of(step) >> (8 * unit) & 0xFF) != 0;
-    return ld16_cached(some ? place(step * kWave + 8 * unit) : base);
-  };
+  uint16_t* hold = holds[wave];
+  const uint32_t mine_hold = dim * kHoldPitch;
+  const uint32_t dump = kMoveDims * kHoldPitch;  // where the values go that do not stay
+  const uint64_t below = (uint64_t{1} << unit8) - 1;
+  uint64_t mark_ahead[kAhead];
   u32x4 ahead[kAhead];
+  uint64_t next_mark = mark_of(0);
+  uint32_t next_entry = entry_of(min(unit8, len - 1));
+  // Step `step` on its way, and the mark and entry of the one behind it.  Units that keep nothing read the beginning of
+  // the layer, all lanes the same 16 bytes.
+  auto issue = [&](int32_t step, uint64_t& mark, u32x4& values) {
+    mark = step < steps ? static_cast<uint64_t>(uniform64(static_cast<int64_t>(next_mark))) : 0;
+    const bool some = (mark >> unit8 & 0xFF) != 0;
+    values = ld16_cached(some ? address(next_entry, step * kWave + unit8) : plane);
+    next_mark = mark_of(step + 1);
+    next_entry = entry_of(min((step + 1) * kWave + unit8, len - 1));
+  };
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i) ahead[i] = load(i);
-  int32_t rank = 0, out = 0;  // tokens in the ring so far, and of them those that left it
-  for (int32_t step0 = 0; rank < keep && step0 < steps; step0 += kAhead) {
+  for (int i = 0; i < kAhead; ++i) issue(i, mark_ahead[i], ahead[i]);
+  int32_t level = 0, out = 0;  // tokens in LDS, and those that left it
+  uint32_t out_entry = entry_of(min(unit8, len - 1));
+  for (int32_t step0 = 0; out + level < keep && step0 < steps; step0 += kAhead) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int32_t step = step0 + i;
-      const uint64_t mark = mark_of(step);
-      const u32x4 values = ahead[i];
+      const uint64_t mark = mark_ahead[i];
       if (mark != 0) {
-        const uint32_t stay = static_cast<uint32_t>(mark >> (8 * unit)) & 0xFFu;
-        uint32_t at = rank + __popcll(mark & ((uint64_t{1} << (8 * unit)) - 1));
+        const uint32_t stay = static_cast<uint32_t>(mark >> unit8) & 0xFFu;
+        uint32_t at = mine_hold + level + __popcll(mark & below);
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
           const uint32_t bit = stay >> t & 1u;
-          const uint32_t to = bit != 0 ? dim * kRingPitch + (at & (kRing - 1)) : dump;
-          ring[to] = static_cast<uint16_t>(elem16(values, t));
+          hold[bit != 0 ? at : dump] = static_cast<uint16_t>(elem16(ahead[i], t));
           at += bit;
         }
-        rank += __popcll(mark);
+        level += __popcll(mark);
         __builtin_amdgcn_wave_barrier();
-        if (rank - out >= kWave) {
-          const u32x4 full = *reinterpret_cast<const u32x4*>(mine_ring + (out & (kRing - 1)) + 8 * unit);
-          if (mine) st16_cached(place(out + 8 * unit), full);
+        if (level >= kWave) {
+          u32x4* from = reinterpret_cast<u32x4*>(hold + mine_hold + unit8);
+          const u32x4 full = from[0], rest = from[kWave / 8];
+          if (mine) st16_cached(const_cast<uint8_t*>(address(out_entry, out + unit8)), full);
+          from[0] = rest;
           out += kWave;
+          level -= kWave;
+          out_entry = entry_of(min(out + unit8, len - 1));
           __builtin_amdgcn_wave_barrier();
         }
       }
-      ahead[i] = load(step + kAhead);
+      issue(step0 + i + kAhead, mark_ahead[i], ahead[i]);
     }
   }
-  const int32_t left = keep - out - 8 * unit;  // of this lane's last unit
+  const int32_t left = keep - out - unit8;  // of this lane's last unit
   if (mine && left > 0) {
-    const uint16_t* from = mine_ring + (out & (kRing - 1)) + 8 * unit;
-    uint8_t* to = place(out + 8 * unit);
+    const uint16_t* from = hold + mine_hold + unit8;
+    uint8_t* to = const_cast<uint8_t*>(address(out_entry, out + unit8));
     if (left >= 8) st16_cached(to, *reinterpret_cast<const u32x4*>(from));
     else
       for (int t = 0; t < left; ++t)
@@ -324,13 +349,17 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictAr
   }
 }
 
-// log2 of the 16-byte pieces of a block's row that neighbouring lanes take, or -1 where the kernel does not fit.
-int move_pieces(const EvictCall& c) {
-  if (c.element_bytes != 2 || c.block_size % 8 != 0) return -1;
+// Whether evict_move_kernel takes the caches, and how.
+bool move_fits(const EvictCall& c, MoveShape& shape) {
+  if (c.element_bytes != 2 || c.block_size % 8 != 0) return false;
   for (int kv = 0; kv < 2; ++kv)
-    if (((reinterpret_cast<uint64_t>(c.cache[kv]) | c.cache_layer_stride[kv] | c.cache_block_stride[kv]) & 15) != 0) return -1;
+    if (((reinterpret_cast<uint64_t>(c.cache[kv]) | c.cache_layer_stride[kv] | c.cache_block_stride[kv]) & 15) != 0 ||
+        c.cache_block_stride[kv] < 0 || c.cache_block_stride[kv] >= int64_t{1} << 32)
+      return false;
   const int64_t pieces = c.block_size / 8;
-  return pieces % 8 == 0 ? 3 : pieces == 4 ? 2 : pieces == 2 ? 1 : 0;
+  shape.log_pieces = pieces % 8 == 0 ? 3 : pieces == 4 ? 2 : pieces == 2 ? 1 : 0;
+  shape.log_block = (c.block_size & (c.block_size - 1)) == 0 ? __builtin_ctzll(c.block_size) : -1;
+  return true;
 }
 
 EvictArgs evict_args(const EvictCall& c) {
@@ -356,9 +385,12 @@ hipError_t launch_evict(const EvictCall& c, hipStream_t stream) {
   if (err != hipSuccess) return err;
   const int64_t slices = (c.head_dim + kMoveDims * kWavesPerBlock - 1) / (kMoveDims * kWavesPerBlock);
   const dim3 grid(lines, slices, 2);
-  const int pieces = move_pieces(c);
-  if (pieces >= 0) evict_move_kernel<<<grid, kBlockThreads, 0, stream>>>(a, pieces);
-  else if (c.element_bytes == 1) evict_move_any_kernel<1><<<grid, kBlockThreads, 0, stream>>>(a);
+  MoveShape shape{};
+  const int64_t staged = a.words * 8 + c.max_blocks * 4;
+  if (move_fits(c, shape)) {
+    if (staged <= kMostStaged) evict_move_kernel<true><<<grid, kBlockThreads, staged, stream>>>(a, shape);
+    else evict_move_kernel<false><<<grid, kBlockThreads, 0, stream>>>(a, shape);
+  } else if (c.element_bytes == 1) evict_move_any_kernel<1><<<grid, kBlockThreads, 0, stream>>>(a);
   else if (c.element_bytes == 2) evict_move_any_kernel<2><<<grid, kBlockThreads, 0, stream>>>(a);
   else evict_move_any_kernel<4><<<grid, kBlockThreads, 0, stream>>>(a);
   return hipGetLastError();
