@@ -65,17 +65,28 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   const int32_t used = static_cast<int32_t>(len < room ? len : room);
   const int32_t seg = ((used + kSelectThreads - 1) / kSelectThreads) * kWave;
   const int32_t p0 = seg * wave + lane, steps = min(seg, max(used - seg * wave, 0) + kWave - 1) / kWave;
-  auto weight_at = [&](int32_t p) { return p < used && p < c.weight_tokens ? weights[p] : 0.0f; };
+  const int32_t last = static_cast<int32_t>(used < c.weight_tokens ? used : c.weight_tokens);  // those with a weight
+  auto weight_at = [&](int32_t p) {
+    if (last == 0) return 0.0f;
+    const float weight = weights[min(p, last - 1)];
+    return p < last ? weight : 0.0f;
+  };
   float held[kHeld];
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) held[i] = i < steps ? weight_at(p0 + i * kWave) : 0.0f;
+  for (int i = 0; i < kHeld; ++i) held[i] = weight_at(p0 + i * kWave);
   // f(position, weight) for all steps of the wave, in order.
   auto each = [&](auto f) {
 #pragma unroll
     for (int i = 0; i < kHeld; ++i)
       if (i < steps) f(p0 + i * kWave, held[i]);
-#pragma unroll 4
-    for (int32_t i = kHeld; i < steps; ++i) f(p0 + i * kWave, weight_at(p0 + i * kWave));
+    for (int32_t j = kHeld; j < steps; j += kHeld) {
+      float more[kHeld];
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) more[i] = weight_at(p0 + (j + i) * kWave);
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i)
+        if (j + i < steps) f(p0 + (j + i) * kWave, more[i]);
+    }
   };
 
   bool miss = asked < 0 || asked >= len || len > room;
@@ -181,7 +192,6 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
     same += __popcll(equal);
   });
   __syncthreads();
-  const int32_t last = static_cast<int32_t>(used < c.weight_tokens ? used : c.weight_tokens);
   for (int32_t p = threadIdx.x; p < last; p += kSelectThreads) weights[p] = p < keep ? moved[p] : 0.0f;
 }
 
@@ -227,27 +237,33 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_any_kernel(const Evi
 }
 
 // ----- moving 16-bit values of blocks of multiples of 8 tokens ---------------------------------------
-// A wave takes 8 head dimensions of a line and goes through its tokens 64 at a time: 16 bytes a lane, whole pieces of
-// the blocks' rows, kAhead steps on their way, the table entry of one more.  What stays is put behind one another in LDS,
-// and leaves it 64 tokens at a time as 16 bytes a lane again.  Bound by the read of every block that keeps a token (lines
+// A wave takes DIMS head dimensions of a line and goes through its tokens 512 / DIMS at a time: 16 bytes a lane, whole
+// pieces of the blocks' rows, kAhead steps on their way, the table entry of one more.  What stays is put behind one
+// another in LDS, and leaves it as many tokens at a time as 16 bytes a lane again.  Bound by the read of every block that keeps a token (lines
 // of 128 bytes hold the same 16 tokens of four dims, so single tokens are no cheaper to read).
 constexpr int kAhead = 8;
-constexpr int kHoldPitch = 2 * kWave + 8;  // tokens of a dim in LDS: less than 64, and 64 more
+template <int DIMS>
+constexpr int kStepTokens = 512 / DIMS;
+template <int DIMS>
+constexpr int kHoldPitch = 2 * kStepTokens<DIMS> + 8;  // tokens of a dim in LDS: less than a step's, and a step's more
 // Bytes of LDS for a table row and a line's marks.  Where they need more, each step reads its own from memory, which
 // waits for all loads that are on their way.
 constexpr int64_t kMostStaged = 96 * 1024;
+
+constexpr int64_t kFewWaves = 4096;  // of one of the two caches
 
 struct MoveShape {
   int log_pieces;  // neighbouring lanes take this many pieces of 16 bytes of a block's row (log2)
   int log_block;   // log2(block_size), or -1
 };
 
-template <bool STAGED>
+template <bool STAGED, int DIMS>
 __global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictArgs a, const MoveShape shape) {
+  constexpr int kTokens = kStepTokens<DIMS>, kWords = kTokens / kWave, kPitch = kHoldPitch<DIMS>;
   const EvictCall& c = a.c;
   const int64_t line = blockIdx.x;
   const int kv = blockIdx.z, lane = lane_id(), wave = wave_in_block();
-  __shared__ __attribute__((aligned(16))) uint16_t holds[kWavesPerBlock][kMoveDims * kHoldPitch + 8];
+  __shared__ __attribute__((aligned(16))) uint16_t holds[kWavesPerBlock][DIMS * kPitch + 8];
   extern __shared__ uint64_t marks[];  // the line's words, then the row's entries
   int32_t* entries = reinterpret_cast<int32_t*>(marks + a.words);
   const int64_t keep64 = uniform64(*line_keep(a, line));
@@ -255,19 +271,21 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictAr
   const int32_t keep = static_cast<int32_t>(keep64), bs = static_cast<int32_t>(c.block_size);
   const int64_t head = line % c.kv_heads, row = line / c.kv_heads % c.batch, layer = line / c.kv_heads / c.batch;
   const int32_t len = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(int_at(c.lens, row, c.wide_lens)));
-  const int32_t steps = (len + kWave - 1) / kWave;
+  const int32_t words = (len + kWave - 1) / kWave, steps = (len + kTokens - 1) / kTokens;
   const uint64_t* bits = line_bits(a, line);
   if constexpr (STAGED) {
     for (int64_t p = threadIdx.x; p * bs < len; p += kBlockThreads)
       entries[p] = static_cast<int32_t>(int_at(c.tables, row * c.table_stride + p, c.wide_tables));
-    for (int32_t p = threadIdx.x; p < steps; p += kBlockThreads) marks[p] = bits[p];
+    for (int32_t p = threadIdx.x; p < words; p += kBlockThreads) marks[p] = bits[p];
     __syncthreads();
   }
-  const int32_t d0 = (blockIdx.y * kWavesPerBlock + wave) * kMoveDims;
+  const int32_t d0 = (blockIdx.y * kWavesPerBlock + wave) * DIMS;
   if (d0 >= c.head_dim) return;
   // Lane: dim and unit of 8 tokens, pieces of a row of a block next to each other.
-  const int dim = lane >> shape.log_pieces & 7;
-  const int unit8 = 8 * ((lane & ((1 << shape.log_pieces) - 1)) | (lane >> (shape.log_pieces + 3) << shape.log_pieces));
+  constexpr int kLogDims = __builtin_ctz(DIMS);
+  const int dim = lane >> shape.log_pieces & (DIMS - 1);
+  const int unit8 = 8 * ((lane & ((1 << shape.log_pieces) - 1)) |
+                         (lane >> (shape.log_pieces + kLogDims) << shape.log_pieces));
   const bool mine = d0 + dim < c.head_dim;
   const uint8_t* plane = static_cast<const uint8_t*>(c.cache[kv]) + layer * c.cache_layer_stride[kv];
   const uint8_t* base = plane + (head * c.head_dim + min(d0 + dim, static_cast<int32_t>(c.head_dim) - 1)) * bs * 2;
@@ -283,27 +301,41 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictAr
     const int32_t place = shape.log_block >= 0 ? token & (bs - 1) : token - column_of(token) * bs;
     return base + static_cast<uint64_t>(entry) * block_bytes + place * 2;
   };
-  auto mark_of = [&](int32_t step) {
-    if constexpr (STAGED) return marks[min(step, steps - 1)];
-    else return bits[min(step, steps - 1)];
+  auto mark_of = [&](int32_t word) {
+    if constexpr (STAGED) return marks[min(word, words - 1)];
+    else return bits[min(word, words - 1)];
   };
 
   uint16_t* hold = holds[wave];
-  const uint32_t mine_hold = dim * kHoldPitch;
-  const uint32_t dump = kMoveDims * kHoldPitch;  // where the values go that do not stay
-  const uint64_t below = (uint64_t{1} << unit8) - 1;
-  uint64_t mark_ahead[kAhead];
+  const uint32_t mine_hold = dim * kPitch;
+  const uint32_t dump = DIMS * kPitch;  // where the values go that do not stay
+  const int bit0 = unit8 % kWave, my_word = unit8 / kWave;
+  const uint64_t below = (uint64_t{1} << bit0) - 1;
+  struct Marks {
+    uint64_t of[kWords];
+  };
+  Marks mark_ahead[kAhead], next_mark;
   u32x4 ahead[kAhead];
-  uint64_t next_mark = mark_of(0);
+#pragma unroll
+  for (int k = 0; k < kWords; ++k) next_mark.of[k] = mark_of(k);
   uint32_t next_entry = entry_of(min(unit8, len - 1));
-  // Step `step` on its way, and the mark and entry of the one behind it.  Units that keep nothing read the beginning of
+  auto mine_of = [&](const Marks& m) {
+    uint64_t word = m.of[0];
+#pragma unroll
+    for (int k = 1; k < kWords; ++k) word = my_word == k ? m.of[k] : word;
+    return word;
+  };
+  // Step `step` on its way, and the marks and entry of the one behind it.  Units that keep nothing read the beginning of
   // the layer, all lanes the same 16 bytes.
-  auto issue = [&](int32_t step, uint64_t& mark, u32x4& values) {
-    mark = step < steps ? static_cast<uint64_t>(uniform64(static_cast<int64_t>(next_mark))) : 0;
-    const bool some = (mark >> unit8 & 0xFF) != 0;
-    values = ld16_cached(some ? address(next_entry, step * kWave + unit8) : plane);
-    next_mark = mark_of(step + 1);
-    next_entry = entry_of(min((step + 1) * kWave + unit8, len - 1));
+  auto issue = [&](int32_t step, Marks& mark, u32x4& values) {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k)
+      mark.of[k] = step * kWords + k < words ? static_cast<uint64_t>(uniform64(static_cast<int64_t>(next_mark.of[k]))) : 0;
+    const bool some = (mine_of(mark) >> bit0 & 0xFF) != 0;
+    values = ld16_cached(some ? address(next_entry, step * kTokens + unit8) : plane);
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) next_mark.of[k] = mark_of((step + 1) * kWords + k);
+    next_entry = entry_of(min((step + 1) * kTokens + unit8, len - 1));
   };
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) issue(i, mark_ahead[i], ahead[i]);
@@ -312,25 +344,33 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictAr
   for (int32_t step0 = 0; out + level < keep && step0 < steps; step0 += kAhead) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const uint64_t mark = mark_ahead[i];
-      if (mark != 0) {
-        const uint32_t stay = static_cast<uint32_t>(mark >> unit8) & 0xFFu;
-        uint32_t at = mine_hold + level + __popcll(mark & below);
+      const Marks& mark = mark_ahead[i];
+      uint64_t any = 0;
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) any |= mark.of[k];
+      if (any != 0) {
+        const uint64_t my_mark = mine_of(mark);
+        const uint32_t stay = static_cast<uint32_t>(my_mark >> bit0) & 0xFFu;
+        uint32_t at = mine_hold + level + __popcll(my_mark & below);
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) {
+          if (k < my_word) at += __popcll(mark.of[k]);
+          level += __popcll(mark.of[k]);
+        }
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
           const uint32_t bit = stay >> t & 1u;
           hold[bit != 0 ? at : dump] = static_cast<uint16_t>(elem16(ahead[i], t));
           at += bit;
         }
-        level += __popcll(mark);
         __builtin_amdgcn_wave_barrier();
-        if (level >= kWave) {
+        if (level >= kTokens) {
           u32x4* from = reinterpret_cast<u32x4*>(hold + mine_hold + unit8);
-          const u32x4 full = from[0], rest = from[kWave / 8];
+          const u32x4 full = from[0], rest = from[kTokens / 8];
           if (mine) st16_cached(const_cast<uint8_t*>(address(out_entry, out + unit8)), full);
           from[0] = rest;
-          out += kWave;
-          level -= kWave;
+          out += kTokens;
+          level -= kTokens;
           out_entry = entry_of(min(out + unit8, len - 1));
           __builtin_amdgcn_wave_barrier();
         }
@@ -388,8 +428,13 @@ hipError_t launch_evict(const EvictCall& c, hipStream_t stream) {
   MoveShape shape{};
   const int64_t staged = a.words * 8 + c.max_blocks * 4;
   if (move_fits(c, shape)) {
-    if (staged <= kMostStaged) evict_move_kernel<true><<<grid, kBlockThreads, staged, stream>>>(a, shape);
-    else evict_move_kernel<false><<<grid, kBlockThreads, 0, stream>>>(a, shape);
+    // Few waves: half the dims each, twice the tokens a step (40001 tokens of 16 lines 137 us, against 215).  With many
+    // the longer pieces of memory of 8 dims are read a little faster (512 lines 280, against 305).
+    const bool few = lines * ((c.head_dim + 7) / 8) < kFewWaves;
+    const dim3 fine(lines, (c.head_dim + 15) / 16, 2);
+    if (staged > kMostStaged) evict_move_kernel<false, 8><<<grid, kBlockThreads, 0, stream>>>(a, shape);
+    else if (few) evict_move_kernel<true, 4><<<fine, kBlockThreads, staged, stream>>>(a, shape);
+    else evict_move_kernel<true, 8><<<grid, kBlockThreads, staged, stream>>>(a, shape);
   } else if (c.element_bytes == 1) evict_move_any_kernel<1><<<grid, kBlockThreads, 0, stream>>>(a);
   else if (c.element_bytes == 2) evict_move_any_kernel<2><<<grid, kBlockThreads, 0, stream>>>(a);
   else evict_move_any_kernel<4><<<grid, kBlockThreads, 0, stream>>>(a);
