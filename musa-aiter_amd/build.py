@@ -26,7 +26,8 @@ OUT_DIR = ROOT / "musa_aiter" / "_lib"
 LIB_NAME = "libmusa_aiter_kv_hip.so"
 SOURCES = ("kv_paged_tiles.hip", "kv_paged_waves.hip", "kv_paged_wide.hip", "kv_rows.hip", "kv_batch_copy.hip", "kv_cachegen.hip",
            "kv_pattern.hip", "kv_block_store.hip", "kv_attention.hip", "kv_attention_wide.hip", "kv_pages.hip",
-           "kv_cache_attention.hip", "kv_cache_attention_rows.hip", "kv_attention_weights.hip", "kv_evict.hip", "kv_abi.hip", "kv_serving_abi.hip",
+           "kv_cache_attention.hip", "kv_cache_attention_rows.hip",
+           "kv_cache_attention_wide.hip", "kv_attention_weights.hip", "kv_evict.hip", "kv_abi.hip", "kv_serving_abi.hip",
            "kv_cache_attention_abi.hip")
 ARCH = os.environ.get("MUSA_AITER_HIP_ARCH", "gfx950")
 

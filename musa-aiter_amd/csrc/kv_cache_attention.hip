@@ -165,6 +165,9 @@ struct Plan {
 
 constexpr int64_t kTurnPlaces = kTilePlaces * kWavesPerBlock;
 constexpr int64_t kRowsGroups = 8192;
+constexpr int64_t kFewRows = 32;
+constexpr int64_t kWidePlaces = 512;
+constexpr int64_t kWideGroups = 1024;
 
 // Parts of a multiple of `unit` places each: no more than give `groups` workgroups, and `most` of a line.
 void cut(Plan& p, int64_t places, int64_t unit, int64_t groups, int64_t most) {
@@ -179,13 +182,16 @@ Plan make_plan(const CacheAttnCall& c) {
   if (tiles_fit(c)) {
     const int64_t group = c.heads / c.kv_heads;
     const int64_t seq_rows = (c.starts == nullptr || c.batch == 0 ? 1 : (c.rows + c.batch - 1) / c.batch) * group;
-    p.size = seq_rows <= 16 || c.head_dim > 128 ? 16 : 32;
+    const bool wide = seq_rows > kFewRows && c.head_dim <= 128 && c.softmax_scale > 0.0;
+    p.size = wide ? kWideTileRows : seq_rows <= 16 || c.head_dim > 128 ? 16 : 32;
     CacheArgs a = cache_args(c, static_cast<int>(p.size));
     p.tiles = tiles_bound(a.r.c, static_cast<int>(p.size));
     if (p.tiles < 1) p.tiles = 1;  // rows of no sequence
     p.lines = p.tiles * c.kv_heads;
     p.slot_rows = c.starts == nullptr && group < p.size ? group : p.size;
-    cut(p, most_places(c, static_cast<int>(p.size)), kTurnPlaces, kRowsGroups, 256);
+    const int64_t places = most_places(c, static_cast<int>(p.size));
+    if (wide) cut(p, places, kWidePlaces, kWideGroups, 64);
+    else cut(p, places, kTurnPlaces, kRowsGroups, 256);
     return p;
   }
   p.lines = c.rows * c.heads;
@@ -203,7 +209,7 @@ template <int DT>
 hipError_t launch(const CacheAttnCall& c, const Plan& p, CacheArgs a, hipStream_t stream) {
   hipError_t err;
   if (p.size > 0) {
-    err = launch_rows(a, static_cast<int>(p.size / 16), stream);
+    err = p.size == kWideTileRows ? launch_wide_tiles(a, stream) : launch_rows(a, static_cast<int>(p.size / 16), stream);
   } else {
     cache_any_kernel<DT><<<dim3(c.rows, c.heads, p.parts), kBlockThreads, 0, stream>>>(a);
     err = hipGetLastError();

@@ -205,7 +205,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_rows_kernel(const Cach
     const int32_t v1 = v0 + kWavesPerBlock * kTilePlaces;
     const Unit next = resolve_unit(a, w, entry, v1 + 8 * unit_k, hi);
     entry = load_unit(a, w, table, v1 + kWavesPerBlock * kTilePlaces + 8 * unit_k, hi);
-    one_tile(ballot(unit.bits != 0xFFu) != 0 || !all_rows_see(a, w, v0), unit, next, v1 < hi);
+    one_tile(ballot(unit.bits != 0xFFu) != 0 || !all_rows_see(a, w, v0, kTilePlaces), unit, next, v1 < hi);
     unit = next;
     v0 = v1;
   }
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_rows_kernel(const Cach
   }
   __syncthreads();
   if (odd_rows != 0)
-    redo_rows<DT, HD>(a, w, tile, kv_head, line, part, count, lo, hi, odd_rows, &exchange[0][0]);
+    redo_rows<DT, HD>(a, w, tile, kv_head, line, part, count, lo, hi, odd_rows, 0, &exchange[0][0]);
 }
 
 template <int DT, int HD>

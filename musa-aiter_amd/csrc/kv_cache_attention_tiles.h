@@ -68,10 +68,10 @@ __device__ __forceinline__ Unit resolve_unit(const CacheArgs& a, const View& w, 
           tile_bits(w, static_cast<int32_t>(token))};
 }
 
-// Whether every row of the tile sees all of the kTilePlaces places from v on, as far as the rows themselves go.
-__device__ __forceinline__ bool all_rows_see(const CacheArgs& a, const View& w, int32_t v) {
+// Whether every row of the tile sees all of the `places` places from v on, as far as the rows themselves go.
+__device__ __forceinline__ bool all_rows_see(const CacheArgs& a, const View& w, int32_t v, int places) {
   if (v < w.front) return false;
-  const int32_t from = v + w.gap, last = from + kTilePlaces - 1;
+  const int32_t from = v + w.gap, last = from + places - 1;
   if (a.masks != nullptr) return last < w.before;
   return last <= w.pos_lo && (a.window == 0 || from > w.pos_hi - a.window);
 }
@@ -140,11 +140,12 @@ __device__ __forceinline__ void store4(void* base, int64_t at, f32x4 o) {
 
 // Rows whose sums are infinite or no numbers, once more without matrix products.  A weight of 0 times an infinite or
 // NaN value of a position that this row does not see, but another of the tile does, is what makes most of them; a
-// product cannot leave a value out.  scratch: LDS that nothing else uses any more.
+// product cannot leave a value out.  rows: bits of the rows from first_row of the tile on; scratch: LDS that nothing else
+// uses any more.
 template <int DT, int HD>
 __device__ __forceinline__ void redo_rows(const CacheArgs& a, const View& w, const RowTile& tile, int32_t kv_head,
                                           int64_t line, int32_t part, int32_t count, int32_t lo, int32_t hi,
-                                          uint32_t rows, float* scratch) {
+                                          uint32_t rows, int32_t first_row, float* scratch) {
   const AttnCall& c = a.r.c;
   const int lane = lane_id(), wave = wave_in_block();
   constexpr int kFloats = HD + (sizeof(VisitScratch) + 15) / 16 * 4;
@@ -152,7 +153,7 @@ __device__ __forceinline__ void redo_rows(const CacheArgs& a, const View& w, con
   VisitScratch& visit = *reinterpret_cast<VisitScratch*>(q + HD);
   for (int32_t turn = 0; rows != 0; rows &= rows - 1, ++turn) {
     if (turn % kWavesPerBlock != wave) continue;
-    const int32_t in_tile = __builtin_ctz(rows);
+    const int32_t in_tile = first_row + __builtin_ctz(rows);
     const TilePlace p = tile_place(a, tile, kv_head, in_tile);
     for (int d = lane; d < HD; d += kWave)
       q[d] = load_q<DT>(c.query, p.row * c.query_row_stride + p.head * c.query_head_stride + d);
@@ -182,6 +183,10 @@ __device__ __forceinline__ void redo_rows(const CacheArgs& a, const View& w, con
 
 // kv_cache_attention_rows.hip: tiles of 16 * nt rows.
 hipError_t launch_rows(const CacheArgs& a, int nt, hipStream_t stream);
+
+// kv_cache_attention_wide.hip: tiles of kWideTileRows rows.
+constexpr int kWideTileRows = 128;
+hipError_t launch_wide_tiles(const CacheArgs& a, hipStream_t stream);
 
 }  // namespace catt
 }  // namespace kvhip
