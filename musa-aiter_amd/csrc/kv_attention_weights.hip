@@ -99,8 +99,8 @@ __global__ __launch_bounds__(kBlockThreads, HD <= 128 ? 2 : 1) void weights_tile
     u32x4 keys[kSteps][8];
     {
       u32x4 raw[kSteps][8];
-      const uint8_t* k = static_cast<const uint8_t*>(c.cache[0]) + unit.block * c.cache_block_stride[0] +
-                         unit.place * 2 + (static_cast<int64_t>(kv_head) * HD + 8 * g) * row_bytes;
+      const uint8_t* k = static_cast<const uint8_t*>(c.cache[0]) + block_offset(a, 0, unit.block, unit.place) +
+                         (static_cast<int64_t>(kv_head) * HD + 8 * g) * row_bytes;
 #pragma unroll
       for (int ks = 0; ks < kSteps; ++ks) {
         const uint8_t* from = k;

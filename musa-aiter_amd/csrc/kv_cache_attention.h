@@ -36,9 +36,10 @@ struct CacheArgs {
 };
 
 // Weights are 2^(score - maximum + kTop): fp16 ones keep their 11 bits down to 2^-28 of the largest, and sums of the
-// largest bf16 and float32 values times weights stay finite for up to 2^20 tokens.  The same factor is in their sum.
+// largest bf16 and float32 values times weights stay finite for up to 2^20 tokens (a row's maximum may pass the reference by 2^8 for
+// a while).  The same factor is in their sum.
 template <int DT>
-constexpr float kTop = DT == kLinF16 ? 14.0f : -20.0f;
+constexpr float kTop = DT == kLinF16 ? 14.0f : -28.0f;
 
 // Positions that the rows of a tile see between them, as an axis without the gap between the first tokens and the
 // window: place v is position v below `front`, v + gap from there on.  `front` and the window's begin are rounded to

@@ -140,6 +140,39 @@ __global__ __launch_bounds__(kBlockThreads) void cache_join_kernel(const CacheAr
   if (threadIdx.x == 0 && c.lse != nullptr) c.lse[out] = log_sum<DT>(top, sum);
 }
 
+// The same with a wave per row, for few parts.
+template <int DT>
+__global__ __launch_bounds__(kBlockThreads) void cache_join_few_kernel(const CacheArgs a) {
+  const AttnCall& c = a.r.c;
+  const int64_t line = blockIdx.x;
+  const int32_t x = blockIdx.y * kWavesPerBlock + wave_in_block();
+  const Line info = *line_of(a, line);
+  const int32_t at = info.base + x;
+  if (info.parts <= 1 || x >= a.slot_rows || at >= info.count * a.r.group) return;
+  const int64_t row = info.first + at / a.r.group, head = (line % c.kv_heads) * a.r.group + at % a.r.group;
+  const int lane = lane_id();
+  const float* ml = slot_ml(a, slot_row(a, line, 0, x));
+  const float* part = slot_acc(a, slot_row(a, line, 0, x));
+  const int64_t pitch = 2 * static_cast<int64_t>(a.slot_rows), step = static_cast<int64_t>(a.slot_rows) * c.head_dim;
+  float top = -__builtin_inff(), sum = 0.0f;
+  for (int32_t s = 0; s < info.parts; ++s) top = fmaxf(top, ml[s * pitch]);
+  constexpr int kDims = 256 / kWave;  // of the forms in tiles
+  float acc[kDims] = {};
+  for (int32_t s = 0; s < info.parts; ++s) {
+    const float fade = fade_to(ml[s * pitch], top);
+    sum += ml[s * pitch + 1] * fade;
+#pragma unroll
+    for (int i = 0; i < kDims; ++i)
+      if (lane + i * kWave < c.head_dim) acc[i] = __builtin_fmaf(part[s * step + lane + i * kWave], fade, acc[i]);
+  }
+  const int64_t out = row * c.heads + head;
+#pragma unroll
+  for (int i = 0; i < kDims; ++i)
+    if (lane + i * kWave < c.head_dim)
+      store_o<DT>(c.out, out * c.head_dim + lane + i * kWave, sum == 0.0f ? 0.0f : acc[i] / sum);
+  if (lane == 0 && c.lse != nullptr) c.lse[out] = log_sum<DT>(top, sum);
+}
+
 // The most places that a line's view has, by `longest` and what a table row has room for.
 int64_t most_places(const CacheAttnCall& c, int rows) {
   const int64_t room = c.max_blocks * c.block_size;
@@ -205,6 +238,8 @@ int64_t plan_workspace(const CacheAttnCall& c, const Plan& p) {
   return p.lines * p.parts * p.slot_rows * (2 + c.head_dim) * 4 + p.lines * static_cast<int64_t>(sizeof(Line));
 }
 
+constexpr int64_t kFewParts = 8;
+
 template <int DT>
 hipError_t launch(const CacheAttnCall& c, const Plan& p, CacheArgs a, hipStream_t stream) {
   hipError_t err;
@@ -216,7 +251,10 @@ hipError_t launch(const CacheAttnCall& c, const Plan& p, CacheArgs a, hipStream_
   }
   if (err != hipSuccess) return err;
   if (p.parts > 1) {
-    cache_join_kernel<DT><<<dim3(p.lines, p.slot_rows), kBlockThreads, 0, stream>>>(a);
+    if (p.size > 0 && p.parts <= kFewParts)
+      cache_join_few_kernel<DT><<<dim3(p.lines, (p.slot_rows + kWavesPerBlock - 1) / kWavesPerBlock), kBlockThreads, 0, stream>>>(a);
+    else
+      cache_join_kernel<DT><<<dim3(p.lines, p.slot_rows), kBlockThreads, 0, stream>>>(a);
   }
   return hipGetLastError();
 }
@@ -229,7 +267,8 @@ bool tiles_fit(const CacheAttnCall& c) {
   if (c.block_size % 8 != 0 || (hd != 64 && hd != 96 && hd != 128 && hd != 192 && hd != 256)) return false;
   if ((reinterpret_cast<uint64_t>(c.out) & 7) != 0 || c.kv_heads > 65535) return false;
   for (int kv = 0; kv < 2; ++kv)
-    if (c.cache[kv] != nullptr && ((reinterpret_cast<uint64_t>(c.cache[kv]) | c.cache_block_stride[kv]) & 15) != 0)
+    if (c.cache[kv] != nullptr && (((reinterpret_cast<uint64_t>(c.cache[kv]) | c.cache_block_stride[kv]) & 15) != 0 ||
+                                   c.cache_block_stride[kv] < 0 || c.cache_block_stride[kv] >= int64_t{1} << 32))
       return false;
   return true;
 }
@@ -273,6 +312,7 @@ CacheArgs cache_args(const CacheAttnCall& c, int size) {
   a.r.num_blocks = static_cast<int32_t>(c.num_blocks);
   a.r.room = static_cast<int32_t>(c.max_blocks * c.block_size);
   a.r.group = static_cast<int32_t>(c.heads / c.kv_heads);
+  a.r.block_shift = (c.block_size & (c.block_size - 1)) == 0 ? __builtin_ctzll(c.block_size) : -1;
   a.r.seq_tiles = size > 0 ? (a.r.group + size - 1) / size : 1;
   a.masks = c.masks;
   a.mask_stride = c.mask_stride;

@@ -105,9 +105,10 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_rows_kernel(const Cach
   // masked: some row does not see some of the positions.  (Two copies of the body, with and without masks, spill.)
   auto one_tile = [&](bool masked, const Unit& unit, const Unit& next, bool more) {
     uint32_t bits[4];
+    const uint64_t v_offset = block_offset(a, 1, unit.block, unit.place);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      v_unit[r] = value + __shfl(unit.block, 4 * g + r) * c.cache_block_stride[1] + __shfl(unit.place, 4 * g + r) * 2;
+      v_unit[r] = value + shfl64(v_offset, 4 * g + r);
       bits[r] = __shfl(unit.bits, 4 * g + r);
     }
     f32x4 s[NT][8];
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_rows_kernel(const Cach
       else load_v(ks + 2 - kSteps);
       __builtin_amdgcn_sched_barrier(0);
     }
-    k_unit = key + next.block * c.cache_block_stride[0] + next.place * 2;
+    k_unit = key + block_offset(a, 0, next.block, next.place);
     u32x4 weight[NT][2][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -196,7 +197,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_rows_kernel(const Cach
   Unit unit = resolve_unit(a, w, entry, v0 + 8 * unit_k, hi);
   entry = load_unit(a, w, table, v0 + kWavesPerBlock * kTilePlaces + 8 * unit_k, hi);
   if (v0 < hi) {
-    k_unit = key + unit.block * c.cache_block_stride[0] + unit.place * 2;
+    k_unit = key + block_offset(a, 0, unit.block, unit.place);
     load_k(0);
     load_k(1);
   }

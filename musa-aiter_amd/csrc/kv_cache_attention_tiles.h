@@ -40,6 +40,28 @@ struct Mma16<kLinBF16> {
 
 constexpr int kTilePlaces = 128;  // places of a wave's tile, 16 units of 8
 
+// Table column of a position.  (block_shift is log2(block_size) here, or -1.)
+__device__ __forceinline__ uint32_t block_column(const CacheArgs& a, int32_t token) {
+  return a.r.block_shift >= 0 ? static_cast<uint32_t>(token) >> a.r.block_shift
+                              : static_cast<uint32_t>(token) / static_cast<uint32_t>(a.r.bs);
+}
+
+// Byte offset of a block's place from its cache's beginning: strides are below 2^32 (see tiles_fit).
+__device__ __forceinline__ uint64_t block_offset(const CacheArgs& a, int kv, int32_t block, int32_t place) {
+  return static_cast<uint64_t>(static_cast<uint32_t>(block)) * static_cast<uint32_t>(a.r.c.cache_block_stride[kv]) +
+         static_cast<uint32_t>(2 * place);
+}
+
+__device__ __forceinline__ uint64_t shfl64(uint64_t v, int lane) {
+  const uint32_t lo = __shfl(static_cast<uint32_t>(v), lane), hi = __shfl(static_cast<uint32_t>(v >> 32), lane);
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
+// How far (in powers of two) a row's maximum may pass the reference its weights are taken to before sums so far are
+// scaled to a new one: float16 weights of up to 2^15 fit, for the others there is much room.
+template <int DT>
+constexpr float kSlack = DT == kLinF16 ? 1.0f : 8.0f;
+
 // The table entry of the unit of 8 places from v on, on its way (see load_entry for the FP8 caches).
 struct UnitEntry {
   uint32_t lo, hi;
@@ -48,7 +70,7 @@ struct UnitEntry {
 __device__ __forceinline__ UnitEntry load_unit(const CacheArgs& a, const View& w, const uint8_t* table, int32_t v,
                                                int32_t end) {
   if (end <= 0) return {0xFFFFFFFFu, 0xFFFFFFFFu};
-  const uint32_t column = static_cast<uint32_t>(position(w, min(v, (end - 1) & ~7))) / static_cast<uint32_t>(a.r.bs);
+  const uint32_t column = block_column(a, position(w, min(v, (end - 1) & ~7)));
   const uint8_t* p = table + static_cast<uint64_t>(column) * (a.r.c.wide_tables ? 8 : 4);
   return {load4(p), load4(p + (a.r.c.wide_tables ? 4 : 0))};
 }
@@ -63,9 +85,10 @@ struct Unit {
 __device__ __forceinline__ Unit resolve_unit(const CacheArgs& a, const View& w, const UnitEntry& e, int32_t v, int32_t end) {
   const bool good = v < end && e.lo < static_cast<uint32_t>(a.r.num_blocks) && (!a.r.c.wide_tables || e.hi == 0);
   if (!good) return {0, 0, 0};
-  const uint32_t token = static_cast<uint32_t>(position(w, v));
-  return {static_cast<int32_t>(e.lo), static_cast<int32_t>(token % static_cast<uint32_t>(a.r.bs)),
-          tile_bits(w, static_cast<int32_t>(token))};
+  const int32_t token = position(w, v);
+  const int32_t place = a.r.block_shift >= 0 ? token & (a.r.bs - 1)
+                                             : token - static_cast<int32_t>(block_column(a, token)) * a.r.bs;
+  return {static_cast<int32_t>(e.lo), place, tile_bits(w, token)};
 }
 
 // Whether every row of the tile sees all of the `places` places from v on, as far as the rows themselves go.

@@ -99,13 +99,15 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
 
   const int64_t row_bytes = static_cast<int64_t>(a.r.bs) * 2;
   const int key_g = lane >> 3 & 3, key_half = lane >> 5;
+  const int key_slot = 16 * g + (x ^ g);  // the 8 bytes that lanes write at a time lie on different banks
   const uint8_t* key = static_cast<const uint8_t*>(c.cache[0]) +
                        (static_cast<int64_t>(kv_head) * HD + 16 * key_half + key_g) * row_bytes;
   const uint8_t* value = static_cast<const uint8_t*>(c.cache[1]) + (static_cast<int64_t>(kv_head) * HD + x) * row_bytes;
   u32x4 raw_keys[kMyKeys][4], raw_values[kMyValues];
   // The lane's shares of a tile: step wave + 4 n of K, image wave + 4 n of V (dims of 16, then the half of the units).
   auto load_tile = [&](const Unit& unit) {
-    const uint8_t* k = key + unit.block * c.cache_block_stride[0] + unit.place * 2;
+    const uint8_t* k = key + block_offset(a, 0, unit.block, unit.place);
+    const uint64_t v = block_offset(a, 1, unit.block, unit.place);
 #pragma unroll
     for (int n = 0; n < kMyKeys; ++n) {
       if (kSteps % kWavesPerBlock != 0 && wave + kWavesPerBlock * n >= kSteps) break;
@@ -119,8 +121,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
 #pragma unroll
     for (int n = 0; n < kMyValues; ++n) {
       const int image = wave + kWavesPerBlock * n, half = image / kDimTiles, dt = image % kDimTiles;
-      const int32_t block = __shfl(unit.block, 4 * half + g), place = __shfl(unit.place, 4 * half + g);
-      raw_values[n] = ld16_cached(value + block * c.cache_block_stride[1] + 16 * dt * row_bytes + place * 2);
+      raw_values[n] = ld16_cached(value + 16 * dt * row_bytes + shfl64(v, 4 * half + g));
     }
   };
   auto store_tile = [&](WideTile<HD>& to, const Unit& unit, bool masked) {
@@ -137,7 +138,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
                                           (t & 1) != 0 ? 0x07060302u : 0x05040100u);
         // Unit u = lane % 8 is 4 (j / 2) + g of product j = 2 (u / 4) + t / 4, its token t in row 4 (u % 4) + t % 4.
         const int j = 2 * ((lane & 7) >> 2) + (t >> 2), row = 4 * (lane & 3) + (t & 3);
-        reinterpret_cast<u32x2*>(&to.keys[j][ks][16 * key_g + row])[key_half] = dims;
+        reinterpret_cast<u32x2*>(&to.keys[j][ks][16 * key_g + (row ^ key_g)])[key_half] = dims;
       }
     }
 #pragma unroll
@@ -173,7 +174,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
     for (int ks = 0; ks < kSteps; ++ks)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const u32x4 keys = at.keys[j][ks][lane];
+        const u32x4 keys = at.keys[j][ks][key_slot];
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt) s[nt][j] = Mma16<DT>::mma(keys, query[nt][ks], s[nt][j]);
       }
@@ -200,9 +201,11 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) most = fmaxf(most, s[nt][j][r]);
-      const float top = fmaxf(m[nt], groups_max(most) * a.factor);
+      float top = groups_max(most) * a.factor;
+      const bool past = ballot(top > m[nt] + kSlack<DT>) != 0;
+      top = past ? fmaxf(m[nt], top) : m[nt];
       const float ref = (top == -__builtin_inff() ? 0.0f : top) - kTop<DT>;
-      if (ballot(top != m[nt]) != 0) {
+      if (past) {
         const float fade = fade_to(m[nt], top);
         l[nt] *= fade;
 #pragma unroll
