@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_rows_kernel(const Cach
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int t = 0; t < 8; ++t) top = fmaxf(top, s[nt][t][r]);
-      top = groups_max(top);
+      top = four_max(top);
       const float ref = (top == -__builtin_inff() ? 0.0f : top) - kTop<DT>;
       if (ballot(top != m[nt]) != 0) {
         const float fade = fade_to(m[nt], top);

@@ -57,6 +57,14 @@ __device__ __forceinline__ uint64_t shfl64(uint64_t v, int lane) {
   return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
+// Maximum and sum over the four lane groups of 16, without LDS: the swaps leave both halves of what they exchange.
+__device__ __forceinline__ float four_max(float v) {
+  const u32x2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a.x), __uint_as_float(a.y));
+  const u32x2 b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b.x), __uint_as_float(b.y));
+}
+
 // How far (in powers of two) a row's maximum may pass the reference its weights are taken to before sums so far are
 // scaled to a new one: float16 weights of up to 2^15 fit, for the others there is much room.
 template <int DT>

@@ -159,10 +159,9 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
   int turn = 0;
   for (int32_t v0 = lo; v0 < hi; v0 += kWideTile, turn ^= 1) {
     const WideTile<HD>& at = tiles[turn];
-    const bool more = v0 + kWideTile < hi;
     const Unit next = resolve_unit(a, w, entry, v0 + kWideTile + my_unit8, hi);
     entry = load_unit(a, w, table, v0 + 2 * kWideTile + my_unit8, hi);
-    if (more) load_tile(next);
+    load_tile(next);
     const bool masked = ballot(unit.bits != 0xFFu) != 0 || !all_rows_see(a, mine, v0, kWideTile);
 
     f32x4 s[2][4];
@@ -192,26 +191,34 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
         }
       }
     }
-    u32x4 weight[2][2];
+    // The factor is positive here: the largest product is the largest score's.
+    float top[2];
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt) {
-      // The factor is positive here: the largest product is the largest score's.
       float most = s[nt][0][0];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) most = fmaxf(most, s[nt][j][r]);
-      float top = groups_max(most) * a.factor;
-      const bool past = ballot(top > m[nt] + kSlack<DT>) != 0;
-      top = past ? fmaxf(m[nt], top) : m[nt];
-      const float ref = (top == -__builtin_inff() ? 0.0f : top) - kTop<DT>;
-      if (past) {
-        const float fade = fade_to(m[nt], top);
+      top[nt] = four_max(most) * a.factor;
+    }
+    if (ballot(top[0] > m[0] + kSlack<DT> || top[1] > m[1] + kSlack<DT>) != 0) {
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        top[nt] = fmaxf(m[nt], top[nt]);
+        const float fade = fade_to(m[nt], top[nt]);
         l[nt] *= fade;
 #pragma unroll
         for (int dt = 0; dt < kDimTiles; ++dt) acc[nt][dt] *= fade;
-        m[nt] = top;
+        m[nt] = top[nt];
       }
+    }
+    // (Behind the last tile: block 0, which is not looked at.)
+    store_tile(tiles[turn ^ 1], next, ballot(next.bits != 0xFFu) != 0);
+    u32x4 weight[2][2];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      const float ref = (m[nt] == -__builtin_inff() ? 0.0f : m[nt]) - kTop<DT>;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -230,7 +237,6 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt) acc[nt][dt] = Mma16<DT>::mma(values, weight[nt][half], acc[nt][dt]);
       }
-    if (more) store_tile(tiles[turn ^ 1], next, ballot(next.bits != 0xFFu) != 0);
     unit = next;
     __syncthreads();
   }
