@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kWideTile = 64;  // positions
 constexpr int kWaveRows = kWideTileRows / kWavesPerBlock;
+constexpr int kReads = 4;  // operands on their way from LDS
 
 template <int HD>
 struct WideTile {  // 1 KiB of 64 lanes for each operand
@@ -169,14 +170,18 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[nt][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // Operands are read from LDS kReads ahead; left alone, the compiler waits for each before it asks for the next.
+    u32x4 operand[kReads];
 #pragma unroll
-    for (int ks = 0; ks < kSteps; ++ks)
+    for (int n = 0; n < kReads; ++n) operand[n] = at.keys[n & 3][n >> 2][key_slot];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u32x4 keys = at.keys[j][ks][key_slot];
+    for (int n = 0; n < 4 * kSteps; ++n) {
+      const int ks = n >> 2, j = n & 3;
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) s[nt][j] = Mma16<DT>::mma(keys, query[nt][ks], s[nt][j]);
-      }
+      for (int nt = 0; nt < 2; ++nt) s[nt][j] = Mma16<DT>::mma(operand[n % kReads], query[nt][ks], s[nt][j]);
+      if (n + kReads < 4 * kSteps) operand[n % kReads] = at.keys[(n + kReads) & 3][(n + kReads) >> 2][key_slot];
+      __builtin_amdgcn_sched_barrier(0);
+    }
     if (masked) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -213,8 +218,6 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
         m[nt] = top[nt];
       }
     }
-    // (Behind the last tile: block 0, which is not looked at.)
-    store_tile(tiles[turn ^ 1], next, ballot(next.bits != 0xFFu) != 0);
     u32x4 weight[2][2];
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt) {
@@ -230,13 +233,19 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
         }
     }
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
+    for (int n = 0; n < kReads; ++n) operand[n] = at.values[0][n][lane];
+    __builtin_amdgcn_sched_barrier(0);  // the sums above are made here, not carried on as 32 summands
 #pragma unroll
-      for (int dt = 0; dt < kDimTiles; ++dt) {
-        const u32x4 values = at.values[half][dt][lane];
+    for (int n = 0; n < 2 * kDimTiles; ++n) {
+      const int half = n / kDimTiles, dt = n % kDimTiles;
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) acc[nt][dt] = Mma16<DT>::mma(values, weight[nt][half], acc[nt][dt]);
-      }
+      for (int nt = 0; nt < 2; ++nt) acc[nt][dt] = Mma16<DT>::mma(operand[n % kReads], weight[nt][half], acc[nt][dt]);
+      if (n + kReads < 2 * kDimTiles)
+        operand[n % kReads] = at.values[(n + kReads) / kDimTiles][(n + kReads) % kDimTiles][lane];
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // (Behind the last tile: block 0, which is not looked at.)
+    store_tile(tiles[turn ^ 1], next, ballot(next.bits != 0xFFu) != 0);
     unit = next;
     __syncthreads();
   }
