@@ -149,15 +149,28 @@ __device__ __forceinline__ void stage_queries(const CacheArgs& a, const RowTile&
   const AttnCall& c = a.r.c;
   const uint16_t* from = static_cast<const uint16_t*>(c.query);
   uint16_t* to = reinterpret_cast<uint16_t*>(queries);
+  auto place = [](int row, int d) {
+    const int lane = (d & 3) * 16 + (row & 15), i = (d & 31) >> 2;
+    return (((row >> 4) * (HD / 32) + d / 32) * kWave + lane) * 8 + i;
+  };
+  auto row_of = [&](int row) {
+    const TilePlace p = tile_place(a, tile, kv_head, row);
+    return from + p.row * c.query_row_stride + p.head * c.query_head_stride;
+  };
+  if (((reinterpret_cast<uint64_t>(from) | 2 * c.query_row_stride | 2 * c.query_head_stride) & 15) == 0) {
+#pragma unroll 4
+    for (int at = threadIdx.x; at < 16 * NT * HD / 8; at += kBlockThreads) {
+      const int row = at / (HD / 8), d = at % (HD / 8) * 8;
+      u32x4 dims{};
+      if (row < tile_rows) dims = ld16_cached(reinterpret_cast<const uint8_t*>(row_of(row) + d));
+#pragma unroll
+      for (int k = 0; k < 8; ++k) to[place(row, d + k)] = static_cast<uint16_t>(elem16(dims, k));
+    }
+    return;
+  }
   for (int at = threadIdx.x; at < 16 * NT * HD; at += kBlockThreads) {
     const int row = at / HD, d = at % HD;
-    uint16_t bits = 0;
-    if (row < tile_rows) {
-      const TilePlace p = tile_place(a, tile, kv_head, row);
-      bits = from[p.row * c.query_row_stride + p.head * c.query_head_stride + d];
-    }
-    const int lane = (d & 3) * 16 + (row & 15), i = (d & 31) >> 2;
-    to[(((row >> 4) * (HD / 32) + d / 32) * kWave + lane) * 8 + i] = bits;
+    to[place(row, d)] = row < tile_rows ? row_of(row)[d] : 0;
   }
 }
 

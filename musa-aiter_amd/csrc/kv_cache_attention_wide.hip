@@ -61,7 +61,9 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
 
   const uint8_t* table = static_cast<const uint8_t*>(c.tables) +
                          static_cast<int64_t>(tile.seq) * c.table_stride * (c.wide_tables ? 8 : 4);
-  const int32_t my_unit8 = 8 * (lane & 7);
+  // Lane: units, halves of 32 dims and quarters of those, so that the 8 bytes that 32 lanes write to LDS at a time lie on
+  // different banks.  Unit k is in lane 32 (k / 4) + k % 4.
+  const int32_t my_unit8 = 8 * ((lane & 3) | lane >> 5 << 2);
   UnitEntry entry = load_unit(a, w, table, lo + my_unit8, hi);
 
   // Each wave's queries, by way of LDS.
@@ -99,8 +101,8 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
   }
 
   const int64_t row_bytes = static_cast<int64_t>(a.r.bs) * 2;
-  const int key_g = lane >> 3 & 3, key_half = lane >> 5;
-  const int key_slot = 16 * g + (x ^ g);  // the 8 bytes that lanes write at a time lie on different banks
+  const int key_g = lane >> 3 & 3, key_half = lane >> 2 & 1;
+  const int key_slot = 16 * g + (x ^ g);
   const uint8_t* key = static_cast<const uint8_t*>(c.cache[0]) +
                        (static_cast<int64_t>(kv_head) * HD + 16 * key_half + key_g) * row_bytes;
   const uint8_t* value = static_cast<const uint8_t*>(c.cache[1]) + (static_cast<int64_t>(kv_head) * HD + x) * row_bytes;
@@ -122,7 +124,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
 #pragma unroll
     for (int n = 0; n < kMyValues; ++n) {
       const int image = wave + kWavesPerBlock * n, half = image / kDimTiles, dt = image % kDimTiles;
-      raw_values[n] = ld16_cached(value + 16 * dt * row_bytes + shfl64(v, 4 * half + g));
+      raw_values[n] = ld16_cached(value + 16 * dt * row_bytes + shfl64(v, 32 * half + g));
     }
   };
   auto store_tile = [&](WideTile<HD>& to, const Unit& unit, bool masked) {
@@ -137,15 +139,15 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
         for (int p = 0; p < 2; ++p)
           dims[p] = __builtin_amdgcn_perm(raw_keys[n][2 * p + 1][t >> 1], raw_keys[n][2 * p][t >> 1],
                                           (t & 1) != 0 ? 0x07060302u : 0x05040100u);
-        // Unit u = lane % 8 is 4 (j / 2) + g of product j = 2 (u / 4) + t / 4, its token t in row 4 (u % 4) + t % 4.
-        const int j = 2 * ((lane & 7) >> 2) + (t >> 2), row = 4 * (lane & 3) + (t & 3);
+        // Unit u is 4 (j / 2) + g of product j = 2 (u / 4) + t / 4, its token t in row 4 (u % 4) + t % 4.
+        const int j = 2 * (lane >> 5) + (t >> 2), row = 4 * (lane & 3) + (t & 3);
         reinterpret_cast<u32x2*>(&to.keys[j][ks][16 * key_g + (row ^ key_g)])[key_half] = dims;
       }
     }
 #pragma unroll
     for (int n = 0; n < kMyValues; ++n) {
       const int image = wave + kWavesPerBlock * n, half = image / kDimTiles, dt = image % kDimTiles;
-      if (masked) raw_values[n] &= token_masks(__shfl(unit.bits, 4 * half + g));
+      if (masked) raw_values[n] &= token_masks(__shfl(unit.bits, 32 * half + g));
       to.values[half][dt][lane] = raw_values[n];
     }
   };
@@ -162,7 +164,6 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
     const WideTile<HD>& at = tiles[turn];
     const Unit next = resolve_unit(a, w, entry, v0 + kWideTile + my_unit8, hi);
     entry = load_unit(a, w, table, v0 + 2 * kWideTile + my_unit8, hi);
-    load_tile(next);
     const bool masked = ballot(unit.bits != 0xFFu) != 0 || !all_rows_see(a, mine, v0, kWideTile);
 
     f32x4 s[2][4];
@@ -185,7 +186,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
     if (masked) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const uint32_t bits = __shfl(unit.bits, 4 * half + g);
+        const uint32_t bits = __shfl(unit.bits, 32 * half + g);
         const int32_t token = position(w, v0 + 8 * (4 * half + g));
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt) {
@@ -196,6 +197,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
         }
       }
     }
+    load_tile(next);
     // The factor is positive here: the largest product is the largest score's.
     float top[2];
 #pragma unroll
