@@ -199,6 +199,7 @@ struct Plan {
 constexpr int64_t kTurnPlaces = kTilePlaces * kWavesPerBlock;
 constexpr int64_t kRowsGroups = 8192;
 constexpr int64_t kFewRows = 32;
+constexpr int64_t kAtOnce = 512;  // two workgroups a CU
 constexpr int64_t kWidePlaces = 512;
 constexpr int64_t kWideGroups = 1024;
 
@@ -215,8 +216,12 @@ Plan make_plan(const CacheAttnCall& c) {
   if (tiles_fit(c)) {
     const int64_t group = c.heads / c.kv_heads;
     const int64_t seq_rows = (c.starts == nullptr || c.batch == 0 ? 1 : (c.rows + c.batch - 1) / c.batch) * group;
-    const bool wide = seq_rows > kFewRows && c.head_dim <= 128 && c.softmax_scale > 0.0;
-    p.size = wide ? kWideTileRows : seq_rows <= 16 || c.head_dim > 128 ? 16 : 32;
+    // Few rows, and calls so small that all of their tiles of 16 rows run at once: those take the shortest way through a
+    // line (three trees of 7 to 13 tokens over 400: 10 us, in wide tiles 23).
+    const int64_t turns = (most_places(c, 16) + kTurnPlaces - 1) / kTurnPlaces;
+    const bool all_at_once = (c.rows * group / 16 + c.batch) * c.kv_heads * turns <= kAtOnce;
+    const bool wide = seq_rows > kFewRows && c.head_dim <= 128 && c.softmax_scale > 0.0 && !all_at_once;
+    p.size = wide ? kWideTileRows : seq_rows <= 16 || c.head_dim > 128 || all_at_once ? 16 : 32;
     CacheArgs a = cache_args(c, static_cast<int>(p.size));
     p.tiles = tiles_bound(a.r.c, static_cast<int>(p.size));
     if (p.tiles < 1) p.tiles = 1;  // rows of no sequence
