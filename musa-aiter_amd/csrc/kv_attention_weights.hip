@@ -60,6 +60,7 @@ __global__ __launch_bounds__(kBlockThreads) void weights_any_kernel(const CacheA
 // With few rows the waves of a workgroup take different positions (bound by the read of K: all of a wave's 32 loads are
 // on their way at once), with many the same positions and a quarter of the rows each (bound by 32 exponentials of a
 // quarter of the full rate next to 32 products).
+constexpr int kAtOnce = 4;     // tokens of the units whose scores are held at a time
 constexpr int kManyTiles = 4;  // row tiles of a sequence from which on the waves share positions
 
 __device__ __forceinline__ float sum_of_16(float v) {  // over lanes that differ in x
@@ -90,8 +91,10 @@ __global__ __launch_bounds__(kBlockThreads, HD <= 128 ? 2 : 1) void weights_tile
                          static_cast<int64_t>(seq) * c.table_stride * (c.wide_tables ? 8 : 4);
   const int64_t row_bytes = static_cast<int64_t>(a.r.bs) * 2;
   const float* lse_of = c.lse + seq_rows_.first * c.heads + static_cast<int64_t>(kv_head) * group;
-  const uint16_t* query = static_cast<const uint16_t*>(c.query) + seq_rows_.first * c.query_row_stride +
-                          static_cast<int64_t>(kv_head) * group * c.query_head_stride + 8 * g;
+  const uint8_t* query = reinterpret_cast<const uint8_t*>(
+      static_cast<const uint16_t*>(c.query) + seq_rows_.first * c.query_row_stride +
+      static_cast<int64_t>(kv_head) * group * c.query_head_stride + 8 * g);
+  const int group_log = (group & (group - 1)) == 0 ? __builtin_ctz(group) : -1;
   for (int32_t base = blockIdx.x * stride; base < w.length; base += gridDim.x * stride) {
     const int32_t v0 = base + (many ? 0 : wave * kTilePlaces);
     const UnitEntry entry = load_unit(a, w, table, v0 + 8 * x, w.length);
@@ -132,42 +135,57 @@ __global__ __launch_bounds__(kBlockThreads, HD <= 128 ? 2 : 1) void weights_tile
     const int32_t skip = max(from - w.before, 0);
     if (skip >= count || v0 >= w.length) at0 = rows;
     else at0 += skip * group / step * step;
+    // The next rows' queries are on their way while these are worked on.
+    u32x4 next16[kSteps];
+    float next_lse = 0.0f;
+    auto fetch = [&](int32_t first) {
+      const uint32_t at = min(first + x, rows - 1), i = group_log >= 0 ? at >> group_log : at / group, head = at - i * group;
+      next_lse = lse_of[static_cast<uint64_t>(i) * static_cast<uint32_t>(c.heads) + head];
+      const uint8_t* q = query + static_cast<uint64_t>(i) * static_cast<uint32_t>(2 * c.query_row_stride) +
+                         static_cast<uint64_t>(head) * static_cast<uint32_t>(2 * c.query_head_stride);
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) next16[ks] = ld16_cached(q + 64 * ks);
+    };
+    if (at0 < rows) fetch(at0);
     for (; at0 < rows; at0 += step) {
-      const int32_t at = min(at0 + x, rows - 1), i = at / group;
-      const int64_t row = i, head = at - i * group;
-      const float lse = lse_of[row * c.heads + head];
-      const uint16_t* q = query + row * c.query_row_stride + head * c.query_head_stride;
+      const float lse = next_lse, less = lse * kLog2e;
       u32x4 rows16[kSteps];
 #pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) rows16[ks] = ld16_cached(reinterpret_cast<const uint8_t*>(q + 32 * ks));
-      f32x4 s[8];
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int ks = 0; ks < kSteps; ++ks) s[t] = Mma16<DT>::mma(keys[ks][t], rows16[ks], s[t]);
-      }
-      const float less = lse * kLog2e;
+      for (int ks = 0; ks < kSteps; ++ks) rows16[ks] = next16[ks];
+      fetch(at0 + step);  // behind the last ones: the last row again
       const bool gives = at0 + x < rows && lse != -__builtin_inff();
       const int32_t pos_lo = w.before + at0 / group, pos_hi = w.before + min(at0 + 15, rows - 1) / group;
       const bool plain = whole && v0 >= w.front && last <= pos_lo && (a.window == 0 || from > pos_hi - a.window) &&
                          ballot(!gives) == 0;
-      if (plain) {
+      uint32_t seen[4];
+      if (!plain) {
+        const int32_t at = min(at0 + x, rows - 1);
+        const RowSight sight{w.before + at / group, nullptr};
 #pragma unroll
-        for (int t = 0; t < 8; ++t)
+        for (int r = 0; r < 4; ++r)
+          seen[r] = gives ? bits[r] & row_bits(a, w, sight, position(w, v0 + 8 * (4 * g + r))) : 0;
+      }
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sum[t][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], a.factor, -less));
-      } else {
-        const RowSight sight{w.before + i, nullptr};
+      for (int t0 = 0; t0 < 8; t0 += kAtOnce) {
+        f32x4 s[kAtOnce];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint32_t seen = gives ? bits[r] & row_bits(a, w, sight, position(w, v0 + 8 * (4 * g + r))) : 0;
+        for (int t = 0; t < kAtOnce; ++t) s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int t = 0; t < 8; ++t) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], a.factor, -less));
-            sum[t][r] += (seen >> t & 1u) != 0 ? p : 0.0f;
-          }
+        for (int ks = 0; ks < kSteps; ++ks)
+#pragma unroll
+          for (int t = 0; t < kAtOnce; ++t) s[t] = Mma16<DT>::mma(keys[ks][t0 + t], rows16[ks], s[t]);
+#pragma unroll
+        for (int t = 0; t < kAtOnce; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], a.factor, -less));
+        if (!plain) {
+#pragma unroll
+          for (int t = 0; t < kAtOnce; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[t][r] = (seen[r] >> (t0 + t) & 1u) != 0 ? s[t][r] : 0.0f;
         }
+#pragma unroll
+        for (int t = 0; t < kAtOnce; ++t) sum[t0 + t] += s[t];
       }
     }
 #pragma unroll
@@ -205,7 +223,9 @@ hipError_t launch_tiles(const CacheArgs& a, dim3 grid, hipStream_t stream) {
 
 // Whether 16 bytes of a query row can be read at a time.
 bool queries_fit(const CacheAttnCall& c) {
-  return ((reinterpret_cast<uint64_t>(c.query) | 2 * c.query_row_stride | 2 * c.query_head_stride) & 15) == 0;
+  const int64_t most = int64_t{1} << 31;
+  return ((reinterpret_cast<uint64_t>(c.query) | 2 * c.query_row_stride | 2 * c.query_head_stride) & 15) == 0 &&
+         c.query_row_stride >= 0 && c.query_row_stride < most && c.query_head_stride >= 0 && c.query_head_stride < most;
 }
 
 template <int DT>
