@@ -211,6 +211,10 @@ void cut(Plan& p, int64_t places, int64_t unit, int64_t groups, int64_t most) {
   p.parts = (places + p.part - 1) / p.part;
 }
 
+// Whether the scaling of scores may be fused with the difference to their maximum, as the form for many rows does it: the
+// factor is positive, and -inf times it is -inf.
+bool fuses_scale(const CacheAttnCall& c) { return c.softmax_scale > 1e-30 && c.softmax_scale < 1e30; }
+
 Plan make_plan(const CacheAttnCall& c) {
   Plan p{};
   if (tiles_fit(c)) {
@@ -220,7 +224,7 @@ Plan make_plan(const CacheAttnCall& c) {
     // line (three trees of 7 to 13 tokens over 400: 10 us, in wide tiles 23).
     const int64_t turns = (most_places(c, 16) + kTurnPlaces - 1) / kTurnPlaces;
     const bool all_at_once = (c.rows * group / 16 + c.batch) * c.kv_heads * turns <= kAtOnce;
-    const bool wide = seq_rows > kFewRows && c.head_dim <= 128 && c.softmax_scale > 0.0 && !all_at_once;
+    const bool wide = seq_rows > kFewRows && c.head_dim <= 128 && fuses_scale(c) && !all_at_once;
     p.size = wide ? kWideTileRows : seq_rows <= 16 || c.head_dim > 128 || all_at_once ? 16 : 32;
     CacheArgs a = cache_args(c, static_cast<int>(p.size));
     p.tiles = tiles_bound(a.r.c, static_cast<int>(p.size));

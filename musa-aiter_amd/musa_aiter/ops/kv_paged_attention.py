@@ -142,7 +142,7 @@ def kv_paged_attention(
 ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """Causal attention of ``query`` rows ``[T, heads, head_dim]`` over paged caches of the same type.
 
-    The rows of sequence ``b`` are ``query_starts[b] : query_starts[b + 1]``, its last tokens; without ``query_starts``
+    The rows of sequence ``b`` are ``query_starts[b] : query_starts[b + 1]`` (ascending), its last tokens; without ``query_starts``
     every sequence has one row (a decode step).  Row ``i`` of ``n`` sits at position ``seq_lens[b] - n + i`` and sees
     the positions up to there: all of them, or with ``window`` the last ``window`` and next to them the sequence's
     first ``sinks`` (their pages may be the only ones in front of the window that are still there).
@@ -331,6 +331,8 @@ def kv_evict_paged_tokens(
         raise ValueError(f"{op}: all tensors must be on the same device")
     if any(not _packed_blocks(c) or _overlaps(c) for c in (key_cache, value_cache)):
         raise ValueError(f"{op}: the blocks of the caches are written and must be contiguous")
+    if key_cache.data_ptr() == value_cache.data_ptr():
+        raise ValueError(f"{op}: key_cache and value_cache are moved each on its own and must not be one tensor")
     if weights.numel() and _overlaps(weights):
         raise ValueError(f"{op}: weights are written and must not be expanded")
     if sinks < 0 or recent < 0:

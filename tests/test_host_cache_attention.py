@@ -154,6 +154,12 @@ def test_evict_refusals(change, match):
         _evict(**change)
 
 
+def test_evict_takes_two_caches():
+    one = torch.zeros(2, 5, 2, 8, 16)
+    with pytest.raises(ValueError, match="one tensor"):
+        _evict(key_cache=one, value_cache=one)
+
+
 def test_evict_on_cpu_tensors_raises():
     with pytest.raises(RuntimeError, match="ROCm"):
         _evict()
