@@ -63,6 +63,15 @@ def test_seventeen_to_thirty_two_rows(dtype, hd, tree):
     case.check(*call(case))
 
 
+@pytest.mark.parametrize("extra", [40, 200])
+@pytest.mark.parametrize("heads,kv_heads", [(64, 1), (40, 2), (130, 1)])
+def test_decode_steps_of_wide_groups(heads, kv_heads, extra):
+    rng = np.random.default_rng(heads)
+    case = Case(lens=rng.integers(0, 300, size=72), heads=heads, kv_heads=kv_heads, hd=64, extra=extra, seed=heads)
+    assert not at_once(case)
+    case.check(*call(case))
+
+
 @pytest.mark.parametrize("tree", [0, 2])
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 def test_many_rows_and_what_they_do_not_see(tree, dtype):
