@@ -61,6 +61,7 @@ __global__ __launch_bounds__(kBlockThreads) void weights_any_kernel(const CacheA
 // on their way at once), with many the same positions and a quarter of the rows each (bound by 32 exponentials of a
 // quarter of the full rate next to 32 products).
 constexpr int kAtOnce = 4;     // tokens of the units whose scores are held at a time
+constexpr int64_t kCus = 256;
 constexpr int kManyTiles = 4;  // row tiles of a sequence from which on the waves share positions
 
 __device__ __forceinline__ float sum_of_16(float v) {  // over lanes that differ in x
@@ -74,19 +75,19 @@ __device__ __forceinline__ float sum_of_16(float v) {  // over lanes that differ
   return v;
 }
 
-template <int DT, int HD>
-__global__ __launch_bounds__(kBlockThreads, HD <= 128 ? 2 : 1) void weights_tile_kernel(const CacheArgs a) {
+template <int DT, int HD, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, HD <= 128 ? 2 : 1) void weights_tile_kernel(const CacheArgs a) {
   constexpr int kSteps = HD / 32;
   const AttnCall& c = a.r.c;
   const int lane = lane_id(), wave = wave_in_block(), x = lane & 15, g = lane >> 4;
   const int32_t seq = blockIdx.y, kv_head = blockIdx.z, group = a.r.group;
-  __shared__ __attribute__((aligned(16))) float sums[kWavesPerBlock][kTilePlaces];
+  __shared__ __attribute__((aligned(16))) float sums[WAVES][kTilePlaces];
   const SeqRows seq_rows_ = seq_rows(c, seq);
   if (seq_rows_.count == 0) return;
   const int32_t count = static_cast<int32_t>(seq_rows_.count), rows = count * group;
   const View w = make_view(a, seq, count, 0, count - 1);
   const bool many = a.parts > 1;  // the waves share positions
-  const int32_t stride = many ? kTilePlaces : kTilePlaces * kWavesPerBlock;
+  const int32_t stride = many ? kTilePlaces : kTilePlaces * WAVES;
   const uint8_t* table = static_cast<const uint8_t*>(c.tables) +
                          static_cast<int64_t>(seq) * c.table_stride * (c.wide_tables ? 8 : 4);
   const int64_t row_bytes = static_cast<int64_t>(a.r.bs) * 2;
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(kBlockThreads, HD <= 128 ? 2 : 1) void weights_tile
 #pragma unroll
     for (int t = 0; t < 8; ++t) sum[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    const int32_t step = many ? 16 * kWavesPerBlock : 16;
+    const int32_t step = many ? 16 * WAVES : 16;
     // Rows in front of the tile's first position see none of it.
     int32_t at0 = many ? 16 * wave : 0;
     const int32_t skip = max(from - w.before, 0);
@@ -197,11 +198,11 @@ __global__ __launch_bounds__(kBlockThreads, HD <= 128 ? 2 : 1) void weights_tile
       }
     __syncthreads();
     float* weights = a.weights + seq * a.weight_row_stride + kv_head * a.weight_head_stride;
-    for (int32_t n = threadIdx.x; n < stride; n += kBlockThreads) {
+    for (int32_t n = threadIdx.x; n < stride; n += WAVES * kWave) {
       const int32_t token = position(w, base + n);
       float all = many ? 0.0f : sums[n / kTilePlaces][n % kTilePlaces];
       if (many)
-        for (int k = 0; k < kWavesPerBlock; ++k) all += sums[k][n];
+        for (int k = 0; k < WAVES; ++k) all += sums[k][n];
       // What no row sees, behind the end among it, gathered nothing and is not written.
       if (base + n < w.length && token < a.weight_tokens && all != 0.0f) weights[token] += all;
     }
@@ -209,16 +210,26 @@ __global__ __launch_bounds__(kBlockThreads, HD <= 128 ? 2 : 1) void weights_tile
   }
 }
 
+template <int DT, int HD>
+hipError_t launch_hd(const CacheArgs& a, dim3 grid, hipStream_t stream) {
+  if constexpr (HD <= 128)
+    if (a.parts == 8) {
+      weights_tile_kernel<DT, HD, 8><<<grid, 8 * kWave, 0, stream>>>(a);
+      return hipGetLastError();
+    }
+  weights_tile_kernel<DT, HD, kWavesPerBlock><<<grid, kBlockThreads, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
 template <int DT>
 hipError_t launch_tiles(const CacheArgs& a, dim3 grid, hipStream_t stream) {
   switch (a.r.hd) {
-    case 64: weights_tile_kernel<DT, 64><<<grid, kBlockThreads, 0, stream>>>(a); break;
-    case 96: weights_tile_kernel<DT, 96><<<grid, kBlockThreads, 0, stream>>>(a); break;
-    case 128: weights_tile_kernel<DT, 128><<<grid, kBlockThreads, 0, stream>>>(a); break;
-    case 192: weights_tile_kernel<DT, 192><<<grid, kBlockThreads, 0, stream>>>(a); break;
-    default: weights_tile_kernel<DT, 256><<<grid, kBlockThreads, 0, stream>>>(a); break;
+    case 64: return launch_hd<DT, 64>(a, grid, stream);
+    case 96: return launch_hd<DT, 96>(a, grid, stream);
+    case 128: return launch_hd<DT, 128>(a, grid, stream);
+    case 192: return launch_hd<DT, 192>(a, grid, stream);
+    default: return launch_hd<DT, 256>(a, grid, stream);
   }
-  return hipGetLastError();
 }
 
 // Whether 16 bytes of a query row can be read at a time.
@@ -244,6 +255,9 @@ hipError_t launch(const CacheAttnCall& c, CacheArgs a, hipStream_t stream) {
   int64_t groups = (longest + share - 1) / share;
   groups = groups < 1 ? 1 : groups < 4096 ? groups : 4096;
   const dim3 grid(groups, c.batch, c.kv_heads);
+  // Positions for less than a workgroup per CU: eight waves share their rows (208 workgroups, 573 row tiles: 94 us,
+  // with four waves 124).
+  if (a.parts > 1 && groups * c.batch * c.kv_heads <= kCus) a.parts = 8;
   if constexpr (DT != kLinF32)
     if (tiles) return launch_tiles<DT>(a, grid, stream);
   weights_any_kernel<DT><<<grid, kBlockThreads, 0, stream>>>(a);

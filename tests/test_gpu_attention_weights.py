@@ -117,3 +117,12 @@ def test_layouts_and_scale():
     assert (base[:, 1::2] == 9).all() and (base[:, :, ::2] == 9).all()
     lse = lse * 0 + 3.0
     check(case, go(case, weights, lse, softmax_scale=-0.11), weights, lse, scale=-0.11)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hd,rows", [(64, 30), (128, 30), (128, 5)])
+def test_many_positions(dtype, hd, rows):
+    """More than 256 workgroups: four waves share positions where there are many rows, or take different ones."""
+    case = Case(lens=[900, 870, 1001, 1024, 600, 77], rows=[rows] * 6, heads=16, kv_heads=8, hd=hd, dtype=dtype, seed=hd)
+    weights, lse = prepared(case)
+    check(case, go(case, weights, lse), weights, lse)
