@@ -257,7 +257,7 @@ struct MoveShape {
   int log_block;   // log2(block_size), or -1
 };
 
-template <bool STAGED, int DIMS>
+template <bool STAGED, int DIMS, bool POW2>  // POW2: log_block is there
 __global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictArgs a, const MoveShape shape) {
   constexpr int kTokens = kStepTokens<DIMS>, kWords = kTokens / kWave, kPitch = kHoldPitch<DIMS>;
   const EvictCall& c = a.c;
@@ -291,14 +291,14 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictAr
   const uint8_t* base = plane + (head * c.head_dim + min(d0 + dim, static_cast<int32_t>(c.head_dim) - 1)) * bs * 2;
   const uint32_t block_bytes = static_cast<uint32_t>(c.cache_block_stride[kv]);
   auto column_of = [&](int32_t token) {
-    return shape.log_block >= 0 ? token >> shape.log_block : static_cast<int32_t>(static_cast<uint32_t>(token) / static_cast<uint32_t>(bs));
+    return POW2 ? token >> shape.log_block : static_cast<int32_t>(static_cast<uint32_t>(token) / static_cast<uint32_t>(bs));
   };
   auto entry_of = [&](int32_t token) -> uint32_t {  // of a position below len
     if constexpr (STAGED) return entries[column_of(token)];
     else return static_cast<uint32_t>(row_block(c, row, token));
   };
   auto address = [&](uint32_t entry, int32_t token) {
-    const int32_t place = shape.log_block >= 0 ? token & (bs - 1) : token - column_of(token) * bs;
+    const int32_t place = POW2 ? token & (bs - 1) : token - column_of(token) * bs;
     return base + static_cast<uint64_t>(entry) * block_bytes + place * 2;
   };
   auto mark_of = [&](int32_t word) {
@@ -432,9 +432,16 @@ hipError_t launch_evict(const EvictCall& c, hipStream_t stream) {
     // the longer pieces of memory of 8 dims are read a little faster (512 lines 280, against 305).
     const bool few = lines * ((c.head_dim + 7) / 8) < kFewWaves;
     const dim3 fine(lines, (c.head_dim + 15) / 16, 2);
-    if (staged > kMostStaged) evict_move_kernel<false, 8><<<grid, kBlockThreads, 0, stream>>>(a, shape);
-    else if (few) evict_move_kernel<true, 4><<<fine, kBlockThreads, staged, stream>>>(a, shape);
-    else evict_move_kernel<true, 8><<<grid, kBlockThreads, staged, stream>>>(a, shape);
+    if (staged > kMostStaged) {
+      if (shape.log_block >= 0) evict_move_kernel<false, 8, true><<<grid, kBlockThreads, 0, stream>>>(a, shape);
+      else evict_move_kernel<false, 8, false><<<grid, kBlockThreads, 0, stream>>>(a, shape);
+    } else if (shape.log_block < 0) {
+      if (few) evict_move_kernel<true, 4, false><<<fine, kBlockThreads, staged, stream>>>(a, shape);
+      else evict_move_kernel<true, 8, false><<<grid, kBlockThreads, staged, stream>>>(a, shape);
+    } else {
+      if (few) evict_move_kernel<true, 4, true><<<fine, kBlockThreads, staged, stream>>>(a, shape);
+      else evict_move_kernel<true, 8, true><<<grid, kBlockThreads, staged, stream>>>(a, shape);
+    }
   } else if (c.element_bytes == 1) evict_move_any_kernel<1><<<grid, kBlockThreads, 0, stream>>>(a);
   else if (c.element_bytes == 2) evict_move_any_kernel<2><<<grid, kBlockThreads, 0, stream>>>(a);
   else evict_move_any_kernel<4><<<grid, kBlockThreads, 0, stream>>>(a);
