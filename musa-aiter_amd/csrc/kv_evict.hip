@@ -4,6 +4,9 @@
 // of the lightest token that stays, then the tokens are marked (one bit each, in the workspace) and their weights moved.  The second moves the tokens' values.  A token's new position is never behind its old one, so a wave that
 // goes through a line in order, with a step's loads ahead of its stores, can move it in place; lines and head
 // dimensions are independent of each other.
+//
+// 8 sequences of 900 to 6000 tokens to 1024 in 8 layers (8 heads of 128 dims, bf16): decisions 33 us, moves 280 (4.2 TB/s
+// of the pages read and written).  One sequence of 40001 tokens to 8000 in two layers: 72 (16 workgroups) and 118.
 #include "kv_cache_attention.h"
 
 namespace kvhip {

@@ -1,6 +1,6 @@
 // Host-side argument handling of the operators on paged caches of plain values (third part of the _kv_host module), as
 // in kv_host_serving.cpp: the common arguments are checked, packed and passed on here, everything else is left to the
-// Python layer's checks with nothing launched.  One of these calls costs 5 to 6 us of host time, in Python about 35.
+// Python layer's checks with nothing launched.  One of these calls costs 6 us of host time, 20 less than in Python.
 #include <torch/extension.h>
 
 #include <cstdint>
