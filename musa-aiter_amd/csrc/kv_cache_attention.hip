@@ -198,7 +198,7 @@ struct Plan {
 };
 
 // Few rows: parts of whole turns of a workgroup, as many as make kRowsGroups workgroups (48 decode rows of 256 to 8192
-// tokens, us: 768 193, 1600 180, 2048 178 to 188 on other days, 4096 182, 8192 187; 16 rows of 2048 visible ones 55, then 48).
+// tokens, us: 768 193, 1600 180, 2048 178 to 188, 4096 182, 8192 187; 16 rows of 2048 visible ones 55, then 48).
 constexpr int64_t kTurnPlaces = kTilePlaces * kWavesPerBlock;
 constexpr int64_t kRowsGroups = 2048;
 constexpr int64_t kFewRows = 32;

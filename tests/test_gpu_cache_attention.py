@@ -343,3 +343,23 @@ def test_prompt_rows_over_a_long_prefix():
     case = Case(lens=[1500, 700, 333], rows=[600, 300, 333], heads=4, kv_heads=1, hd=64, window=250, sinks=20,
                 dtype="fp16", seed=22)
     case.check(*call(case))
+
+
+def test_addresses_that_are_no_multiples_of_16():
+    case = Case(lens=[100, 330, 8], rows=[3, 20, 2], heads=8, hd=128, window=90, sinks=7, seed=15)
+    query, key, value, tables, lens = case.args()
+
+    def odd(t):
+        flat = torch.zeros(t.numel() + 1, dtype=t.dtype, device=DEV)[1:].view(t.shape)
+        return flat.copy_(t)
+
+    for args in ((odd(query), key, value), (query, odd(key), value), (query, key, odd(value))):
+        case.check(*musa_aiter.kv_paged_attention(*args, tables, lens, **case.sight(), return_lse=True))
+    out = odd(query)
+    got, lse = musa_aiter.kv_paged_attention(query, key, value, tables, lens, **case.sight(), return_lse=True, out=out)
+    assert got is out
+    case.check(got, lse)
+    plain, moved = (torch.zeros((3, 2, 330), device=DEV) for _ in range(2))
+    musa_aiter.kv_accumulate_attention_weights(plain, query, key, tables, lens, lse, **case.sight())
+    musa_aiter.kv_accumulate_attention_weights(moved, odd(query), odd(key), tables, lens, odd(lse), **case.sight())
+    assert torch.allclose(plain, moved, rtol=1e-5)
