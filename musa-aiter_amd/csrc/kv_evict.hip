@@ -239,16 +239,12 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_any_kernel(const Evi
   }
 }
 
-// ----- moving 16-bit values of blocks of multiples of 8 tokens ---------------------------------------
-// A wave takes DIMS head dimensions of a line and goes through its tokens 512 / DIMS at a time: 16 bytes a lane, whole
+// ----- moving values of blocks whose rows are multiples of 16 bytes ------------------------------------
+// A wave takes 16 bytes of a token's dims (or 8) and goes through a line's tokens 64 (128) at a time: 16 bytes a lane, whole
 // pieces of the blocks' rows, kAhead steps on their way, the table entry of one more.  What stays is put behind one
 // another in LDS, and leaves it as many tokens at a time as 16 bytes a lane again.  Bound by the read of every block that keeps a token (lines
 // of 128 bytes hold the same 16 tokens of four dims, so single tokens are no cheaper to read).
 constexpr int kAhead = 8;
-template <int DIMS>
-constexpr int kStepTokens = 512 / DIMS;
-template <int DIMS>
-constexpr int kHoldPitch = 2 * kStepTokens<DIMS> + 8;  // tokens of a dim in LDS: less than a step's, and a step's more
 // Bytes of LDS for a table row and a line's marks.  Where they need more, each step reads its own from memory, which
 // waits for all loads that are on their way.
 constexpr int64_t kMostStaged = 96 * 1024;
@@ -260,13 +256,28 @@ struct MoveShape {
   int log_block;   // log2(block_size), or -1
 };
 
-template <bool STAGED, int DIMS, bool POW2>  // POW2: log_block is there
+template <int ELT>
+__device__ __forceinline__ typename VecType<ELT>::T element(const u32x4& v, int t) {
+  if constexpr (ELT == 1) return static_cast<uint8_t>(elem8(v, t));
+  else if constexpr (ELT == 2) return static_cast<uint16_t>(elem16(v, t));
+  else return v[t];
+}
+
+// Half the dims of a wave, twice the tokens of a step.
+template <int ELT, bool FEW>
+constexpr int kDimsOf = (FEW ? 8 : 16) / ELT;
+
+template <int ELT, bool FEW, bool STAGED, bool POW2>  // POW2: log_block is there
 __global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictArgs a, const MoveShape shape) {
-  constexpr int kTokens = kStepTokens<DIMS>, kWords = kTokens / kWave, kPitch = kHoldPitch<DIMS>;
+  using T = typename VecType<ELT>::T;
+  constexpr int kDims = kDimsOf<ELT, FEW>, kUnit = 16 / ELT;  // tokens of a lane
+  constexpr int kTokens = FEW ? 2 * kWave : kWave, kWords = kTokens / kWave;
+  constexpr int kPitch = 2 * kTokens + kUnit;  // tokens of a dim in LDS: less than a step's, and a step's more
+  constexpr uint32_t kUnitBits = (1u << kUnit) - 1;
   const EvictCall& c = a.c;
   const int64_t line = blockIdx.x;
   const int kv = blockIdx.z, lane = lane_id(), wave = wave_in_block();
-  __shared__ __attribute__((aligned(16))) uint16_t holds[kWavesPerBlock][DIMS * kPitch + 8];
+  __shared__ __attribute__((aligned(16))) T holds[kWavesPerBlock][kDims * kPitch + kUnit];
   extern __shared__ uint64_t marks[];  // the line's words, then the row's entries
   int32_t* entries = reinterpret_cast<int32_t*>(marks + a.words);
   const int64_t keep64 = uniform64(*line_keep(a, line));
@@ -282,16 +293,16 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictAr
     for (int32_t p = threadIdx.x; p < words; p += kBlockThreads) marks[p] = bits[p];
     __syncthreads();
   }
-  const int32_t d0 = (blockIdx.y * kWavesPerBlock + wave) * DIMS;
+  const int32_t d0 = (blockIdx.y * kWavesPerBlock + wave) * kDims;
   if (d0 >= c.head_dim) return;
-  // Lane: dim and unit of 8 tokens, pieces of a row of a block next to each other.
-  constexpr int kLogDims = __builtin_ctz(DIMS);
-  const int dim = lane >> shape.log_pieces & (DIMS - 1);
-  const int unit8 = 8 * ((lane & ((1 << shape.log_pieces) - 1)) |
-                         (lane >> (shape.log_pieces + kLogDims) << shape.log_pieces));
+  // Lane: dim and unit of tokens, pieces of a row of a block next to each other.
+  constexpr int kLogDims = __builtin_ctz(kDims);
+  const int dim = lane >> shape.log_pieces & (kDims - 1);
+  const int first = kUnit * ((lane & ((1 << shape.log_pieces) - 1)) |
+                             (lane >> (shape.log_pieces + kLogDims) << shape.log_pieces));
   const bool mine = d0 + dim < c.head_dim;
   const uint8_t* plane = static_cast<const uint8_t*>(c.cache[kv]) + layer * c.cache_layer_stride[kv];
-  const uint8_t* base = plane + (head * c.head_dim + min(d0 + dim, static_cast<int32_t>(c.head_dim) - 1)) * bs * 2;
+  const uint8_t* base = plane + (head * c.head_dim + min(d0 + dim, static_cast<int32_t>(c.head_dim) - 1)) * bs * ELT;
   const uint32_t block_bytes = static_cast<uint32_t>(c.cache_block_stride[kv]);
   auto column_of = [&](int32_t token) {
     return POW2 ? token >> shape.log_block : static_cast<int32_t>(static_cast<uint32_t>(token) / static_cast<uint32_t>(bs));
@@ -302,17 +313,17 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictAr
   };
   auto address = [&](uint32_t entry, int32_t token) {
     const int32_t place = POW2 ? token & (bs - 1) : token - column_of(token) * bs;
-    return base + static_cast<uint64_t>(entry) * block_bytes + place * 2;
+    return base + static_cast<uint64_t>(entry) * block_bytes + static_cast<uint64_t>(static_cast<uint32_t>(place)) * ELT;
   };
   auto mark_of = [&](int32_t word) {
     if constexpr (STAGED) return marks[min(word, words - 1)];
     else return bits[min(word, words - 1)];
   };
 
-  uint16_t* hold = holds[wave];
+  T* hold = holds[wave];
   const uint32_t mine_hold = dim * kPitch;
-  const uint32_t dump = DIMS * kPitch;  // where the values go that do not stay
-  const int bit0 = unit8 % kWave, my_word = unit8 / kWave;
+  const uint32_t dump = kDims * kPitch;  // where the values go that do not stay
+  const int bit0 = first % kWave, my_word = first / kWave;
   const uint64_t below = (uint64_t{1} << bit0) - 1;
   struct Marks {
     uint64_t of[kWords];
@@ -321,7 +332,7 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictAr
   u32x4 ahead[kAhead];
 #pragma unroll
   for (int k = 0; k < kWords; ++k) next_mark.of[k] = mark_of(k);
-  uint32_t next_entry = entry_of(min(unit8, len - 1));
+  uint32_t next_entry = entry_of(min(first, len - 1));
   auto mine_of = [&](const Marks& m) {
     uint64_t word = m.of[0];
 #pragma unroll
@@ -334,16 +345,16 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictAr
 #pragma unroll
     for (int k = 0; k < kWords; ++k)
       mark.of[k] = step * kWords + k < words ? static_cast<uint64_t>(uniform64(static_cast<int64_t>(next_mark.of[k]))) : 0;
-    const bool some = (mine_of(mark) >> bit0 & 0xFF) != 0;
-    values = ld16_cached(some ? address(next_entry, step * kTokens + unit8) : plane);
+    const bool some = (mine_of(mark) >> bit0 & kUnitBits) != 0;
+    values = ld16_cached(some ? address(next_entry, step * kTokens + first) : plane);
 #pragma unroll
     for (int k = 0; k < kWords; ++k) next_mark.of[k] = mark_of((step + 1) * kWords + k);
-    next_entry = entry_of(min((step + 1) * kTokens + unit8, len - 1));
+    next_entry = entry_of(min((step + 1) * kTokens + first, len - 1));
   };
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) issue(i, mark_ahead[i], ahead[i]);
   int32_t level = 0, out = 0;  // tokens in LDS, and those that left it
-  uint32_t out_entry = entry_of(min(unit8, len - 1));
+  uint32_t out_entry = entry_of(min(first, len - 1));
   for (int32_t step0 = 0; out + level < keep && step0 < steps; step0 += kAhead) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
@@ -353,7 +364,7 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictAr
       for (int k = 0; k < kWords; ++k) any |= mark.of[k];
       if (any != 0) {
         const uint64_t my_mark = mine_of(mark);
-        const uint32_t stay = static_cast<uint32_t>(my_mark >> bit0) & 0xFFu;
+        const uint32_t stay = static_cast<uint32_t>(my_mark >> bit0) & kUnitBits;
         uint32_t at = mine_hold + level + __popcll(my_mark & below);
 #pragma unroll
         for (int k = 0; k < kWords; ++k) {
@@ -361,48 +372,83 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_kernel(const EvictAr
           level += __popcll(mark.of[k]);
         }
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
+        for (int t = 0; t < kUnit; ++t) {
           const uint32_t bit = stay >> t & 1u;
-          hold[bit != 0 ? at : dump] = static_cast<uint16_t>(elem16(ahead[i], t));
+          hold[bit != 0 ? at : dump] = element<ELT>(ahead[i], t);
           at += bit;
         }
         __builtin_amdgcn_wave_barrier();
         if (level >= kTokens) {
-          u32x4* from = reinterpret_cast<u32x4*>(hold + mine_hold + unit8);
-          const u32x4 full = from[0], rest = from[kTokens / 8];
-          if (mine) st16_cached(const_cast<uint8_t*>(address(out_entry, out + unit8)), full);
+          u32x4* from = reinterpret_cast<u32x4*>(hold + mine_hold + first);
+          const u32x4 full = from[0], rest = from[kTokens / kUnit];
+          if (mine) st16_cached(const_cast<uint8_t*>(address(out_entry, out + first)), full);
           from[0] = rest;
           out += kTokens;
           level -= kTokens;
-          out_entry = entry_of(min(out + unit8, len - 1));
+          out_entry = entry_of(min(out + first, len - 1));
           __builtin_amdgcn_wave_barrier();
         }
       }
       issue(step0 + i + kAhead, mark_ahead[i], ahead[i]);
     }
   }
-  const int32_t left = keep - out - unit8;  // of this lane's last unit
+  const int32_t left = keep - out - first;  // of this lane's last unit
   if (mine && left > 0) {
-    const uint16_t* from = hold + mine_hold + unit8;
-    uint8_t* to = const_cast<uint8_t*>(address(out_entry, out + unit8));
-    if (left >= 8) st16_cached(to, *reinterpret_cast<const u32x4*>(from));
+    const T* from = hold + mine_hold + first;
+    uint8_t* to = const_cast<uint8_t*>(address(out_entry, out + first));
+    if (left >= kUnit) st16_cached(to, *reinterpret_cast<const u32x4*>(from));
     else
       for (int t = 0; t < left; ++t)
-        reinterpret_cast<KVHIP_GLOBAL uint16_t*>(reinterpret_cast<uint64_t>(to))[t] = from[t];
+        reinterpret_cast<KVHIP_GLOBAL T*>(reinterpret_cast<uint64_t>(to))[t] = from[t];
   }
 }
 
 // Whether evict_move_kernel takes the caches, and how.
 bool move_fits(const EvictCall& c, MoveShape& shape) {
-  if (c.element_bytes != 2 || c.block_size % 8 != 0) return false;
+  const int64_t unit = 16 / c.element_bytes;
+  if (c.block_size % unit != 0) return false;
   for (int kv = 0; kv < 2; ++kv)
     if (((reinterpret_cast<uint64_t>(c.cache[kv]) | c.cache_layer_stride[kv] | c.cache_block_stride[kv]) & 15) != 0 ||
         c.cache_block_stride[kv] < 0 || c.cache_block_stride[kv] >= int64_t{1} << 32)
       return false;
-  const int64_t pieces = c.block_size / 8;
+  const int64_t pieces = c.block_size / unit;
   shape.log_pieces = pieces % 8 == 0 ? 3 : pieces == 4 ? 2 : pieces == 2 ? 1 : 0;
   shape.log_block = (c.block_size & (c.block_size - 1)) == 0 ? __builtin_ctzll(c.block_size) : -1;
   return true;
+}
+
+template <int ELT, bool FEW>
+void launch_move(const EvictArgs& a, MoveShape shape, hipStream_t stream) {
+  const EvictCall& c = a.c;
+  constexpr int kLogUnits = __builtin_ctz(kWave / kDimsOf<ELT, FEW>);  // of a step
+  if (shape.log_pieces > kLogUnits) shape.log_pieces = kLogUnits;
+  constexpr int kSlice = kDimsOf<ELT, FEW> * kWavesPerBlock;
+  const dim3 grid(a.lines, (c.head_dim + kSlice - 1) / kSlice, 2);
+  const int64_t staged = a.words * 8 + c.max_blocks * 4;
+  const bool pow2 = shape.log_block >= 0;
+  if (staged > kMostStaged) {
+    if (pow2) evict_move_kernel<ELT, FEW, false, true><<<grid, kBlockThreads, 0, stream>>>(a, shape);
+    else evict_move_kernel<ELT, FEW, false, false><<<grid, kBlockThreads, 0, stream>>>(a, shape);
+  } else {
+    if (pow2) evict_move_kernel<ELT, FEW, true, true><<<grid, kBlockThreads, staged, stream>>>(a, shape);
+    else evict_move_kernel<ELT, FEW, true, false><<<grid, kBlockThreads, staged, stream>>>(a, shape);
+  }
+}
+
+template <int ELT>
+void launch_moves(const EvictArgs& a, hipStream_t stream) {
+  const EvictCall& c = a.c;
+  MoveShape shape{};
+  if (move_fits(c, shape)) {
+    // Few waves: half the dims each, twice the tokens a step (40001 tokens of 16 lines, 16 bits: 137 us, against 215).
+    // With many the longer pieces of memory are read a little faster (512 lines 280, against 305).
+    const int64_t waves = a.lines * ((c.head_dim + kDimsOf<ELT, false> - 1) / kDimsOf<ELT, false>);
+    if (waves < kFewWaves) launch_move<ELT, true>(a, shape, stream);
+    else launch_move<ELT, false>(a, shape, stream);
+    return;
+  }
+  const int64_t slices = (c.head_dim + kMoveDims * kWavesPerBlock - 1) / (kMoveDims * kWavesPerBlock);
+  evict_move_any_kernel<ELT><<<dim3(a.lines, slices, 2), kBlockThreads, 0, stream>>>(a);
 }
 
 EvictArgs evict_args(const EvictCall& c) {
@@ -426,28 +472,9 @@ hipError_t launch_evict(const EvictCall& c, hipStream_t stream) {
   evict_select_kernel<<<dim3(lines), kSelectThreads, 0, stream>>>(a);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  const int64_t slices = (c.head_dim + kMoveDims * kWavesPerBlock - 1) / (kMoveDims * kWavesPerBlock);
-  const dim3 grid(lines, slices, 2);
-  MoveShape shape{};
-  const int64_t staged = a.words * 8 + c.max_blocks * 4;
-  if (move_fits(c, shape)) {
-    // Few waves: half the dims each, twice the tokens a step (40001 tokens of 16 lines 137 us, against 215).  With many
-    // the longer pieces of memory of 8 dims are read a little faster (512 lines 280, against 305).
-    const bool few = lines * ((c.head_dim + 7) / 8) < kFewWaves;
-    const dim3 fine(lines, (c.head_dim + 15) / 16, 2);
-    if (staged > kMostStaged) {
-      if (shape.log_block >= 0) evict_move_kernel<false, 8, true><<<grid, kBlockThreads, 0, stream>>>(a, shape);
-      else evict_move_kernel<false, 8, false><<<grid, kBlockThreads, 0, stream>>>(a, shape);
-    } else if (shape.log_block < 0) {
-      if (few) evict_move_kernel<true, 4, false><<<fine, kBlockThreads, staged, stream>>>(a, shape);
-      else evict_move_kernel<true, 8, false><<<grid, kBlockThreads, staged, stream>>>(a, shape);
-    } else {
-      if (few) evict_move_kernel<true, 4, true><<<fine, kBlockThreads, staged, stream>>>(a, shape);
-      else evict_move_kernel<true, 8, true><<<grid, kBlockThreads, staged, stream>>>(a, shape);
-    }
-  } else if (c.element_bytes == 1) evict_move_any_kernel<1><<<grid, kBlockThreads, 0, stream>>>(a);
-  else if (c.element_bytes == 2) evict_move_any_kernel<2><<<grid, kBlockThreads, 0, stream>>>(a);
-  else evict_move_any_kernel<4><<<grid, kBlockThreads, 0, stream>>>(a);
+  if (c.element_bytes == 1) launch_moves<1>(a, stream);
+  else if (c.element_bytes == 2) launch_moves<2>(a, stream);
+  else launch_moves<4>(a, stream);
   return hipGetLastError();
 }
 

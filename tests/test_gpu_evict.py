@@ -150,28 +150,33 @@ def test_nothing_to_do():
     assert kept.shape == (0,)
 
 
-def test_many_lines():
-    """512 lines of 64 dims: the form with eight dims a wave."""
-    Case(lens=[70, 300, 129, 64, 65, 200, 17, 1], keep=[20, 100, 128, 30, 64, 50, 3, 1], layers=8, kv_heads=8, hd=64,
-         seed=14).check(sinks=2, recent=9)
+@pytest.mark.parametrize("size,hd", [(1, 128), (2, 64), (4, 32)])
+@pytest.mark.parametrize("bs", [8, 16, 24, 32, 64, 128])
+def test_many_lines(size, hd, bs):
+    """512 lines: the form with 16 bytes of dims a wave."""
+    Case(lens=[70, 300, 129, 64, 65, 200, 17, 1], keep=[20, 100, 128, 30, 64, 50, 3, 1], layers=8, kv_heads=8, hd=hd, bs=bs,
+         size=size, seed=14).check(sinks=2, recent=9)
 
 
+@pytest.mark.parametrize("size", [1, 2, 4])
 @pytest.mark.parametrize("bs,extra", [(8, 7000), (8, 14000), (8, 30000), (64, 1400), (16, 200000)])
-def test_long_table_rows(bs, extra):
+def test_long_table_rows(bs, extra, size):
     """Rows whose entries and marks take 70 KiB of LDS and more, up to none that would hold them."""
-    case = Case(lens=[500, 77], keep=[200, 30], bs=bs, seed=bs)
+    case = Case(lens=[500, 77], keep=[200, 30], bs=bs, size=size, seed=bs)
     case.tables = np.concatenate([case.tables, np.full((2, extra), -1, dtype=np.int64)], axis=1)
     case.check(sinks=2, recent=9)
 
 
 def test_one_dim_more_than_a_slice():
-    for hd in (4, 5, 12, 36, 100):
-        Case(lens=[300], keep=[77], hd=hd, layers=None, seed=hd).check(recent=5)
+    for size in (1, 2, 4):
+        for hd in (4, 5, 12, 36, 100):
+            Case(lens=[300], keep=[77], hd=hd, layers=None, size=size, seed=hd).check(recent=5)
 
 
 def test_dense_and_sparse_marks():
-    for keep in (1, 5, 64, 128, 1000, 1990, 1999):
-        Case(lens=[2000], keep=[keep], layers=None, seed=keep).check()
+    for size in (1, 2, 4):
+        for keep in (1, 5, 64, 128, 1000, 1990, 1999):
+            Case(lens=[2000], keep=[keep], layers=None, size=size, seed=keep).check()
     case = Case(lens=[2000], keep=[1000], layers=None, seed=3)
     case.weights[..., ::2] = 1.0
     case.weights[..., 1::2] = 2.0
