@@ -36,8 +36,8 @@ struct CacheArgs {
 };
 
 // Weights are 2^(score - maximum + kTop): fp16 ones keep their 11 bits down to 2^-28 of the largest, and sums of the
-// largest bf16 and float32 values times weights stay finite for up to 2^20 tokens (a row's maximum may pass the reference by 2^8 for
-// a while).  The same factor is in their sum.
+// largest bf16 and float32 values times weights stay finite for up to 2^20 tokens (a row's maximum may pass the
+// reference by 2^8 for a while).  The same factor is in their sum.
 template <int DT>
 constexpr float kTop = DT == kLinF16 ? 14.0f : -28.0f;
 
@@ -224,7 +224,7 @@ __device__ __forceinline__ void visit_row(const CacheArgs& a, const View& w, int
   }
 }
 
-// m * x with m possibly -inf on both sides of a difference.
+// 2^(m - top), with m and top possibly both -inf.
 __device__ __forceinline__ float fade_to(float m, float top) {
   return m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
 }

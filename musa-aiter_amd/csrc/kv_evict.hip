@@ -1,9 +1,10 @@
 // Eviction from a paged cache by gathered attention weight: kv_evict_paged_tokens.
 //
 // Two launches.  The first decides, one workgroup per line (a layer, row and kv head): a radix select finds the weight
-// of the lightest token that stays, then the tokens are marked (one bit each, in the workspace) and their weights moved.  The second moves the tokens' values.  A token's new position is never behind its old one, so a wave that
-// goes through a line in order, with a step's loads ahead of its stores, can move it in place; lines and head
-// dimensions are independent of each other.
+// of the lightest token that stays, then the tokens are marked (one bit each, in the workspace) and their weights moved.
+// The second moves the tokens' values.  A token's new position is never behind its old one, so a wave that goes through a
+// line in order, with a step's loads ahead of its stores, can move it in place; lines and head dimensions are independent
+// of each other.
 //
 // 8 sequences of 900 to 6000 tokens to 1024 in 8 layers (8 heads of 128 dims, bf16): decisions 33 us, moves 280 (4.2 TB/s
 // of the pages read and written).  One sequence of 40001 tokens to 8000 in two layers: 72 (16 workgroups) and 118.
@@ -44,7 +45,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 // The deciding launch: 16 waves of a workgroup take a 16th of the line each, 64 positions at a time; the first kHeld
-// steps stay in registers (lines of up to 8192 tokens are read once).  Three digits of 11, 11 and 10 bits: 2048 bins, two a
+// steps stay in registers (lines of up to 8192 tokens are read once; with 32 steps, and five loops of
+// as many copies, 24 lines of up to 500 tokens took 22 us instead of 11).  Three digits of 11, 11 and 10 bits: 2048 bins, two a
 // thread.
 constexpr int kSelectWaves = 16;
 constexpr int kSelectThreads = kSelectWaves * kWave;
@@ -242,8 +244,8 @@ __global__ __launch_bounds__(kBlockThreads) void evict_move_any_kernel(const Evi
 // ----- moving values of blocks whose rows are multiples of 16 bytes ------------------------------------
 // A wave takes 16 bytes of a token's dims (or 8) and goes through a line's tokens 64 (128) at a time: 16 bytes a lane, whole
 // pieces of the blocks' rows, kAhead steps on their way, the table entry of one more.  What stays is put behind one
-// another in LDS, and leaves it as many tokens at a time as 16 bytes a lane again.  Bound by the read of every block that keeps a token (lines
-// of 128 bytes hold the same 16 tokens of four dims, so single tokens are no cheaper to read).
+// another in LDS, and leaves it as many tokens at a time as 16 bytes a lane again.  Bound by the read of every block that
+// keeps a token (lines of 128 bytes hold the same 16 tokens of four dims, so single tokens are no cheaper to read).
 constexpr int kAhead = 8;
 // Bytes of LDS for a table row and a line's marks.  Where they need more, each step reads its own from memory, which
 // waits for all loads that are on their way.
