@@ -24,7 +24,6 @@ last n tokens; head h reads kv head ``h // (heads // kv_heads)``.
 
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -331,7 +330,6 @@ def _plain_evict(s: dict) -> list:
 # ----- the framework's calls --------------------------------------------------------------------
 
 
-@functools.cache
 def _framework():
     package = str(Path(__file__).resolve().parents[1] / "musa-aiter_amd")
     if package not in sys.path:
