@@ -8,10 +8,12 @@
 //   * K is brought in by lanes that each read 4 rows of 16 bytes, d = 32 k + 16 h + 4 i + g, i = 0..3 (four rows of a
 //     block, a 128-byte line, in an instruction), and turned with byte permutes into 4 dims of each of the 8 tokens.
 // The next tile's loads are on their way while a tile is worked on, in registers; two tiles of LDS leave one barrier a
-// tile.  Bound by vector instructions (about seven for a score, one of them an exponential of a quarter of the rate) next
-// to the matrix ones, and by LDS reads of as many cycles as the matrix instructions take.  A weight is rounded to the
-// caches' type once: the two summands of the form for few rows would make half of all products twice.  Chunks of 1500 and
-// 2048 rows with a window of 4000 (32 heads, 8 in the cache, 128 dims, bf16): 327 us, 760 TFLOP/s.
+// tile.  A weight goes in as two summands of the caches' type, as in the form for few rows: rounded once, a row's output
+// would be off by 2^-8 of its values (bf16), and by how much would go with the form that its neighbours in the call bring
+// about.  Bound by vector instructions (about nine for a score, one of them an exponential of a quarter of the rate) next to
+// the matrix ones: matrix units busy 35 % of the time, vector ones 49 %, 1.6 waves a SIMD on average.  Chunks of 1753 and
+// 2048 rows with a window of 4000 (32 heads, 8 in the cache, 128 dims, bf16): 434 us, 575 TFLOP/s without the second
+// products; with one summand 329.
 #include "kv_cache_attention_tiles.h"
 
 namespace kvhip {
@@ -221,7 +223,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
         m[nt] = top[nt];
       }
     }
-    u32x4 weight[2][2];
+    u32x4 weight[2][2][2];  // half, row tile, summand
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt) {
       const float ref = (m[nt] == -__builtin_inff() ? 0.0f : m[nt]) - kTop<DT>;
@@ -232,7 +234,10 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
           const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nt][j][r], a.factor, -ref));
           const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nt][j][r + 1], a.factor, -ref));
           l[nt] += p0 + p1;
-          weight[nt][j >> 1][2 * (j & 1) + (r >> 1)] = Mma16<DT>::pack(p0, p1);
+          const uint32_t high = Mma16<DT>::pack(p0, p1);
+          const f32x2 back = Mma16<DT>::unpack(high);
+          weight[j >> 1][nt][0][2 * (j & 1) + (r >> 1)] = high;
+          weight[j >> 1][nt][1][2 * (j & 1) + (r >> 1)] = Mma16<DT>::pack(p0 - back.x, p1 - back.y);
         }
     }
 #pragma unroll
@@ -242,7 +247,10 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
     for (int n = 0; n < 2 * kDimTiles; ++n) {
       const int half = n / kDimTiles, dt = n % kDimTiles;
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) acc[nt][dt] = Mma16<DT>::mma(operand[n % kReads], weight[nt][half], acc[nt][dt]);
+      for (int summand = 0; summand < 2; ++summand)
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+          acc[nt][dt] = Mma16<DT>::mma(operand[n % kReads], weight[half][nt][summand], acc[nt][dt]);
       if (n + kReads < 2 * kDimTiles)
         operand[n % kReads] = at.values[(n + kReads) / kDimTiles][(n + kReads) % kDimTiles][lane];
       __builtin_amdgcn_sched_barrier(0);

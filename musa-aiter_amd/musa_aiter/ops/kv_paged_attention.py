@@ -158,8 +158,9 @@ def kv_paged_attention(
     ``return_lse`` also the float32 ``[T, heads]`` logarithms of the rows' softmax sums.  There is no backward pass:
     the output carries no gradient, also where ``query`` requires one.
 
-    Scores, softmax statistics and sums are float32.  With 16-bit caches a weight is rounded to their type (float16
-    weights keep its 11 bits down to 2**-28 of a row's largest, bfloat16 ones 8 bits); with float32 ones nothing is.
+    Scores, softmax statistics and sums are float32.  With 16-bit caches a weight enters its products as two numbers of
+    their type, 2**-16 (float16 2**-22) of it off at most; float16 ones lose what lies below 2**-28 of a row's largest.
+    With float32 caches no weight is rounded.
     """
     op = "kv_paged_attention"
     sight = _native_sight(query, max_seq_len, softmax_scale, window, sinks)
