@@ -43,7 +43,8 @@ __global__ __launch_bounds__(kBlockThreads) void weights_any_kernel(const CacheA
       float dot = 0.0f;
       for (int64_t d = 0; d < hd; ++d) dot = __builtin_fmaf(q[d], load_q<DT>(c.cache[0], k + d * bs), dot);
       // The difference first: it is small where a weight is large, and its product then loses nothing.
-      sum += __builtin_amdgcn_exp2f(__builtin_fmaf(dot, a.scale, -lse) * kLog2e);
+      const float less = __builtin_fmaf(dot, a.scale_rest, __builtin_fmaf(dot, a.scale, -lse));
+      sum += __builtin_amdgcn_exp2f(less * kLog2e);
     }
     if (k >= 0) {
       float* to = a.weights + seq * a.weight_row_stride + head * a.weight_head_stride + token;
@@ -151,7 +152,11 @@ __global__ __launch_bounds__(WAVES * kWave, HD <= 128 ? 2 : 1) void weights_tile
     };
     if (at0 < rows) fetch(at0);
     for (; at0 < rows; at0 += step) {
-      const float lse = next_lse, less = lse * kLog2e;
+      // e^(score - lse) is 2^(score * factor - less) times what the rounding of less leaves: for logarithms of thousands
+      // it is off by 2^-11 and more.  It goes into the sums as their factor, at no instruction a score.
+      const float lse = next_lse, less = lse * a.lse_factor;
+      const float rest = __builtin_isfinite(less) ? __builtin_fmaf(lse, a.lse_rest, __builtin_fmaf(lse, a.lse_factor, -less)) : 0.0f;
+      const float give = __builtin_amdgcn_exp2f(-rest);
       u32x4 rows16[kSteps];
 #pragma unroll
       for (int ks = 0; ks < kSteps; ++ks) rows16[ks] = next16[ks];
@@ -188,7 +193,9 @@ __global__ __launch_bounds__(WAVES * kWave, HD <= 128 ? 2 : 1) void weights_tile
             for (int r = 0; r < 4; ++r) s[t][r] = (seen[r] >> (t0 + t) & 1u) != 0 ? s[t][r] : 0.0f;
         }
 #pragma unroll
-        for (int t = 0; t < kAtOnce; ++t) sum[t0 + t] += s[t];
+        for (int t = 0; t < kAtOnce; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum[t0 + t][r] = __builtin_fmaf(s[t][r], give, sum[t0 + t][r]);
       }
     }
 #pragma unroll

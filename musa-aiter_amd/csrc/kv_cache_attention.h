@@ -33,6 +33,10 @@ struct CacheArgs {
   int32_t tiles;         // row tiles of the launch
   int64_t lines;         // (row tile, kv head) pairs, or (row, head) pairs of the form for any shape
   float scale, factor;   // softmax_scale, and times log2(e)
+  // What float32 takes from the two: scale + scale_rest is softmax_scale, lse_factor + lse_rest is factor / softmax_scale
+  // (log2(e), with the rounding that factor has), so that (score * factor) - lse * (factor / scale) is small where
+  // score * scale - lse is, however large the two are.
+  float scale_rest, lse_factor, lse_rest;
 };
 
 // Weights are 2^(score - maximum + kTop): fp16 ones keep their 11 bits down to 2^-28 of the largest, and sums of the

@@ -339,6 +339,11 @@ CacheArgs cache_args(const CacheAttnCall& c, int size) {
   a.sinks = static_cast<int32_t>(c.sinks < kMostRoom ? c.sinks : kMostRoom);
   a.scale = static_cast<float>(c.softmax_scale);
   a.factor = static_cast<float>(c.softmax_scale * 1.4426950408889634);
+  const bool ratio = a.factor != 0.0f && __builtin_isfinite(a.factor);
+  const double per_lse = ratio ? a.factor / c.softmax_scale : 1.4426950408889634;
+  a.lse_factor = static_cast<float>(per_lse);
+  a.lse_rest = static_cast<float>(per_lse - a.lse_factor);
+  a.scale_rest = __builtin_isfinite(a.scale) ? static_cast<float>(c.softmax_scale - a.scale) : 0.0f;
   return a;
 }
 
