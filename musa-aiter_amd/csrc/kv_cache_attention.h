@@ -39,11 +39,12 @@ struct CacheArgs {
   float scale_rest, lse_factor, lse_rest;
 };
 
-// Weights are 2^(score - maximum + kTop): fp16 ones keep their 11 bits down to 2^-28 of the largest, and sums of the
-// largest bf16 and float32 values times weights stay finite for up to 2^20 tokens (a row's maximum may pass the
-// reference by 2^8 for a while).  The same factor is in their sum.
+// Weights are 2^(score - m), with m a row's maximum so far less kTop: fp16 ones keep their 11 bits down to 2^-28 of the
+// largest.  The others have float32's range, and a weight of one for the maximum, so that products with its smallest
+// values stay normal numbers; where sums with its largest ones pass its range, a row is done once more (see visit_row).
+// Waves and parts hand on (m, l, o): the sum of the row's weights is l * 2^m, o what they make of the values.
 template <int DT>
-constexpr float kTop = DT == kLinF16 ? 14.0f : -28.0f;
+constexpr float kTop = DT == kLinF16 ? 14.0f : 0.0f;
 
 // Positions that the rows of a tile see between them, as an axis without the gap between the first tokens and the
 // window: place v is position v below `front`, v + gap from there on.  `front` and the window's begin are rounded to
@@ -146,7 +147,7 @@ __device__ __forceinline__ Span part_places(const CacheArgs& a, int32_t length, 
   return {lo, s + 1 < count ? lo + a.part : length};
 }
 
-// Workspace: (m, l) of every part's rows, their acc of head_dim values each, and a Line for each line.
+// Workspace: (m, l) of every part's rows, their outputs of head_dim values each, and a Line for each line.
 struct Line {
   int32_t parts, first, count, base;  // parts 0: no rows
 };
@@ -157,11 +158,11 @@ __device__ __forceinline__ int64_t slot_row(const CacheArgs& a, int64_t line, in
 __device__ __forceinline__ float* slot_ml(const CacheArgs& a, int64_t at) {
   return static_cast<float*>(a.r.c.workspace) + 2 * at;
 }
-__device__ __forceinline__ float* slot_acc(const CacheArgs& a, int64_t at) {
+__device__ __forceinline__ float* slot_out(const CacheArgs& a, int64_t at) {
   return static_cast<float*>(a.r.c.workspace) + 2 * a.lines * a.parts * a.slot_rows + at * a.r.hd;
 }
 __device__ __forceinline__ Line* line_of(const CacheArgs& a, int64_t line) {
-  return reinterpret_cast<Line*>(slot_acc(a, a.lines * a.parts * a.slot_rows)) + line;
+  return reinterpret_cast<Line*>(slot_out(a, a.lines * a.parts * a.slot_rows)) + line;
 }
 
 // ----- float32 throughout, one row: the form for any shape, and what a tile falls back to --------
@@ -174,11 +175,16 @@ struct VisitScratch {
 };
 
 // One row's (m, l) and acc (dims lane + 64 i) over the places lo, lo + 1, .. of 64 at a time, `step` apart.  q: the
-// row's query, in LDS.
+// row's query, in LDS.  l and acc are 2^-lower of what m says.  Sums over float32's largest values may be infinite with
+// lower 0: a dim whose output is then no finite number is taken from a second visit with kLower, where such sums of up
+// to 2^28 tokens are finite (and where the smallest values would be lost).
+constexpr float kLower = 28.0f;
+
 template <int DT, int DIMS>
 __device__ __forceinline__ void visit_row(const CacheArgs& a, const View& w, int32_t seq, const RowSight& row,
                                           int32_t kv_head, const float* q, int32_t lo, int32_t hi, int32_t step,
-                                          VisitScratch& scratch, float& m, float& l, float (&acc)[DIMS / kWave]) {
+                                          float lower, VisitScratch& scratch, float& m, float& l,
+                                          float (&acc)[DIMS / kWave]) {
   const AttnCall& c = a.r.c;
   const int lane = lane_id();
   const int64_t bs = a.r.bs, hd = a.r.hd;
@@ -207,7 +213,7 @@ __device__ __forceinline__ void visit_row(const CacheArgs& a, const View& w, int
     const float top = fmaxf(m, wave_max(s));
     const float ref = top == -__builtin_inff() ? 0.0f : top;
     // A masked position's score is -inf; with a row's maximum of +inf its weight would be no number.
-    const float p = off >= 0 ? __builtin_amdgcn_exp2f(s - ref + kTop<DT>) : 0.0f;
+    const float p = off >= 0 ? __builtin_amdgcn_exp2f(s - ref - lower) : 0.0f;
     const float fade = __builtin_amdgcn_exp2f(m - ref);
     m = top;
     l = l * fade + wave_sum(p);
@@ -233,9 +239,8 @@ __device__ __forceinline__ float fade_to(float m, float top) {
   return m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
 }
 
-template <int DT>
 __device__ __forceinline__ float log_sum(float m, float l) {
-  return l == 0.0f ? -__builtin_inff() : (m - kTop<DT> + log2f(l)) * kLn2;
+  return l == 0.0f ? -__builtin_inff() : (m + log2f(l)) * kLn2;
 }
 
 // Arguments of a launch in tiles of `size` rows (0: the form for any shape, a line per row and head).

@@ -4,7 +4,7 @@
 //   o_d = sum_j e^(s_j - lse) V[blk(j), h, d, j % bs]
 //
 // over the positions j that the row sees.  One pass over the cache with a running maximum and sum in base 2; parts of a
-// line (a row tile and a kv head) that run side by side leave (m, l, acc) in a workspace and a second launch joins them.
+// line (a row tile and a kv head) that run side by side leave (m, l, o) in a workspace and a second launch joins them.
 #include "kv_cache_attention_tiles.h"
 
 namespace kvhip {
@@ -45,45 +45,63 @@ __global__ __launch_bounds__(kBlockThreads) void cache_any_kernel(const CacheArg
   for (int64_t d = threadIdx.x; d < c.head_dim; d += kBlockThreads)
     q[d] = load_q<DT>(c.query, t * c.query_row_stride + hq * c.query_head_stride + d);
   __syncthreads();
-  float m, l, acc[kVisitDims / kWave];
   const RowSight sight = row_sight(a, w, first, i);
-  visit_row<DT, kVisitDims>(a, w, seq, sight, static_cast<int32_t>(hq) / a.r.group, q,
-                            static_cast<int32_t>(span.lo) + wave * kWave, static_cast<int32_t>(span.hi), kBlockThreads,
-                            scratch[wave], m, l, acc);
-  if (lane == 0) {
-    m_of[wave] = m;
-    l_of[wave] = l;
+  const int64_t at = slot_row(a, line, part, 0);
+  constexpr int kMine = kVisitDims / kBlockThreads;
+  float out[kMine] = {};
+  for (float lower = 0.0f;; lower = kLower) {
+    float m, l, acc[kVisitDims / kWave];
+    visit_row<DT, kVisitDims>(a, w, seq, sight, static_cast<int32_t>(hq) / a.r.group, q,
+                              static_cast<int32_t>(span.lo) + wave * kWave, static_cast<int32_t>(span.hi), kBlockThreads,
+                              lower, scratch[wave], m, l, acc);
+    if (lane == 0) {
+      m_of[wave] = m;
+      l_of[wave] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < kVisitDims / kWave; ++i)
+      if (lane + i * kWave < c.head_dim) acc_of[wave][lane + i * kWave] = acc[i];
+    __syncthreads();
+    float top = m_of[0];
+    for (int x = 1; x < kWavesPerBlock; ++x) top = fmaxf(top, m_of[x]);
+    float fade[kWavesPerBlock], sum = 0.0f;
+    for (int x = 0; x < kWavesPerBlock; ++x) {
+      fade[x] = fade_to(m_of[x], top);
+      sum += l_of[x] * fade[x];
+    }
+    bool over = false;
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      const int64_t d = threadIdx.x + k * kBlockThreads;
+      if (d >= c.head_dim) break;
+      float o = 0.0f;
+      for (int x = 0; x < kWavesPerBlock; ++x) o += acc_of[x][d] * fade[x];
+      if (lower == 0.0f || !__builtin_isfinite(out[k])) out[k] = sum == 0.0f ? 0.0f : o / sum;
+      over |= !__builtin_isfinite(out[k]);
+    }
+    if (lower == 0.0f && threadIdx.x == 0) {
+      if (count > 1) {
+        slot_ml(a, at)[0] = top;
+        slot_ml(a, at)[1] = sum;
+      } else if (c.lse != nullptr) {
+        c.lse[line] = log_sum(top, sum);
+      }
+    }
+    if (DT == kLinF16 || lower != 0.0f || !__builtin_isfinite(sum)) break;
+    if (__syncthreads_or(over) == 0) break;
   }
 #pragma unroll
-  for (int i = 0; i < kVisitDims / kWave; ++i)
-    if (lane + i * kWave < c.head_dim) acc_of[wave][lane + i * kWave] = acc[i];
-  __syncthreads();
-  float top = m_of[0];
-  for (int x = 1; x < kWavesPerBlock; ++x) top = fmaxf(top, m_of[x]);
-  float fade[kWavesPerBlock], sum = 0.0f;
-  for (int x = 0; x < kWavesPerBlock; ++x) {
-    fade[x] = fade_to(m_of[x], top);
-    sum += l_of[x] * fade[x];
-  }
-  const int64_t at = slot_row(a, line, part, 0);
-  for (int64_t d = threadIdx.x; d < c.head_dim; d += kBlockThreads) {
-    float o = 0.0f;
-    for (int x = 0; x < kWavesPerBlock; ++x) o += acc_of[x][d] * fade[x];
-    if (count > 1) slot_acc(a, at)[d] = o;
-    else store_o<DT>(c.out, line * c.head_dim + d, sum == 0.0f ? 0.0f : o / sum);
-  }
-  if (threadIdx.x == 0) {
-    if (count > 1) {
-      slot_ml(a, at)[0] = top;
-      slot_ml(a, at)[1] = sum;
-    } else if (c.lse != nullptr) {
-      c.lse[line] = log_sum<DT>(top, sum);
-    }
+  for (int k = 0; k < kMine; ++k) {
+    const int64_t d = threadIdx.x + k * kBlockThreads;
+    if (d >= c.head_dim) break;
+    if (count > 1) slot_out(a, at)[d] = out[k];
+    else store_o<DT>(c.out, line * c.head_dim + d, out[k]);
   }
 }
 
 // ----- join -----------------------------------------------------------------------------------------
-// One workgroup per row of a line.  Its waves take the parts in turn, in the same order in every run.
+// The mean of the parts' outputs, weighted by their sums.  One workgroup per row of a line.  Its waves take the parts in
+// turn, in the same order in every run.
 template <int DT>
 __global__ __launch_bounds__(kBlockThreads) void cache_join_kernel(const CacheArgs a) {
   const AttnCall& c = a.r.c;
@@ -114,30 +132,33 @@ __global__ __launch_bounds__(kBlockThreads) void cache_join_kernel(const CacheAr
   __syncthreads();
   for (int k = 0; k < kWavesPerBlock; ++k) top = fmaxf(top, top_of[k]);
   float acc[kVisitDims / kWave] = {}, sum = 0.0f;
-  const float* part = slot_acc(a, slot_row(a, line, 0, x));
+  for (int32_t s = threadIdx.x; s < info.parts; s += kBlockThreads) sum += ml[s * pitch + 1] * fade_to(ml[s * pitch], top);
+  sum = wave_sum(sum);
+  if (lane == 0) sum_of[wave] = sum;
+  __syncthreads();
+  sum = 0.0f;
+  for (int k = 0; k < kWavesPerBlock; ++k) sum += sum_of[k];
+  const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float* part = slot_out(a, slot_row(a, line, 0, x));
   const int64_t step = static_cast<int64_t>(a.slot_rows) * c.head_dim;
 #pragma unroll 4
   for (int32_t s = wave; s < info.parts; s += kWavesPerBlock) {
-    const float fade = fade_to(ml[s * pitch], top);
-    sum += ml[s * pitch + 1] * fade;
+    const float share = ml[s * pitch + 1] * fade_to(ml[s * pitch], top) * scale;
 #pragma unroll
     for (int i = 0; i < kVisitDims / kWave; ++i)
-      if (lane + i * kWave < c.head_dim) acc[i] = __builtin_fmaf(part[s * step + lane + i * kWave], fade, acc[i]);
+      if (lane + i * kWave < c.head_dim) acc[i] = __builtin_fmaf(part[s * step + lane + i * kWave], share, acc[i]);
   }
-  if (lane == 0) sum_of[wave] = sum;
 #pragma unroll
   for (int i = 0; i < kVisitDims / kWave; ++i)
     if (lane + i * kWave < c.head_dim) acc_of[wave][lane + i * kWave] = acc[i];
   __syncthreads();
-  sum = 0.0f;
-  for (int k = 0; k < kWavesPerBlock; ++k) sum += sum_of[k];
   const int64_t out = row * c.heads + head;
   for (int64_t d = threadIdx.x; d < c.head_dim; d += kBlockThreads) {
     float o = 0.0f;
     for (int k = 0; k < kWavesPerBlock; ++k) o += acc_of[k][d];
-    store_o<DT>(c.out, out * c.head_dim + d, sum == 0.0f ? 0.0f : o / sum);
+    store_o<DT>(c.out, out * c.head_dim + d, o);
   }
-  if (threadIdx.x == 0 && c.lse != nullptr) c.lse[out] = log_sum<DT>(top, sum);
+  if (threadIdx.x == 0 && c.lse != nullptr) c.lse[out] = log_sum(top, sum);
 }
 
 // The same with a wave per row, for few parts (the rows of 16 trees in three parts: 14 us, with a workgroup each 36).
@@ -152,25 +173,26 @@ __global__ __launch_bounds__(kBlockThreads) void cache_join_few_kernel(const Cac
   const int64_t row = info.first + at / a.r.group, head = (line % c.kv_heads) * a.r.group + at % a.r.group;
   const int lane = lane_id();
   const float* ml = slot_ml(a, slot_row(a, line, 0, x));
-  const float* part = slot_acc(a, slot_row(a, line, 0, x));
+  const float* part = slot_out(a, slot_row(a, line, 0, x));
   const int64_t pitch = 2 * static_cast<int64_t>(a.slot_rows), step = static_cast<int64_t>(a.slot_rows) * c.head_dim;
   float top = -__builtin_inff(), sum = 0.0f;
   for (int32_t s = 0; s < info.parts; ++s) top = fmaxf(top, ml[s * pitch]);
+  for (int32_t s = 0; s < info.parts; ++s) sum += ml[s * pitch + 1] * fade_to(ml[s * pitch], top);
+  const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
   constexpr int kDims = 256 / kWave;  // of the forms in tiles
   float acc[kDims] = {};
   for (int32_t s = 0; s < info.parts; ++s) {
-    const float fade = fade_to(ml[s * pitch], top);
-    sum += ml[s * pitch + 1] * fade;
+    const float share = ml[s * pitch + 1] * fade_to(ml[s * pitch], top) * scale;
 #pragma unroll
     for (int i = 0; i < kDims; ++i)
-      if (lane + i * kWave < c.head_dim) acc[i] = __builtin_fmaf(part[s * step + lane + i * kWave], fade, acc[i]);
+      if (lane + i * kWave < c.head_dim) acc[i] = __builtin_fmaf(part[s * step + lane + i * kWave], share, acc[i]);
   }
   const int64_t out = row * c.heads + head;
 #pragma unroll
   for (int i = 0; i < kDims; ++i)
     if (lane + i * kWave < c.head_dim)
-      store_o<DT>(c.out, out * c.head_dim + lane + i * kWave, sum == 0.0f ? 0.0f : acc[i] / sum);
-  if (lane == 0 && c.lse != nullptr) c.lse[out] = log_sum<DT>(top, sum);
+      store_o<DT>(c.out, out * c.head_dim + lane + i * kWave, acc[i]);
+  if (lane == 0 && c.lse != nullptr) c.lse[out] = log_sum(top, sum);
 }
 
 // The most places that a line's view has, by `longest` and what a table row has room for.

@@ -148,13 +148,13 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_rows_kernel(const Cach
             if ((seen >> t & 1u) == 0) s[nt][t][r] = -__builtin_inff();
         }
       }
-      float top = m[nt];
+      float top = -__builtin_inff();
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int t = 0; t < 8; ++t) top = fmaxf(top, s[nt][t][r]);
-      top = four_max(top);
-      const float ref = (top == -__builtin_inff() ? 0.0f : top) - kTop<DT>;
+      top = fmaxf(m[nt], four_max(top) - kTop<DT>);
+      const float ref = top == -__builtin_inff() ? 0.0f : top;
       if (ballot(top != m[nt]) != 0) {
         const float fade = fade_to(m[nt], top);
         l[nt] *= fade;
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_rows_kernel(const Cach
     float all_top = -__builtin_inff(), sum = 0.0f;
     for (int k = 0; k < kWavesPerBlock; ++k) all_top = fmaxf(all_top, ml_of[k][in_tile][0]);
     for (int k = 0; k < kWavesPerBlock; ++k) sum += ml_of[k][in_tile][1] * fade_to(ml_of[k][in_tile][0], all_top);
-    const float scale = count > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
     const TilePlace to = tile_place(a, tile, kv_head, in_tile);
     const int64_t slot = slot_row(a, line, part, in_tile);
     bool odd = !__builtin_isfinite(sum);
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_rows_kernel(const Cach
 #pragma unroll
       for (int k = 1; k < kWavesPerBlock; ++k) o += *reinterpret_cast<const f32x4*>(&exchange[k][row16 * kPitch + d]);
       odd |= !__builtin_isfinite(o.x + o.y + o.z + o.w);
-      if (count > 1) *reinterpret_cast<f32x4*>(slot_acc(a, slot) + d) = o;
+      if (count > 1) *reinterpret_cast<f32x4*>(slot_out(a, slot) + d) = o * scale;
       else store4<DT>(c.out, (to.row * c.heads + to.head) * HD + d, o * scale);
     }
     if constexpr (HD % 64 != 0) {
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_rows_kernel(const Cach
 #pragma unroll
         for (int k = 1; k < kWavesPerBlock; ++k) o += *reinterpret_cast<const f32x4*>(&exchange[k][row16 * kPitch + d]);
         odd |= !__builtin_isfinite(o.x + o.y + o.z + o.w);
-        if (count > 1) *reinterpret_cast<f32x4*>(slot_acc(a, slot) + d) = o;
+        if (count > 1) *reinterpret_cast<f32x4*>(slot_out(a, slot) + d) = o * scale;
         else store4<DT>(c.out, (to.row * c.heads + to.head) * HD + d, o * scale);
       }
     }
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_rows_kernel(const Cach
         slot_ml(a, slot)[0] = all_top;
         slot_ml(a, slot)[1] = sum;
       } else if (c.lse != nullptr) {
-        c.lse[to.row * c.heads + to.head] = log_sum<DT>(all_top, sum);
+        c.lse[to.row * c.heads + to.head] = log_sum(all_top, sum);
       }
     }
   }

@@ -183,8 +183,8 @@ __device__ __forceinline__ void store4(void* base, int64_t at, f32x4 o) {
 }
 
 // Rows whose sums are infinite or no numbers, once more without matrix products.  A weight of 0 times an infinite or
-// NaN value of a position that this row does not see, but another of the tile does, is what makes most of them; a
-// product cannot leave a value out.  rows: bits of the rows from first_row of the tile on; scratch: LDS that nothing else
+// NaN value of a position that this row does not see, but another of the tile does, is what makes most of them, since a
+// product cannot leave a value out; sums over bf16's largest values are the others.  rows: bits of the rows from first_row of the tile on; scratch: LDS that nothing else
 // uses any more.
 template <int DT, int HD>
 __device__ __forceinline__ void redo_rows(const CacheArgs& a, const View& w, const RowTile& tile, int32_t kv_head,
@@ -202,23 +202,38 @@ __device__ __forceinline__ void redo_rows(const CacheArgs& a, const View& w, con
     for (int d = lane; d < HD; d += kWave)
       q[d] = load_q<DT>(c.query, p.row * c.query_row_stride + p.head * c.query_head_stride + d);
     __builtin_amdgcn_wave_barrier();
-    float m, l, acc[(HD + kWave - 1) / kWave];
+    constexpr int kMine = (HD + kWave - 1) / kWave;
+    float m = 0.0f, l = 0.0f, out[kMine] = {};
     const RowSight sight = row_sight(a, w, tile.first, static_cast<int32_t>(p.row) - tile.first);
-    visit_row<DT, (HD + kWave - 1) / kWave * kWave>(a, w, tile.seq, sight, kv_head, q, lo, hi, kWave, visit, m, l, acc);
+    for (float lower = 0.0f;; lower = kLower) {
+      float top, sum, acc[kMine];
+      visit_row<DT, kMine * kWave>(a, w, tile.seq, sight, kv_head, q, lo, hi, kWave, lower, visit, top, sum, acc);
+      bool over = false;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        if (lower == 0.0f || !__builtin_isfinite(out[i])) out[i] = sum == 0.0f ? 0.0f : acc[i] / sum;
+        over |= !__builtin_isfinite(out[i]);
+      }
+      if (lower == 0.0f) {
+        m = top;
+        l = sum;
+      }
+      if (DT == kLinF16 || lower != 0.0f || !__builtin_isfinite(sum) || ballot(over) == 0) break;
+    }
     const int64_t slot = slot_row(a, line, part, in_tile);
 #pragma unroll
-    for (int i = 0; i < (HD + kWave - 1) / kWave; ++i) {
+    for (int i = 0; i < kMine; ++i) {
       const int d = lane + i * kWave;
       if (d >= HD) continue;
-      if (count > 1) slot_acc(a, slot)[d] = acc[i];
-      else store_o<DT>(c.out, (p.row * c.heads + p.head) * HD + d, l == 0.0f ? 0.0f : acc[i] / l);
+      if (count > 1) slot_out(a, slot)[d] = out[i];
+      else store_o<DT>(c.out, (p.row * c.heads + p.head) * HD + d, out[i]);
     }
     if (lane == 0) {
       if (count > 1) {
         slot_ml(a, slot)[0] = m;
         slot_ml(a, slot)[1] = l;
       } else if (c.lse != nullptr) {
-        c.lse[p.row * c.heads + p.head] = log_sum<DT>(m, l);
+        c.lse[p.row * c.heads + p.head] = log_sum(m, l);
       }
     }
     __builtin_amdgcn_wave_barrier();

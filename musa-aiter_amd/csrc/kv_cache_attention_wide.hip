@@ -210,7 +210,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) most = fmaxf(most, s[nt][j][r]);
-      top[nt] = four_max(most) * a.factor;
+      top[nt] = __builtin_fmaf(four_max(most), a.factor, -kTop<DT>);
     }
     if (ballot(top[0] > m[0] + kSlack<DT> || top[1] > m[1] + kSlack<DT>) != 0) {
 #pragma unroll
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
     u32x4 weight[2][2][2];  // half, row tile, summand
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt) {
-      const float ref = (m[nt] == -__builtin_inff() ? 0.0f : m[nt]) - kTop<DT>;
+      const float ref = m[nt] == -__builtin_inff() ? 0.0f : m[nt];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -267,14 +267,14 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
     const int32_t in_tile = kWaveRows * wave + 16 * nt + x;
     bool odd = !__builtin_isfinite(sum);
     if (in_tile < tile_rows) {
-      const float scale = count > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+      const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
       const TilePlace to = tile_place(a, tile, kv_head, in_tile);
       const int64_t slot = slot_row(a, line, part, in_tile);
 #pragma unroll
       for (int dt = 0; dt < kDimTiles; ++dt) {
         const f32x4 o = acc[nt][dt];
         odd |= !__builtin_isfinite(o.x + o.y + o.z + o.w);
-        if (count > 1) *reinterpret_cast<f32x4*>(slot_acc(a, slot) + 16 * dt + 4 * g) = o;
+        if (count > 1) *reinterpret_cast<f32x4*>(slot_out(a, slot) + 16 * dt + 4 * g) = o * scale;
         else store4<DT>(c.out, (to.row * c.heads + to.head) * HD + 16 * dt + 4 * g, o * scale);
       }
       if (g == 0) {
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void cache_wide_kernel(const Cach
           slot_ml(a, slot)[0] = m[nt];
           slot_ml(a, slot)[1] = sum;
         } else if (c.lse != nullptr) {
-          c.lse[to.row * c.heads + to.head] = log_sum<DT>(m[nt], sum);
+          c.lse[to.row * c.heads + to.head] = log_sum(m[nt], sum);
         }
       }
       if (odd) atomicOr(&odd_rows[wave], 1u << (16 * nt + x));

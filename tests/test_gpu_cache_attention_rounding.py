@@ -59,3 +59,67 @@ def test_a_row_keeps_its_bits_whatever_its_neighbours(dtype, hd, tree):
     assert not at_once(many)
     for case in (many, few):
         check_two_summands(case, call(case, softmax_scale=1.0)[0])
+
+
+SIZES = {"any": dict(lens=[40, 3000, 7], rows=[2, 3, 1], heads=2, kv_heads=1, hd=40),
+         "few": dict(lens=[40, 3000, 7], rows=[2, 3, 1], heads=8, hd=64),
+         "many": dict(lens=[1300, 640, 700], rows=[200, 64, 129], heads=12, kv_heads=3, hd=64, extra=60)}
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("size", [2.0 ** -126, 2.0 ** -122, 2.0 ** -110, 2.0 ** -98, 2.0 ** 120, 1.5 * 2.0 ** 127])
+@pytest.mark.parametrize("form", ["any", "few", "many"])
+def test_values_of_every_size(dtype, size, form):
+    """One value everywhere: every row's output is that value, be it the smallest normal one or next to the largest.
+
+    What is off: the output's rounding, the sums of weights and of products (tokens + 8) * 2^-24 each, a weight as two
+    summands 2^-16, and of a product below float32's smallest normal value 2^-126 what lies under its last place, 2^-149:
+    times the tokens, over a sum of weights of at least one.
+    """
+    case = one_product(Case(**SIZES[form], dtype=dtype, seed=33))
+    case.cache[1] = torch.full_like(case.cache[1], size)
+    if form == "many":
+        assert not at_once(case)
+    out, lse = call(case, softmax_scale=1.0)
+    _, want_lse, *_ = case.expect(1.0)
+    tokens = int(case.lens.max())
+    step = torch.finfo(case.dtype).eps / 2
+    bound = size * (step + 2.0 ** -16 + 2 * (tokens + 8) * 2.0 ** -24) + tokens * 2.0 ** -149
+    off = np.abs(out.double().cpu().numpy() - size)
+    assert off.max() <= bound, f"{off.max() / size} of {size}, bound {bound / size}"
+    assert np.abs(lse.double().cpu().numpy() - want_lse).max() <= 2.0 ** -19 + (tokens + 8) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("form", ["any", "few", "many"])
+def test_small_and_large_values_side_by_side(form):
+    """A dim next to float32's largest values does not cost another its small ones."""
+    case = one_product(Case(**SIZES[form], dtype="fp32" if form == "any" else "bf16", seed=34))
+    case.cache[1] = torch.full_like(case.cache[1], 2.0 ** -110)
+    case.cache[1][:, :, 5] = 1.5 * 2.0 ** 127
+    out, _ = call(case, softmax_scale=1.0)
+    want = torch.full_like(out, 2.0 ** -110)
+    want[:, :, 5] = 1.5 * 2.0 ** 127
+    step, tokens = torch.finfo(case.dtype).eps / 2, int(case.lens.max())
+    assert ((out.double() / want.double() - 1).abs() <= step + 2.0 ** -16 + 2 * (tokens + 8) * 2.0 ** -24 + tokens * 2.0 ** -39).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("form", ["few", "many"])
+@pytest.mark.parametrize("power", [22, 24, 26])
+def test_scores_with_coarse_steps(dtype, form, power):
+    """Scores of 2^power, where float32 has steps of up to 8 in base 2, all of a row the same: outputs are the means of
+    the values, and a logarithm is off by its own rounding and those of the product with the scale and of its ways between
+    the bases: 4 * 2^-24."""
+    case = Case(**SIZES[form], dtype=dtype, seed=35)
+    query, key = torch.zeros_like(case.query), torch.zeros_like(case.cache[0])
+    query[:, :, 3] = 64.0
+    key[:, :, 3] = 64.0
+    case.query, case.cache[0] = query, key
+    scale = 2.0 ** (power - 12)
+    out, lse = call(case, softmax_scale=scale)
+    want, want_lse, weight, *_ = case.expect(scale)
+    step, tokens = torch.finfo(case.dtype).eps / 2, int(case.lens.max())
+    off = np.abs(out.double().cpu().numpy() - want)
+    assert (off <= step * np.abs(want) + weight * (step * step + 2.0 ** -20 + (tokens + 8) * 2.0 ** -23)
+            + (2.0 ** -25 if case.dtype is torch.float16 else 0)).all()
+    assert (np.abs(lse.double().cpu().numpy() - want_lse) <= 2.0 ** -22 * np.abs(want_lse)).all()
