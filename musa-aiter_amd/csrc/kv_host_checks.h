@@ -36,6 +36,17 @@ inline bool packed_blocks(const at::Tensor& c) {
   return true;
 }
 
+// Whether the bytes from one tensor's first element to its last meet another's (their elements may lie apart for all that).
+inline bool spans_meet(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  auto end = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return reinterpret_cast<uint64_t>(t.data_ptr()) + (last + 1) * t.element_size();
+  };
+  return reinterpret_cast<uint64_t>(a.data_ptr()) < end(b) && reinterpret_cast<uint64_t>(b.data_ptr()) < end(a);
+}
+
 inline bool rows_packed(const at::Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }
 
 inline py::tuple not_taken() { return py::make_tuple(kNotTaken, py::none(), py::none()); }

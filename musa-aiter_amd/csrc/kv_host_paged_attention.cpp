@@ -96,6 +96,10 @@ py::tuple paged_attention_call(const py::handle& query_h, const py::handle& key_
   } else {
     const at::Tensor* o = plain(out_h, device);
     if (!o || o->sizes() != q->sizes() || o->scalar_type() != q->scalar_type() || !o->is_contiguous()) return not_taken();
+    for (const py::handle& h : {query_h, key_h, value_h, tables_h, lens_h, starts_h, masks_h}) {
+      const at::Tensor* read = plain(h, device);
+      if (read && spans_meet(*o, *read)) return not_taken();
+    }
     out = *o;
   }
   if (with_lse) lse = at::empty({c.rows, c.heads}, q->options().dtype(at::kFloat));

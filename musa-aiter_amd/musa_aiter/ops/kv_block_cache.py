@@ -67,11 +67,19 @@ def _packed_blocks(cache: torch.Tensor) -> bool:
     return True
 
 
+def _spans_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the bytes from one tensor's first element to its last meet another's."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    ends = [t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() for t in (a, b)]
+    return a.data_ptr() < ends[1] and b.data_ptr() < ends[0]
+
+
 class _Written:
-    """A tensor that a call writes: itself where the kernels take its layout, else a copy that goes back."""
+    """A tensor that a call writes: itself where the kernels can write there, else a copy that goes back."""
 
     def __init__(self, t: torch.Tensor, fits: bool):
-        self.user, self.t = t, t if fits else t.contiguous()
+        self.user, self.t = t, t if fits else t.clone(memory_format=torch.contiguous_format)
 
     def finish(self) -> None:
         if self.t is not self.user:

@@ -18,7 +18,7 @@ import math
 import torch
 
 from musa_aiter.ops import _hip
-from musa_aiter.ops.kv_block_cache import _index_rows, _overlaps, _packed_blocks, _Written
+from musa_aiter.ops.kv_block_cache import _index_rows, _overlaps, _packed_blocks, _spans_meet, _Written
 from musa_aiter.ops.kv_transfer import (
     _INDEX_DTYPES,
     _LIN_DTYPE,
@@ -81,6 +81,7 @@ class _Rows:
         self.rows, self.heads, self.kv_heads, self.batch, self.room = rows, heads, nh, batch, width * bs
         self.query, self.device = query, device
         self._caches, self._indices = caches, (block_tables, seq_lens, query_starts)
+        self.read = (query, *caches, *indices)
         self._shape = (rows, batch, heads, nh, hd, bs, nb, width)
         self._scale, self._window, self._sinks = scale, min(int(window or 0), _MAX_ROOM), min(int(sinks), _MAX_ROOM) if window else 0
         self._longest = width * bs if max_seq_len is None else min(int(max_seq_len), 1 << 62)
@@ -118,7 +119,8 @@ def _attention(op: str, rows: _Rows, masks: torch.Tensor | None, out: torch.Tens
         raise ValueError(f"{op}: out is written and must not be expanded")
     _require_rocm(op, query)
     result = torch.empty(query.shape, dtype=query.dtype, device=device) if out is None else out
-    target = _Written(result, result.is_contiguous())
+    read = rows.read if masks is None else (*rows.read, masks)
+    target = _Written(result, result.is_contiguous() and (out is None or not any(_spans_meet(out, t) for t in read)))
     lse = torch.empty((rows.rows, rows.heads), dtype=torch.float32, device=device) if return_lse else None
     _hip.paged_attention(op=op, out=target.t, lse=lse, masks=masks, fill_rows=out is None, **rows.call())
     target.finish()
@@ -151,7 +153,8 @@ def kv_paged_attention(
     A position without a table entry, or whose entry lies outside the cache, is not seen.  A row that sees nothing
     gives zeros (``lse`` -inf).  Rows of ``query`` that belong to no sequence (a padded batch) are left as they are in
     ``out``, and are zeros in a new tensor; their ``lse`` is -inf either way.  What positions that a row does not see
-    hold does not reach it, infinities and NaN included.
+    hold does not reach it, infinities and NaN included.  An ``out`` that shares memory with an argument, ``query``
+    itself among them, is computed apart and copied.
 
     ``max_seq_len``, an upper bound of ``seq_lens`` that the caller knows, only decides how the work is cut; by
     default it is what ``block_tables`` has room for.  Returns the output, in ``query``'s type, and with
