@@ -147,10 +147,13 @@ __device__ __forceinline__ Span part_places(const CacheArgs& a, int32_t length, 
   return {lo, s + 1 < count ? lo + a.part : length};
 }
 
-// Workspace: (m, l) of every part's rows, their outputs of head_dim values each, and a Line for each line.
+// Workspace: (m, l) of every part's rows, their outputs of head_dim values each (from a multiple of 16 bytes on: the
+// matrix-core forms write 16 at a time), and a Line for each line.
 struct Line {
   int32_t parts, first, count, base;  // parts 0: no rows
 };
+
+__host__ __device__ __forceinline__ int64_t ml_floats(int64_t slots) { return (2 * slots + 3) & ~int64_t{3}; }
 
 __device__ __forceinline__ int64_t slot_row(const CacheArgs& a, int64_t line, int32_t s, int32_t row) {
   return (line * a.parts + s) * a.slot_rows + row;
@@ -159,7 +162,7 @@ __device__ __forceinline__ float* slot_ml(const CacheArgs& a, int64_t at) {
   return static_cast<float*>(a.r.c.workspace) + 2 * at;
 }
 __device__ __forceinline__ float* slot_out(const CacheArgs& a, int64_t at) {
-  return static_cast<float*>(a.r.c.workspace) + 2 * a.lines * a.parts * a.slot_rows + at * a.r.hd;
+  return static_cast<float*>(a.r.c.workspace) + ml_floats(a.lines * a.parts * a.slot_rows) + at * a.r.hd;
 }
 __device__ __forceinline__ Line* line_of(const CacheArgs& a, int64_t line) {
   return reinterpret_cast<Line*>(slot_out(a, a.lines * a.parts * a.slot_rows)) + line;

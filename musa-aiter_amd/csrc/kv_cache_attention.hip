@@ -271,7 +271,8 @@ Plan make_plan(const CacheAttnCall& c) {
 
 int64_t plan_workspace(const CacheAttnCall& c, const Plan& p) {
   if (p.parts <= 1) return 0;
-  return p.lines * p.parts * p.slot_rows * (2 + c.head_dim) * 4 + p.lines * static_cast<int64_t>(sizeof(Line));
+  const int64_t slots = p.lines * p.parts * p.slot_rows;
+  return (ml_floats(slots) + slots * c.head_dim) * 4 + p.lines * static_cast<int64_t>(sizeof(Line));
 }
 
 constexpr int64_t kFewParts = 8;
