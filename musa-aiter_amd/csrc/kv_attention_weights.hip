@@ -10,6 +10,19 @@ namespace kvhip {
 namespace catt {
 namespace {
 
+// Rows [first, end) of a sequence that can see one of the positions from .. last, places v0 and up: those in front of the
+// first position see none of them, and with a window those do not whose window begins behind the last, but where some of
+// them are first tokens.
+struct RowSpan {
+  int32_t first, end;
+};
+
+__device__ __forceinline__ RowSpan rows_that_see(const CacheArgs& a, const View& w, int32_t count, int32_t v0,
+                                                 int32_t from, int32_t last) {
+  const bool past = a.window > 0 && v0 >= w.front && from >= a.sinks;
+  return {min(max(from - w.before, 0), count), past ? min(max(last + a.window - w.before, 0), count) : count};
+}
+
 // ----- any shape and type: a thread per token, one row and head after the other --------------------
 template <int DT>
 __global__ __launch_bounds__(kBlockThreads) void weights_any_kernel(const CacheArgs a) {
@@ -30,8 +43,9 @@ __global__ __launch_bounds__(kBlockThreads) void weights_any_kernel(const CacheA
       const int64_t blk = position_block(a, seq, token);
       if (blk >= 0) k = blk * (c.cache_block_stride[0] / kElt) + head * hd * bs + token % bs;
     }
+    const RowSpan span = rows_that_see(a, w, count, base, base < w.front ? 0 : base + w.gap, position(w, base + kBlockThreads - 1));
     float sum = 0.0f;
-    for (int32_t x = 0; x < count * a.r.group; ++x) {
+    for (int32_t x = span.first * a.r.group; x < span.end * a.r.group; ++x) {
       const int32_t i = x / a.r.group;
       const int64_t row = rows.first + i, hq = head * a.r.group + x % a.r.group;
       __syncthreads();
@@ -123,9 +137,6 @@ __global__ __launch_bounds__(WAVES * kWave, HD <= 128 ? 2 : 1) void weights_tile
 #pragma unroll
         for (int t = 0; t < 8; ++t) keys[ks][t] = token_dims(raw[ks], t);
     }
-    uint32_t bits[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) bits[r] = __shfl(unit.bits, 4 * g + r);
     const bool whole = ballot(unit.bits != 0xFFu) == 0;
     // Positions of the tile: none of them is past last, none but first ones in front of from.
     const int32_t from = v0 < w.front ? 0 : v0 + w.gap, last = position(w, v0 + kTilePlaces - 1);
@@ -134,11 +145,9 @@ __global__ __launch_bounds__(WAVES * kWave, HD <= 128 ? 2 : 1) void weights_tile
     for (int t = 0; t < 8; ++t) sum[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
     const int32_t step = many ? 16 * WAVES : 16;
-    // Rows in front of the tile's first position see none of it.
-    int32_t at0 = many ? 16 * wave : 0;
-    const int32_t skip = max(from - w.before, 0);
-    if (skip >= count || v0 >= w.length) at0 = rows;
-    else at0 += skip * group / step * step;
+    const RowSpan span = rows_that_see(a, w, count, v0, from, last);
+    const int32_t end = __builtin_amdgcn_readfirstlane(v0 < w.length ? span.end * group : 0);
+    int32_t at0 = __builtin_amdgcn_readfirstlane((many ? 16 * wave : 0) + span.first * group / step * step);
     // The next rows' queries are on their way while these are worked on.
     u32x4 next16[kSteps];
     float next_lse = 0.0f;
@@ -150,12 +159,12 @@ __global__ __launch_bounds__(WAVES * kWave, HD <= 128 ? 2 : 1) void weights_tile
 #pragma unroll
       for (int ks = 0; ks < kSteps; ++ks) next16[ks] = ld16_cached(q + 64 * ks);
     };
-    if (at0 < rows) fetch(at0);
-    for (; at0 < rows; at0 += step) {
+    if (at0 < end) fetch(at0);
+    for (; at0 < end; at0 += step) {
       // e^(score - lse) is 2^(score * factor - less) times what the rounding of less leaves: for logarithms of thousands
       // it is off by 2^-11 and more.  It goes into the sums as their factor, at no instruction a score.
-      const float lse = next_lse, less = lse * a.lse_factor;
-      const float rest = __builtin_isfinite(less) ? __builtin_fmaf(lse, a.lse_rest, __builtin_fmaf(lse, a.lse_factor, -less)) : 0.0f;
+      const float lse = next_lse, less = lse * -a.lse_factor;
+      const float rest = __builtin_isfinite(less) ? __builtin_fmaf(lse, a.lse_rest, __builtin_fmaf(lse, a.lse_factor, less)) : 0.0f;
       const float give = __builtin_amdgcn_exp2f(-rest);
       u32x4 rows16[kSteps];
 #pragma unroll
@@ -171,7 +180,7 @@ __global__ __launch_bounds__(WAVES * kWave, HD <= 128 ? 2 : 1) void weights_tile
         const RowSight sight{w.before + at / group, nullptr};
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          seen[r] = gives ? bits[r] & row_bits(a, w, sight, position(w, v0 + 8 * (4 * g + r))) : 0;
+          seen[r] = (gives ? row_bits(a, w, sight, position(w, v0 + 8 * (4 * g + r))) : 0) & __shfl(unit.bits, 4 * g + r);
       }
 #pragma unroll
       for (int t0 = 0; t0 < 8; t0 += kAtOnce) {
@@ -185,7 +194,7 @@ __global__ __launch_bounds__(WAVES * kWave, HD <= 128 ? 2 : 1) void weights_tile
 #pragma unroll
         for (int t = 0; t < kAtOnce; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], a.factor, -less));
+          for (int r = 0; r < 4; ++r) s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], a.factor, less));
         if (!plain) {
 #pragma unroll
           for (int t = 0; t < kAtOnce; ++t)
