@@ -4,6 +4,7 @@
 #include <c10/util/Exception.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cstdint>
 
 namespace kv_host {
@@ -45,6 +46,26 @@ inline bool spans_meet(const at::Tensor& a, const at::Tensor& b) {
     return reinterpret_cast<uint64_t>(t.data_ptr()) + (last + 1) * t.element_size();
   };
   return reinterpret_cast<uint64_t>(a.data_ptr()) < end(b) && reinterpret_cast<uint64_t>(b.data_ptr()) < end(a);
+}
+
+// Whether a block of one of two caches of the same shape shares bytes with one of the other ([blocks, ..] or [layers,
+// blocks, ..], each block packed; K and V may lie between each other in one buffer).
+inline bool blocks_meet(const at::Tensor& a, const at::Tensor& b) {
+  if (!spans_meet(a, b)) return false;
+  const int64_t n = a.dim(), elt = a.element_size();
+  const int64_t packed = a.size(n - 3) * a.size(n - 2) * a.size(n - 1) * elt;
+  const int64_t apart = static_cast<const char*>(b.data_ptr()) - static_cast<const char*>(a.data_ptr());
+  if (a.strides().slice(0, n - 3) != b.strides().slice(0, n - 3)) return true;  // not looked at further
+  const int64_t layers = n == 5 ? a.size(0) : 1, layer = n == 5 ? a.stride(0) * elt : 0;
+  const int64_t last = a.size(n - 4) - 1, block = last > 0 ? a.stride(n - 4) * elt : 1;
+  for (int64_t i = 1 - layers; i < layers; ++i) {
+    const int64_t off = apart + i * layer, near = -off / block;
+    for (int64_t j = near - 1; j <= near + 1; ++j) {
+      const int64_t at = off + std::clamp(j, -last, last) * block;
+      if (at > -packed && at < packed) return true;
+    }
+  }
+  return false;
 }
 
 inline bool rows_packed(const at::Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }

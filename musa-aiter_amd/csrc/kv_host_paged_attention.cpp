@@ -160,7 +160,7 @@ py::tuple evict_call(const py::handle& key_h, const py::handle& value_h, const p
   const int64_t layers = lead ? kc->size(0) : 1, nb = kc->size(lead), nh = kc->size(lead + 1), hd = kc->size(lead + 2),
                 bs = kc->size(lead + 3), batch = tables->size(0), width = tables->size(1), elt = kc->element_size();
   if ((elt != 1 && elt != 2 && elt != 4) || batch < 1 || kc->data_ptr() == vc->data_ptr() || lens->size(0) != batch || keep->size(0) != batch ||
-      !packed_blocks(*kc) || !packed_blocks(*vc) || !index_kind(tables->scalar_type()) ||
+      !packed_blocks(*kc) || !packed_blocks(*vc) || blocks_meet(*kc, *vc) || !index_kind(tables->scalar_type()) ||
       !index_kind(lens->scalar_type()) || !index_kind(keep->scalar_type()) || !rows_packed(*tables) ||
       !rows_packed(*lens) || !rows_packed(*keep) || weights->scalar_type() != at::kFloat ||
       (lead && weights->size(0) != layers) || weights->size(lead) != batch || weights->size(lead + 1) != nh ||

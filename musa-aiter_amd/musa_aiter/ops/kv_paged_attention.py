@@ -32,6 +32,25 @@ _MAX_HEAD_DIM = 512
 _MAX_ROOM = 1 << 29
 
 
+def _blocks_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether a packed block of one of two caches of the same shape shares bytes with one of the other."""
+    if not _spans_meet(a, b):
+        return False
+    if a.stride()[:-3] != b.stride()[:-3]:
+        return True  # not looked at further
+    size = a.element_size()
+    packed, apart = a[(0,) * (a.dim() - 3)].numel() * size, b.data_ptr() - a.data_ptr()
+    layers, layer = (a.shape[0], a.stride(0) * size) if a.dim() == 5 else (1, 0)
+    last = a.shape[-4] - 1
+    block = a.stride(-4) * size if last else 1
+    for i in range(1 - layers, layers):
+        off = apart + i * layer
+        near = -off // block
+        if any(abs(off + min(max(j, -last), last) * block) < packed for j in (near, near + 1)):
+            return True
+    return False
+
+
 class _Rows:
     """The checked arguments that the three operators on query rows share."""
 
@@ -337,6 +356,8 @@ def kv_evict_paged_tokens(
         raise ValueError(f"{op}: the blocks of the caches are written and must be contiguous")
     if key_cache.data_ptr() == value_cache.data_ptr():
         raise ValueError(f"{op}: key_cache and value_cache are moved each on its own and must not be one tensor")
+    if _blocks_meet(key_cache, value_cache):
+        raise ValueError(f"{op}: key_cache and value_cache are moved each on its own and must not share memory")
     if weights.numel() and _overlaps(weights):
         raise ValueError(f"{op}: weights are written and must not be expanded")
     if sinks < 0 or recent < 0:
