@@ -31,8 +31,9 @@ extern "C" {
  *
  * musa_aiter_hip_paged_attention: out (packed, of query's type) and lse float32 [rows, heads] (or NULL).  A row that
  * sees nothing gives 0 and lse -inf.  Rows of no sequence are zeroed in out with fill_rows, else left as they are
- * there; their lse is -inf.  `longest` is an upper bound of lens; only how the work is cut depends on it.  workspace
- * holds musa_aiter_hip_paged_attention_workspace bytes (NULL where that is 0).
+ * there; their lse is -inf.  out and lse share no memory with what the call reads.  `longest` is an upper bound of
+ * lens; only how the work is cut depends on it.  workspace holds musa_aiter_hip_paged_attention_workspace bytes (NULL
+ * where that is 0).
  *
  * musa_aiter_hip_attention_weights (masks NULL; cache[1], out and the workspace are not used): adds to
  * weights[b, kv head, j] the sum of e^(score - lse) over the rows and heads of the kv head that see position
@@ -68,6 +69,7 @@ int64_t musa_aiter_hip_paged_attention_workspace(const musa_aiter_hip_paged_atte
 int musa_aiter_hip_attention_weights(const musa_aiter_hip_paged_attention_call* call, void* stream);
 
 /* ---- Eviction ------------------------------------------------------------------------------------
+ * The two caches share no memory (their blocks may lie between each other).
  * cache [layers, num_blocks, kv_heads, head_dim, block_size] of 1-, 2- or 4-byte elements (a block's packed, strides in
  * bytes), weights float32 [layers, batch, kv_heads, weight_tokens] (strides in elements, the last extent packed),
  * tables [batch, max_blocks], lens and keep [batch], refs [num_blocks] or NULL.

@@ -74,8 +74,9 @@ __global__ __launch_bounds__(kBlockThreads) void weights_any_kernel(const CacheA
 // query are an operand as they are.
 // With few rows the waves of a workgroup take different positions (bound by the read of K: all of a wave's 32 loads are
 // on their way at once), with many the same positions and a quarter of the rows each (bound by 32 exponentials of a
-// quarter of the full rate next to 32 products).  16 decode rows of 300 to 4097 tokens: 20 us, 3.1 TB/s; chunks of 600 and
-// 1024 rows over up to 6001 tokens (32 heads, 8 in the cache, 128 dims): 110 us, 577 TFLOP/s.
+// quarter of the full rate next to 32 products).  16 decode rows of 430 to 4097 tokens: 20 us, 3.1 TB/s; chunks of 795 and
+// 1024 rows over 3120 and 6001 tokens (32 heads, 8 in the cache, 128 dims): 116 us, 550 TFLOP/s; 4096 rows over as many
+// tokens with a window of 64: 21 us, of 256: 30, without 144.
 constexpr int kAtOnce = 4;     // tokens of the units whose scores are held at a time
 constexpr int64_t kCus = 256;
 // Row tiles of a sequence from which on the waves share positions: each of the four has one.
@@ -273,8 +274,8 @@ hipError_t launch(const CacheAttnCall& c, CacheArgs a, hipStream_t stream) {
   int64_t groups = (longest + share - 1) / share;
   groups = groups < 1 ? 1 : groups < 4096 ? groups : 4096;
   const dim3 grid(groups, c.batch, c.kv_heads);
-  // Positions for less than a workgroup per CU: eight waves share their rows (208 workgroups, 573 row tiles: 94 us,
-  // with four waves 124).
+  // Positions for less than a workgroup per CU: eight waves share their rows (208 workgroups, 573 row tiles: 90 us,
+  // with four waves 119).
   if (a.parts > 1 && groups * c.batch * c.kv_heads <= kCus) a.parts = 8;
   if constexpr (DT != kLinF32)
     if (tiles) return launch_tiles<DT>(a, grid, stream);

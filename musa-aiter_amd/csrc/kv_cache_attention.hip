@@ -219,14 +219,14 @@ struct Plan {
   int64_t size, lines, parts, part, slot_rows, tiles;
 };
 
-// Few rows: parts of whole turns of a workgroup, as many as make kRowsGroups workgroups (48 decode rows of 256 to 8192
+// Few rows: parts of whole turns of a workgroup, as many as make kRowsGroups workgroups (48 decode rows of 295 to 8192
 // tokens, us: 768 193, 1600 180, 2048 178 to 188, 4096 182, 8192 187; 16 rows of 2048 visible ones 55, then 48).
 constexpr int64_t kTurnPlaces = kTilePlaces * kWavesPerBlock;
 constexpr int64_t kRowsGroups = 2048;
 constexpr int64_t kFewRows = 32;
 constexpr int64_t kAtOnce = 512;  // two workgroups a CU
-// Many rows (16 trees of 33 to 64 tokens over 500 to 4001, us: 320 129, 640 102, 1024 88, 1536 109, 2048 113; two chunks
-// of 1500 and 2048 rows, whose tiles alone make 904: uncut 329, in two parts 399).
+// Many rows (16 trees of 34 to 64 tokens over 620 to 4001, us: 320 157, 640 124, 1024 103, 1536 126, 2048 131; two chunks
+// of 1753 and 2048 rows, whose tiles alone make 960: uncut 432, in two parts 504).
 constexpr int64_t kWidePlaces = 512;
 constexpr int64_t kWideGroups = 1024;
 
@@ -248,7 +248,7 @@ Plan make_plan(const CacheAttnCall& c) {
     const int64_t group = c.heads / c.kv_heads;
     const int64_t seq_rows = (c.starts == nullptr || c.batch == 0 ? 1 : (c.rows + c.batch - 1) / c.batch) * group;
     // Few rows, and calls so small that all of their tiles of 16 rows run at once: those take the shortest way through a
-    // line (three trees of 7 to 13 tokens over 400: 12 us, in wide tiles 23).
+    // line (three trees of 7 to 13 tokens over 400: 12 us, in wide tiles 28).
     const int64_t turns = (most_places(c, 16) + kTurnPlaces - 1) / kTurnPlaces;
     const bool all_at_once = (c.rows * group / 16 + c.batch) * c.kv_heads * turns <= kAtOnce;
     const bool wide = seq_rows > kFewRows && c.head_dim <= 128 && fuses_scale(c) && !all_at_once;

@@ -6,7 +6,7 @@
 // line in order, with a step's loads ahead of its stores, can move it in place; lines and head dimensions are independent
 // of each other.
 //
-// 8 sequences of 900 to 6000 tokens to 1024 in 8 layers (8 heads of 128 dims, bf16): decisions 33 us, moves 280 (4.2 TB/s
+// 8 sequences of 1520 to 6000 tokens to 1024 in 8 layers (8 heads of 128 dims, bf16): decisions 33 us, moves 279 (4.2 TB/s
 // of the pages read and written).  One sequence of 40001 tokens to 8000 in two layers: 72 (16 workgroups) and 118.
 #include "kv_cache_attention.h"
 
@@ -442,8 +442,8 @@ void launch_moves(const EvictArgs& a, hipStream_t stream) {
   const EvictCall& c = a.c;
   MoveShape shape{};
   if (move_fits(c, shape)) {
-    // Few waves: half the dims each, twice the tokens a step (40001 tokens of 16 lines, 16 bits: 137 us, against 215).
-    // With many the longer pieces of memory are read a little faster (512 lines 280, against 305).
+    // Few waves: half the dims each, twice the tokens a step (40001 tokens of 16 lines, 16 bits: 119 us, against 186).
+    // With many the longer pieces of memory are read a little faster (512 lines 279, against 295).
     const int64_t waves = a.lines * ((c.head_dim + kDimsOf<ELT, false> - 1) / kDimsOf<ELT, false>);
     if (waves < kFewWaves) launch_move<ELT, true>(a, shape, stream);
     else launch_move<ELT, false>(a, shape, stream);
