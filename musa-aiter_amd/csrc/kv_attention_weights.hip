@@ -57,7 +57,8 @@ __global__ __launch_bounds__(kBlockThreads) void weights_any_kernel(const CacheA
       float dot = 0.0f;
       for (int64_t d = 0; d < hd; ++d) dot = __builtin_fmaf(q[d], load_q<DT>(c.cache[0], k + d * bs), dot);
       // The difference first: it is small where a weight is large, and its product then loses nothing.
-      const float less = __builtin_fmaf(dot, a.scale_rest, __builtin_fmaf(dot, a.scale, -lse));
+      float less = __builtin_fmaf(dot, a.scale, -lse);
+      if (__builtin_isfinite(less)) less = __builtin_fmaf(dot, a.scale_rest, less);
       sum += __builtin_amdgcn_exp2f(less * kLog2e);
     }
     if (k >= 0) {

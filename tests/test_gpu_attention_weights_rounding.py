@@ -63,3 +63,22 @@ def test_gathered_weights_of_logarithms_that_are_none(lse, rows):
     got = gather(case, given, None)
     assert np.array_equal(got[1:], want[1:])
     assert np.isnan(got[0, :, 0]).all() if np.isnan(lse) else np.isfinite(got).all() and (got[0] <= want[0]).all()
+
+
+@pytest.mark.parametrize("dtype,hd", [("fp32", 64), ("bf16", 40), ("bf16", 64), ("fp16", 128)])
+@pytest.mark.parametrize("scale", [0.125, 40 ** -0.5, -0.3])
+@pytest.mark.parametrize("rows", [[1, 3, 2], [40, 9, 70]])
+def test_gathered_weights_of_infinite_scores(dtype, hd, scale, rows):
+    """Keys that make a score -inf gather nothing; one of +inf makes its position's sum infinite, and no other."""
+    case = Case(lens=[50, 301, 129], rows=rows, heads=8, kv_heads=2, hd=hd, dtype=dtype, seed=38)
+    case.query[:, :, 3] = 1.0
+    lse = case.expect(scale)[1].astype(np.float32)
+    want = gather(case, lse, scale)
+    sign = 1.0 if scale > 0 else -1.0
+    for at, value in ((7, -np.inf), (40, np.inf)):
+        case.cache[0][case.tables[0, at // 16], 1, 3, at % 16] = sign * value
+    got = gather(case, lse, scale)
+    assert got[0, 1, 7] == 0.0 and np.isposinf(got[0, 1, 40])
+    same = np.ones(want.shape, dtype=bool)
+    same[0, 1, [7, 40]] = False
+    assert np.array_equal(got[same], want[same])
