@@ -55,7 +55,8 @@ inline bool blocks_meet(const at::Tensor& a, const at::Tensor& b) {
   const int64_t n = a.dim(), elt = a.element_size();
   const int64_t packed = a.size(n - 3) * a.size(n - 2) * a.size(n - 1) * elt;
   const int64_t apart = static_cast<const char*>(b.data_ptr()) - static_cast<const char*>(a.data_ptr());
-  if (a.strides().slice(0, n - 3) != b.strides().slice(0, n - 3)) return true;  // not looked at further
+  for (int64_t i = 0; i < n - 3; ++i)
+    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return true;  // not looked at further
   const int64_t layers = n == 5 ? a.size(0) : 1, layer = n == 5 ? a.stride(0) * elt : 0;
   const int64_t last = a.size(n - 4) - 1, block = last > 0 ? a.stride(n - 4) * elt : 1;
   for (int64_t i = 1 - layers; i < layers; ++i) {

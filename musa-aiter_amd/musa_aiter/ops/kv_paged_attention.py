@@ -36,7 +36,7 @@ def _blocks_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether a packed block of one of two caches of the same shape shares bytes with one of the other."""
     if not _spans_meet(a, b):
         return False
-    if a.stride()[:-3] != b.stride()[:-3]:
+    if any(n > 1 and s != t for n, s, t in zip(a.shape[:-3], a.stride(), b.stride())):
         return True  # not looked at further
     size = a.element_size()
     packed, apart = a[(0,) * (a.dim() - 3)].numel() * size, b.data_ptr() - a.data_ptr()

@@ -60,3 +60,15 @@ def test_against_every_pair_of_blocks():
         starts = [i * layer + j * block for i in range(L) for j in range(NB)]
         want = any(abs(apart + x - y) < BLOCK for x in starts for y in starts)
         assert _blocks_meet(*pair) is want and _blocks_meet(*reversed(pair)) is want, (apart, layer, block)
+
+
+def test_strides_of_extents_of_one_do_not_count():
+    base = torch.zeros(2 * NB * BLOCK + 2 * BLOCK)
+    shape = (1, NB, H, D, BS)
+    key = base.as_strided(shape, (7, 2 * BLOCK, D * BS, BS, 1), 0)
+    value = base.as_strided(shape, (2 * NB * BLOCK, 2 * BLOCK, D * BS, BS, 1), BLOCK)
+    assert not _blocks_meet(key, value)
+    assert _blocks_meet(key, base.as_strided(shape, (9, 2 * BLOCK, D * BS, BS, 1), 2 * BLOCK))
+    one = torch.zeros(1, 2, NB, H, D, BS)
+    with pytest.raises(RuntimeError, match="ROCm"):
+        evict(one[:, 0, ::2], one[:, 1, ::2])
