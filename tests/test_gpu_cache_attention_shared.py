@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+import musa_aiter
 from tests.test_gpu_cache_attention import DEV, Case, call
 
 pytestmark = pytest.mark.gpu
@@ -53,9 +54,37 @@ def test_out_in_the_cache():
     case = Case(lens=[40, 300, 7], rows=[2, 3, 1], heads=8, kv_heads=2, hd=64, seed=43)
     want, _ = call(case)
     query, key, value, tables, lens = case.args()
-    import musa_aiter
-
     block = int(tables[1, 3])
     out = value.view(-1)[block * 2 * 64 * 16:][:query.numel()].view(query.shape)
     got = musa_aiter.kv_paged_attention(query, key, value, tables, lens, **case.sight(), out=out)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("form", ["few", "many"])
+def test_captured_in_place(form):
+    """A captured step that writes over its query, replayed with eager work in between."""
+    case = Case(**FORMS[form], seed=44)
+    want, _ = call(case)
+    source, query = case.query.to(DEV), torch.empty(case.query.shape, dtype=case.dtype, device=DEV)
+    _, *caches = case.args()
+    case.query = query
+
+    def step():
+        query.copy_(source)
+        return musa_aiter.kv_paged_attention(query, *caches, **case.sight(), out=query)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph, starts = torch.cuda.CUDAGraph(), case.index_of(case.starts)
+    case.sight = lambda: {"query_starts": starts, "window": None, "sinks": 0}
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(3):
+        query.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(query, want)
+        assert torch.equal(step(), want)
