@@ -10,9 +10,9 @@ namespace kvhip {
 namespace catt {
 namespace {
 
-// Rows [first, end) of a sequence that can see one of the positions from .. last, places v0 and up: those in front of the
-// first position see none of them, and with a window those do not whose window begins behind the last, but where some of
-// them are first tokens.
+// Rows [first, end) of a sequence that can see one of the positions from .. last (places v0 and up).  Those in front of
+// the first position see none of them; with a window, and no first tokens among them, those do not either whose window
+// begins behind the last.
 struct RowSpan {
   int32_t first, end;
 };
@@ -43,7 +43,8 @@ __global__ __launch_bounds__(kBlockThreads) void weights_any_kernel(const CacheA
       const int64_t blk = position_block(a, seq, token);
       if (blk >= 0) k = blk * (c.cache_block_stride[0] / kElt) + head * hd * bs + token % bs;
     }
-    const RowSpan span = rows_that_see(a, w, count, base, base < w.front ? 0 : base + w.gap, position(w, base + kBlockThreads - 1));
+    const RowSpan span = rows_that_see(a, w, count, base, base < w.front ? 0 : base + w.gap,
+                                       position(w, base + kBlockThreads - 1));
     float sum = 0.0f;
     for (int32_t x = span.first * a.r.group; x < span.end * a.r.group; ++x) {
       const int32_t i = x / a.r.group;
@@ -163,10 +164,11 @@ __global__ __launch_bounds__(WAVES * kWave, HD <= 128 ? 2 : 1) void weights_tile
     };
     if (at0 < end) fetch(at0);
     for (; at0 < end; at0 += step) {
-      // e^(score - lse) is 2^(score * factor - less) times what the rounding of less leaves: for logarithms of thousands
-      // it is off by 2^-11 and more.  It goes into the sums as their factor, at no instruction a score.
+      // e^(score - lse) is 2^(score * factor + less) times what the rounding of less leaves, which is 2^-11 and more for
+      // logarithms of thousands.  That goes into the sums as their factor, at no instruction a score.
       const float lse = next_lse, less = lse * -a.lse_factor;
-      const float rest = __builtin_isfinite(less) ? __builtin_fmaf(lse, a.lse_rest, __builtin_fmaf(lse, a.lse_factor, less)) : 0.0f;
+      const float past = __builtin_fmaf(lse, a.lse_rest, __builtin_fmaf(lse, a.lse_factor, less));
+      const float rest = __builtin_isfinite(less) ? past : 0.0f;
       const float give = __builtin_amdgcn_exp2f(-rest);
       u32x4 rows16[kSteps];
 #pragma unroll

@@ -184,8 +184,8 @@ __device__ __forceinline__ void store4(void* base, int64_t at, f32x4 o) {
 
 // Rows whose sums are infinite or no numbers, once more without matrix products.  A weight of 0 times an infinite or
 // NaN value of a position that this row does not see, but another of the tile does, is what makes most of them, since a
-// product cannot leave a value out; sums over bf16's largest values are the others.  rows: bits of the rows from first_row of the tile on; scratch: LDS that nothing else
-// uses any more.
+// product cannot leave a value out; sums over bf16's largest values are the others.  rows: bits of the rows from
+// first_row of the tile on; scratch: LDS that nothing else uses any more.
 template <int DT, int HD>
 __device__ __forceinline__ void redo_rows(const CacheArgs& a, const View& w, const RowTile& tile, int32_t kv_head,
                                           int64_t line, int32_t part, int32_t count, int32_t lo, int32_t hi,
