@@ -14,8 +14,8 @@
 //   * s(4 g + r) = 8 (g / 2) + 2 r + g % 2: the units of lanes g = 0, 1 (and 2, 3) are the halves of one block.
 // The path is bound by the reads of K and V; the products of 16 rows take a twentieth of their time, and so weights may go
 // in as two summands of the caches' type (a rounding of 2^-16 and less), which costs half as many products again.  48
-// decode rows of 295 to 8192 tokens (32 heads, 8 of them in the cache, 128 dims, bf16): 178 to 188 us with the join, 4.3
-// to 4.6 TB/s.
+// decode rows of 295 to 8192 tokens (32 heads, 8 of them in the cache, 128 dims, bf16): 176 to 191 us with the join, by
+// where the caches lie, 4.2 to 4.6 TB/s.
 // With each group of loads asked for where it is used it was 326.
 #include "kv_cache_attention_tiles.h"
 
